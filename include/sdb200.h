@@ -66,7 +66,8 @@ void* sdb200_get_stream(void);
 /* Synchronises the stream, then reads the device error word that kernels set when a
  * bounded wait expires (0 = none) without clearing it. Bits: 1-16 GEMM / convolution
  * pipeline waits, 32 attention pipeline, 64 tensor-parallel barrier (a peer rank did not
- * arrive). */
+ * arrive), 128 an index or length read on the device (row_adapter, pos, q_begin, ...) was
+ * out of range and its row or sequence was skipped. */
 int sdb200_device_error_word(int* out);
 
 /* ---- memory (backend_cuda.h:29-36) --------------------------------------------- */
@@ -83,7 +84,8 @@ int sdb200_copy(void* dst, const void* src, size_t bytes);
 /* backend_cuda.h:35 zero() */
 int sdb200_zero(void* dst, size_t bytes);
 /* backend_cuda.h:36 synchronize(); also reports an expired device wait as
- * SDB200_ERR_DEVICE_WAIT (and clears the error word). */
+ * SDB200_ERR_DEVICE_WAIT, and an index out of range (bit 128 alone) as
+ * SDB200_ERR_INVALID_ARG, and clears the error word. */
 int sdb200_synchronize(void);
 
 /* ---- GEMM (the hot path) ------------------------------------------------------- */
@@ -210,6 +212,68 @@ int sdb200_pack_heads_f16(const float* x, void* y, int64_t rows, int heads, int6
  * operands for head dims <= 128, tf32 GEMMs above), 1 = exact fp32 streaming kernel.
  * Applies to later sdb200_attention calls of this process. */
 int sdb200_set_attention_path(int path);
+
+/* ---- several requests at once ----------------------------------------------------- */
+/* Extensions: one transformer layer for the packed tokens of many requests. The reference
+ * runs one prompt and one set of weights at a time (pipeline.cpp, qwen3.cpp, zimage.cpp);
+ * its fine-tuning part merges an adapter into the weights before use. These take the
+ * requests' tokens as one [T, ...] matrix.
+ *   - Index and length arrays are int32 on the device. They are checked there: a value out
+ *     of range sets bit 128 of the device error word, and its row or sequence is left as it
+ *     was (a row with a bad adapter gets no adapter); sdb200_synchronize reports it.
+ *   - Workspaces are the caller's (256-byte aligned, contents arbitrary, free again when
+ *     the call's work is done), so calls may be captured into graphs. No call allocates.
+ *   - Element types: */
+#define SDB200_F32 0
+#define SDB200_BF16 1
+#define SDB200_F16 2
+
+/* rms_norm_heads() of q and of k and rope() in one pass: for every row t < T and head,
+ * u = x / sqrt(mean(x^2) + eps) * gamma (gq / gk [d] or null for 1), then the pairs of the
+ * first rot channels (even, <= d) rotated as rope() rotates them, by row pos[t] of cos / sin
+ * [n_pos, rot] (pos null: row t % n_pos); channels rot..d-1 stay u. q [T, heads * d] and
+ * k [T, kv_heads * d] have row pitches ldq / ldk (views of a fused QKV projection), either
+ * head count may be 0. in_type / out_type: SDB200_F32, _BF16 or _F16; computed in fp32,
+ * rounded once. q_out may be q itself (same type and pitch), likewise k_out. d <= 1024. */
+int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const void* k, int64_t ldk, int kv_heads,
+                        int in_type, int64_t d, int64_t rot, const float* gq, const float* gk, float eps,
+                        const float* cos, const float* sin, int64_t n_pos, const int32_t* pos, int interleaved,
+                        void* q_out, int64_t ldqo, void* k_out, int64_t ldko, int out_type);
+
+/* A shared projection plus each row's own low-rank adapter, a = row_adapter[t]:
+ *   Y[t, n] = X[t, :] W[n, :] (+ bias[n]) + scale[a] * sum_j (X[t, :] A_a[j, :]) B_a[n, j]
+ * and no second term where a < 0. X [T, ldx] bf16 (x_bf16 != 0) or fp32 (rounded to bf16 as
+ * gemm_nt_bf16 rounds it); W [N, ldw], A [n_adapters, r, lda], B [n_adapters, N, ldb] bf16;
+ * scale fp32 [n_adapters] or null for 1; Y fp32 or bf16 (y_bf16). r <= 256; adapters of
+ * smaller rank are padded with zeros. Accumulation is fp32. ws: at least
+ * sdb200_linear_lora_workspace() bytes for the same arguments. */
+int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void* X, int64_t ldx, int x_bf16,
+                                     const uint16_t* W, int64_t ldw, int64_t n_adapters, int64_t r, const uint16_t* A,
+                                     int64_t lda, const uint16_t* B, int64_t ldb);
+int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t ldx, int x_bf16, const uint16_t* W,
+                       int64_t ldw, const float* bias, const int32_t* row_adapter, int64_t n_adapters, int64_t r,
+                       const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, const float* scale, void* Y,
+                       int64_t ldy, int y_bf16, void* ws, int64_t ws_bytes);
+
+/* attention() of n_seq sequences of their own lengths, from one query token against a long
+ * cache to whole documents. Sequence s has the query rows [q_begin[s], + q_len[s]) of q and
+ * out and the key rows [kv_begin[s], + kv_len[s]) of k and v; query i stands at position
+ * p = i + kv_len - q_len among its keys. Per query head h (key head h / (heads / kv_heads)):
+ *   z_j = scale q.k_j;  cap > 0: z_j = cap tanh(z_j / cap);  slopes: z_j -= slopes[h] |p - j|
+ *   keys: all, or with causal j <= p, and with prefix [n_seq] also j < prefix[s]
+ *   out = softmax(z) v, 0 where no key is left
+ * q [Tq, ldq], k / v [Tkv, ldk / ldv] bf16 or fp16 (in_type), out [Tq, ldo] bf16 or fp16
+ * (out_type), heads d <= 256 wide, out apart from the inputs. max_q / max_kv bound the lengths.
+ * What a mask hides does not reach the result, whatever it holds; rows of no sequence are
+ * left as they were. ws: at least sdb200_attention_ragged_workspace() bytes. */
+int64_t sdb200_attention_ragged_workspace(int n_seq, int64_t max_q, int64_t max_kv, int heads, int kv_heads,
+                                          int64_t d);
+int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                            int in_type, void* out, int64_t ldo, int out_type, int64_t Tq, int64_t Tkv, int n_seq,
+                            const int32_t* q_begin, const int32_t* q_len, const int32_t* kv_begin,
+                            const int32_t* kv_len, int64_t max_q, int64_t max_kv, int heads, int kv_heads, int64_t d,
+                            float scale, float cap, const float* slopes, int causal, const int32_t* prefix, void* ws,
+                            int64_t ws_bytes);
 
 /* ---- Z-Image DiT forward (zimage.h:56 ZImageTransformer::forward) ------------------
  * The whole transformer on the device: create with the Config values of zimage.h:40-47,

@@ -28,6 +28,7 @@ enum : int {
   kErrWaitDrain = 16,     // teardown waited too long for in-flight copies
   kErrAttnWait = 32,      // attention pipeline wait timed out
   kErrTpBarrier = 64,     // tensor-parallel flag barrier: a peer did not arrive in time
+  kErrBadIndex = 128,     // an index or length read on the device is out of range
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

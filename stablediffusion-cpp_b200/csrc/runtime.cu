@@ -32,6 +32,7 @@ constexpr int kMaxDevices = 64;
 DeviceContext g_ctx[kMaxDevices];
 std::mutex g_ctx_mutex;
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+constexpr int kErrBadIndexWord = 128;  // kErrBadIndex of ptx.cuh
 }  // namespace
 
 void fail(int code, const std::string& msg) { throw Error{code, msg}; }
@@ -414,6 +415,8 @@ int sdb200_synchronize(void) {
     check_cuda(cudaMemcpy(&w, c.err_word, sizeof(int), cudaMemcpyDeviceToHost), "read error word");
     if (w) check_cuda(cudaMemset(c.err_word, 0, sizeof(int)), "clear error word");
     w |= noalloc_error_word(c.device, true);
+    if (w == kErrBadIndexWord)
+      fail(kErrInvalidArg, "an index or length read on the device was out of range (device error word 0x80)");
     if (w) {
       char buf[128];
       std::snprintf(buf, sizeof buf, "a kernel's bounded wait expired (device error word 0x%x)", w);

@@ -80,6 +80,14 @@ _SIGS = {
     "sdb200_attention_f16": ([_v, _v, _v, _v, _i, _i64, _i64, _i64, _i, _i, _i64, _i64, _i], _i),
     "sdb200_pack_heads_f16": ([_v, _v, _i64, _i, _i64, _i64], _i),
     "sdb200_attention": ([_v, _v, _v, _v, _i64, _i64, _i64, _i, _i, _i64, _i], _i),
+    "sdb200_qk_norm_rope": ([_i64, _v, _i64, _i, _v, _i64, _i, _i, _i64, _i64, _v, _v, _f, _v, _v, _i64, _v, _i, _v,
+                             _i64, _v, _i64, _i], _i),
+    "sdb200_linear_lora_workspace": ([_i64, _i64, _i64, _v, _i64, _i, _v, _i64, _i64, _i64, _v, _i64, _v, _i64], _i64),
+    "sdb200_linear_lora": ([_i64, _i64, _i64, _v, _i64, _i, _v, _i64, _v, _v, _i64, _i64, _v, _i64, _v, _i64, _v, _v,
+                            _i64, _i, _v, _i64], _i),
+    "sdb200_attention_ragged_workspace": ([_i, _i64, _i64, _i, _i, _i64], _i64),
+    "sdb200_attention_ragged": ([_v, _i64, _v, _i64, _v, _i64, _i, _v, _i64, _i, _i64, _i64, _i, _v, _v, _v, _v, _i64,
+                                 _i64, _i, _i, _i64, _f, _f, _v, _i, _v, _v, _i64], _i),
     "sdb200_zimage_create": ([_i, _i, _f, _f, _f, _i, _i, _i], _v),
     "sdb200_zimage_set_weight": ([_v, C.c_char_p, _v, _i, C.POINTER(_i64), _i], _i),
     "sdb200_zimage_finalize": ([_v], _i),

@@ -226,6 +226,159 @@ def conv2d(x, w, bias, stride, pad):
     return out
 
 
+# ---------------------------------------------------------------------------------
+# Several requests at once: adapters, per-head norms with the rotation, ragged attention
+# ---------------------------------------------------------------------------------
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_args(op, like, **tensors):
+    """Every tensor on `like`'s device, which must be the current one. (name, dtype, shape)
+    triples; None tensors are skipped, a shape of None is not checked."""
+    if not like.is_cuda or like.device.index != torch.cuda.current_device():
+        raise ValueError(f"{op}: tensors must be on the current CUDA device, got {like.device}")
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise TypeError(f"{op}: {name} must be {dtype}, got {t.dtype}")
+        if t.device != like.device:
+            raise ValueError(f"{op}: {name} is on {t.device}, expected {like.device}")
+        if shape is not None and (tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+            raise ValueError(f"{op}: {name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _head_pitch(op, name, t):
+    """Row pitch (elements) of [T, heads, d] whose heads lie next to each other."""
+    T, h, d = t.shape
+    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+        raise ValueError(f"{op}: the heads of {name} must be dense within a row")
+    return t.stride(0) if T > 1 else max(t.stride(0), h * d)
+
+
+def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleaved=False, out_dtype=None, q_out=None,
+                 k_out=None):
+    """rms_norm_heads and rope of q [T, heads, d] and k [T, kv_heads, d] in one pass (rows may
+    be strided, as views of a fused projection); cos / sin [n_pos, rot] fp32 with rot <= d,
+    row pos[t] (int32), or t % n_pos without pos. Returns (q, k) in out_dtype (default: as
+    given), or in q_out / k_out, which may be q / k themselves. k may be None."""
+    op = "qk_norm_rope"
+    if q.dtype not in _TYPES or q.dim() != 3:
+        raise TypeError(f"{op}: q must be [T, heads, d] fp32, bf16 or fp16, got {q.dtype} {tuple(q.shape)}")
+    T, heads, d = q.shape
+    out_dtype = out_dtype or (q_out.dtype if q_out is not None else q.dtype)
+    if out_dtype not in _TYPES:
+        raise TypeError(f"{op}: output type {out_dtype}")
+    if cos.dim() != 2:
+        raise ValueError(f"{op}: cos must be [n_pos, rot]")
+    _check_args(op, q, k=(k, q.dtype, None), cos=(cos, torch.float32, cos.shape), sin=(sin, torch.float32, cos.shape),
+                gq=(gq, torch.float32, (d,)), gk=(gk, torch.float32, (d,)), pos=(pos, torch.int32, (T,)),
+                q_out=(q_out, out_dtype, None), k_out=(k_out, out_dtype, None))
+    if q_out is None:
+        q_out = torch.empty((T, heads, d), device=q.device, dtype=out_dtype)
+    kv, ldk, ldko = 0, 0, 0
+    if k is not None:
+        if k.dim() != 3 or k.shape[0] != T or k.shape[2] != d:
+            raise ValueError(f"{op}: k must be [{T}, kv_heads, {d}], got {tuple(k.shape)}")
+        if k_out is None:
+            k_out = torch.empty(k.shape, device=q.device, dtype=out_dtype)
+        if k_out.shape != k.shape:
+            raise ValueError(f"{op}: k_out must have the shape of k")
+        kv, ldk, ldko = k.shape[1], _head_pitch(op, "k", k), _head_pitch(op, "k_out", k_out)
+    if q_out.shape != q.shape:
+        raise ValueError(f"{op}: q_out must have the shape of q")
+    bind_stream()
+    check(lib().sdb200_qk_norm_rope(T, q.data_ptr(), _head_pitch(op, "q", q), heads, _p(k), ldk, kv, _TYPES[q.dtype],
+                                    d, cos.shape[1], _p(gq), _p(gk), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                                    _p(pos), int(interleaved), q_out.data_ptr(), _head_pitch(op, "q_out", q_out),
+                                    _p(k_out) if k is not None else None, ldko, _TYPES[out_dtype]))
+    return q_out, (k_out if k is not None else None)
+
+
+def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32, out=None):
+    """x W^T (+ bias) + scale[a] (x A[a]^T) B[a]^T with a = rows[t] for row t (int32, < 0: no
+    adapter). x [T, K] bf16 or fp32 (rounded to bf16), W [N, K], A [n, r, K], B [n, N, r] bf16,
+    scale [n] and bias [N] fp32. Returns [T, N] in out_dtype (fp32 or bf16), or out."""
+    op = "linear_lora"
+    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+        raise TypeError(f"{op}: x [T, K] fp32 or bf16, W [N, K], A [n, r, K], B [n, N, r]")
+    T, K = x.shape
+    N, (n, r) = W.shape[0], A.shape[:2]
+    if W.shape[1] != K or A.shape[2] != K or B.shape != (n, N, r):
+        raise ValueError(f"{op}: shapes {tuple(x.shape)}, {tuple(W.shape)}, {tuple(A.shape)}, {tuple(B.shape)}")
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{op}: output type {out_dtype}")
+    bf = torch.bfloat16
+    _check_args(op, x, W=(W, bf, None), A=(A, bf, None), B=(B, bf, None), rows=(rows, torch.int32, (T,)),
+                scale=(scale, torch.float32, (n,)), bias=(bias, torch.float32, (N,)), out=(out, out_dtype, None))
+    for name, t in (("x", x), ("W", W)):
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{op}: the rows of {name} must be dense")
+    pitch = []
+    for name, t in (("A", A), ("B", B)):
+        ld = t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2])
+        if (t.shape[2] > 1 and t.stride(2) != 1) or (n > 1 and t.stride(0) != t.shape[1] * ld):
+            raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
+        pitch.append(ld)
+    if out is None:
+        out = torch.empty((T, N), device=x.device, dtype=out_dtype)
+    if out.shape != (T, N) or (N > 1 and out.stride(1) != 1):
+        raise ValueError(f"{op}: out must be [{T}, {N}] with dense rows")
+    ldx, ldw, ldy = (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]) for t in (x, W, out))
+    L = lib()
+    need = L.sdb200_linear_lora_workspace(T, N, K, x.data_ptr(), ldx, int(x.dtype == bf), W.data_ptr(), ldw, n, r,
+                                          A.data_ptr(), pitch[0], B.data_ptr(), pitch[1])
+    ws = torch.empty(max(need, 1), device=x.device, dtype=torch.uint8)
+    bind_stream()
+    check(L.sdb200_linear_lora(T, N, K, x.data_ptr(), ldx, int(x.dtype == bf), W.data_ptr(), ldw, _p(bias),
+                               rows.data_ptr(), n, r, A.data_ptr(), pitch[0], B.data_ptr(), pitch[1], _p(scale),
+                               out.data_ptr(), ldy, int(out_dtype == bf), ws.data_ptr(), need))
+    return out
+
+
+def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, scale=None, causal=False, prefix=None,
+                     cap=0.0, slopes=None, out_dtype=None, out=None):
+    """Attention of sequences of their own lengths: sequence s reads query rows
+    q_begin[s] .. + q_len[s] of q [Tq, heads, d] and key rows kv_begin[s] .. + kv_len[s] of
+    k, v [Tkv, kv_heads, d] (bf16 or fp16; rows may be strided), at most max_q and max_kv long.
+    Query i stands at position i + kv_len - q_len; causal hides later keys except the first
+    prefix[s]; cap > 0 turns a score z into cap tanh(z / cap); slopes [heads] subtract
+    slope * distance. scale defaults to 1 / sqrt(d). Returns out [Tq, heads, d] in out_dtype
+    (bf16 or fp16, default as q); rows of no sequence keep what out held (zeros without out)."""
+    op = "attention_ragged"
+    if q.dtype not in (torch.bfloat16, torch.float16) or q.dim() != 3 or k.dim() != 3:
+        raise TypeError(f"{op}: q, k, v must be [T, heads, d] bf16 or fp16, got {q.dtype}")
+    (Tq, heads, d), (Tkv, kv_heads, dk) = q.shape, k.shape
+    if dk != d or v.shape != k.shape:
+        raise ValueError(f"{op}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    out_dtype = out.dtype if out is not None else (out_dtype or q.dtype)
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{op}: output type {out_dtype}")
+    n = q_begin.numel()
+    i32 = torch.int32
+    _check_args(op, q, k=(k, q.dtype, None), v=(v, q.dtype, None), q_begin=(q_begin, i32, (n,)),
+                q_len=(q_len, i32, (n,)), kv_begin=(kv_begin, i32, (n,)), kv_len=(kv_len, i32, (n,)),
+                prefix=(prefix, i32, (n,)), slopes=(slopes, torch.float32, (heads,)), out=(out, out_dtype, None))
+    if out is None:
+        out = torch.zeros((Tq, heads, d), device=q.device, dtype=out_dtype)
+    if out.shape != q.shape:
+        raise ValueError(f"{op}: out must have the shape of q")
+    L = lib()
+    max_q, max_kv = min(max_q, Tq), min(max_kv, Tkv)
+    need = L.sdb200_attention_ragged_workspace(n, max_q, max_kv, heads, kv_heads, d)
+    ws = torch.empty(max(need, 1), device=q.device, dtype=torch.uint8)
+    bind_stream()
+    check(L.sdb200_attention_ragged(q.data_ptr(), _head_pitch(op, "q", q), k.data_ptr(), _head_pitch(op, "k", k),
+                                    v.data_ptr(), _head_pitch(op, "v", v), _TYPES[q.dtype], out.data_ptr(),
+                                    _head_pitch(op, "out", out), _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(),
+                                    q_len.data_ptr(), kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads,
+                                    kv_heads, d, d ** -0.5 if scale is None else scale, cap, _p(slopes), int(causal),
+                                    _p(prefix), ws.data_ptr(), need))
+    return out
+
+
 def mul_rows_(x, v):
     bind_stream()
     check(lib().sdb200_mul_rows(_p(x), _p(v), x.numel() // v.numel(), v.numel()))
