@@ -7,12 +7,18 @@
 #include <algorithm>
 #include <cmath>
 
-#include "elem.cuh"
-#include "internal.h"
-#include "ptx.cuh"
-#include "serving.h"
+#include "attention_ragged_tc.cuh"
 
 namespace sdb {
+namespace ragged {
+#define SDB_RAGGED_TC(DP, T) \
+  extern template void launch_tc<DP, T>(TcParams, const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, bool);
+SDB_RAGGED_TC(64, __half)
+SDB_RAGGED_TC(128, __half)
+SDB_RAGGED_TC(64, __nv_bfloat16)
+SDB_RAGGED_TC(128, __nv_bfloat16)
+#undef SDB_RAGGED_TC
+}  // namespace ragged
 namespace {
 
 constexpr int kWarps = 8;
@@ -85,12 +91,63 @@ void launch_any(const RaggedAttention& p) {
   check_launch("attention_ragged");
 }
 
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// TMA reads rows and heads that start on 16-byte boundaries; wider heads than two swizzle
+// atoms do not fit the tensor-core kernels' shared memory.
+bool tensor_core_shape(const RaggedAttention& p) {
+  return p.d <= 128 && p.d % 8 == 0 && p.ldq % 8 == 0 && p.ldk % 8 == 0 && p.ldv % 8 == 0 && p.max_kv > 0 &&
+         aligned16(p.q) && aligned16(p.k) && aligned16(p.v);
+}
+
+// Whether every sequence's queries fit one tile of 128 rows.
+bool one_tile(const RaggedAttention& p) { return p.max_q <= ragged::kBQ / (p.heads / p.kv_heads); }
+
+void launch_tensor_core(const RaggedAttention& a, void* ws) {
+  using namespace ragged;
+  TcParams p{};
+  p.a = a;
+  p.G = a.heads / a.kv_heads;
+  p.scale_log2 = a.scale * kLog2e;
+  if (a.cap > 0.0f) {
+    p.cap_in = 2.0f * kLog2e * a.scale / a.cap;
+    p.cap_log2 = a.cap * kLog2e;
+  }
+  p.out_vec = aligned16(a.out) && a.ldo % 8 == 0;
+  const bool streams = one_tile(a);
+  // One tile holds all tokens, however few: the Q box and its shared memory shrink with them.
+  p.tpt = streams ? (int)a.max_q : kBQ / p.G;
+  p.part = static_cast<float*>(ws);
+  p.part_rows = p.G * (int)std::min<int64_t>(a.max_q, kBQ);
+  p.q_atom = (p.G * p.tpt + 7) / 8 * 8 * 128;
+  const CUtensorMapDataType dt = a.in_type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tq, tk, tv;
+  auto map = [&](CUtensorMap* m, const void* x, int heads, int64_t rows, int64_t ld, int box_heads, int box_rows) {
+    const uint64_t dims[3] = {(uint64_t)a.d, (uint64_t)heads, (uint64_t)rows};
+    const uint64_t str[2] = {(uint64_t)a.d * 2, (uint64_t)ld * 2};
+    const uint32_t box[3] = {64, (uint32_t)box_heads, (uint32_t)box_rows};
+    encode_tmap(m, dt, 3, x, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  map(&tq, a.q, a.heads, a.Tq, a.ldq, p.G, p.tpt);
+  map(&tk, a.k, a.kv_heads, a.Tkv, a.ldk, 1, kBK);
+  map(&tv, a.v, a.kv_heads, a.Tkv, a.ldv, 1, kBK);
+  if (a.in_type == kBF16)
+    a.d <= 64 ? launch_tc<64, __nv_bfloat16>(p, tq, tk, tv, streams) : launch_tc<128, __nv_bfloat16>(p, tq, tk, tv, streams);
+  else
+    a.d <= 64 ? launch_tc<64, __half>(p, tq, tk, tv, streams) : launch_tc<128, __half>(p, tq, tk, tv, streams);
+}
+
 }  // namespace
 
-size_t ragged_attention_workspace(const RaggedAttention&) { return 0; }
+// The cut rows of k_ragged_streams: two pieces per worker.
+size_t ragged_attention_workspace(const RaggedAttention& p) {
+  if (!one_tile(p) || p.max_kv <= ragged::kBK || p.d > 128) return 0;
+  return (size_t)(4 * ctx().num_sms) * (size_t)(p.heads / p.kv_heads * p.max_q) * (size_t)(p.d + 2) * 4;
+}
 
-void launch_ragged_attention(RaggedAttention p, void*) {
+void launch_ragged_attention(RaggedAttention p, void* ws) {
   p.err = ctx().err_word;
+  if (tensor_core_shape(p)) return launch_tensor_core(p, ws);
   if (p.in_type == kBF16) return p.out_type == kBF16 ? launch_any<__nv_bfloat16, __nv_bfloat16>(p) : launch_any<__nv_bfloat16, __half>(p);
   p.out_type == kBF16 ? launch_any<__half, __nv_bfloat16>(p) : launch_any<__half, __half>(p);
 }

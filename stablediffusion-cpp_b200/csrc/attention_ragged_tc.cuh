@@ -1,0 +1,1164 @@
+// attention_ragged_tc.cuh - tensor-core kernels of attention_ragged (sm_100a), for head
+// widths up to 128. Flash attention: the running maximum m and sum l of a softmax, so
+// scores never leave the SM:
+//   S = Q K^T (tcgen05, fp32 in TMEM);  P = 2^(S' - m) in the operand type, back in TMEM over
+//   S;  O += P V (tcgen05);  O is rescaled when m grows by more than 2^8; out = O / l.
+//
+// The G = heads / kv_heads query heads of a key head share its keys, so a 128-row tile
+// holds floor(128 / G) tokens x G heads (row r is token r / G, head r % G): K and V are read
+// once per key head, and one token of 4 heads fills 4 rows of a tile.
+//
+// Two kernels:
+//   k_ragged_tiles    sequences of several tiles: a CTA owns two neighbouring tiles of one
+//                     key head, which share one ring of K / V slots and take turns at the
+//                     exp pass (as attention_tc.cu).
+//   k_ragged_streams  sequences of one tile (single tokens, short prompts): the CTAs are
+//                     persistent, each with two workers that own a tile and a ring of
+//                     their own. The key tiles of all sequences and heads form one list,
+//                     cut into equal parts, one per worker, whatever the lengths are;
+//                     a worker's first and last piece may be part of a row, kept as
+//                     (m, l, O) in fp32 and joined by k_ragged_join.
+// A score's modifications (MOD bit 0: cap tanh(z / cap), bit 1: minus slope x distance) are
+// applied between the TMEM load and the maximum. Masks are row limits: row r sees keys
+// j < lim = min(kv_len, max(p + 1, prefix)).
+#pragma once
+
+#include <algorithm>
+#include <string>
+
+#include "elem.cuh"
+#include "internal.h"
+#include "ptx.cuh"
+#include "serving.h"
+
+namespace sdb {
+namespace ragged {
+
+constexpr int kBQ = 128;       // rows of a query tile (TMEM lanes)
+constexpr int kBK = 128;       // keys of a K / V tile
+constexpr int kThreads = 384;  // control warpgroup + two softmax warpgroups
+// setmaxnreg split as in attention_tc.cu: 128 x 56 + 256 x 224 = 384 x 168.
+constexpr int kRegsLaunch = 168, kRegsControl = 56, kRegsSoftmax = 224;
+static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split");
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays <= 256
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxSeqs = 512;  // sequences of one k_ragged_streams launch
+constexpr int kMaxSmem = 232448;
+
+struct TcParams {
+  RaggedAttention a;
+  int G, tpt;          // heads per key head, tokens per tile
+  float scale_log2;    // scale log2(e)
+  float cap_in;        // 2 log2(e) scale / cap
+  float cap_log2;      // cap log2(e)
+  int out_vec;         // 16-byte stores allowed
+  // k_ragged_streams
+  int slots, q_atom;   // K / V slots per worker, bytes of one 64-channel Q atom
+  float* part;         // [2 workers' pieces][rows][d + 2]: O, m, l
+  int part_rows;       // rows of a piece: G * max_q
+  int seq0;            // first sequence of this launch
+};
+
+template <class T>
+struct Op;
+template <>
+struct Op<__half> {
+  static constexpr uint32_t kFmt = 0;
+  __device__ static uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Op<__nv_bfloat16> {
+  static constexpr uint32_t kFmt = 1;
+  __device__ static uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One sequence's rows, and whether its numbers fit the tensors and the launch.
+struct Seq {
+  int q0, ql, k0, kl;
+};
+__device__ __forceinline__ bool load_seq(const RaggedAttention& p, int s, Seq& q) {
+  q.q0 = p.q_begin[s];
+  q.ql = p.q_len[s];
+  q.k0 = p.kv_begin[s];
+  q.kl = p.kv_len[s];
+  return q.q0 >= 0 && q.ql >= 0 && q.k0 >= 0 && q.kl >= 0 && (int64_t)q.q0 + q.ql <= p.Tq &&
+         (int64_t)q.k0 + q.kl <= p.Tkv && q.ql <= p.max_q && q.kl <= p.max_kv;
+}
+
+// What one thread of a softmax warpgroup knows of its row.
+struct Row {
+  int tok, head;  // token of the sequence, query head
+  bool valid;
+  int lim;        // keys [0, lim) are seen
+  float pos;      // position among the keys
+  float nslope;   // -slope log2(e)
+};
+__device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, int kvh, int tok0, int r) {
+  Row w;
+  const int t = r / p.G;
+  w.tok = tok0 + t;
+  w.head = kvh * p.G + (r - t * p.G);
+  w.valid = t < p.tpt && w.tok < q.ql;
+  const int pos = w.tok + q.kl - q.ql;
+  w.lim = q.kl;
+  if (p.a.causal) w.lim = min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0));
+  w.pos = (float)pos;
+  w.nslope = p.a.slopes && w.valid ? -p.a.slopes[w.head] * kLog2e : 0.0f;
+  return w;
+}
+
+// One softmax step of a warp's 32 rows: S (128 keys, TMEM) -> P over its first 64 columns.
+// `turn` runs before the exp pass and returns false to abandon; `half` runs when keys 0..63
+// of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys.
+template <int DP, class T, int MOD, class Turn, class Half>
+__device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr, uint32_t o_addr, bool have_o, bool masked,
+                                             int n_ok, float dist0, float nslope, float& m_used, float& l, Turn turn,
+                                             Half half) {
+  uint32_t u[4][32];
+  __syncwarp();
+#pragma unroll
+  for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x32(s_addr + (uint32_t)(g * 32), u[g]);
+  tmem_wait_ld();
+  if constexpr (MOD != 0) {
+    // To log2 units. tanh(x) = 1 - 2 / (1 + e^2x): exact to 2^-23 of 1 where tanh.approx is to
+    // 2^-11, which times a cap of 50 would be 2% of a probability. e^2x = inf gives 1.
+#pragma unroll
+    for (int c = 0; c < kBK; c += 2) {
+      float2 z = make_float2(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1]));
+      if constexpr (MOD & 1) {
+        z = fmul2(z, make_float2(p.cap_in, p.cap_in));
+        const float2 e = fadd2(make_float2(ex2_approx(z.x), ex2_approx(z.y)), make_float2(1.0f, 1.0f));
+        z = ffma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), make_float2(-2.0f * p.cap_log2, -2.0f * p.cap_log2),
+                  make_float2(p.cap_log2, p.cap_log2));
+      } else {
+        z = fmul2(z, make_float2(p.scale_log2, p.scale_log2));
+      }
+      if constexpr (MOD & 2) {
+        z.x = fmaf(nslope, fabsf(dist0 - (float)c), z.x);
+        z.y = fmaf(nslope, fabsf(dist0 - (float)(c + 1)), z.y);
+      }
+      u[c >> 5][c & 31] = __float_as_uint(z.x);
+      u[c >> 5][(c & 31) + 1] = __float_as_uint(z.y);
+    }
+  }
+  if (masked) {
+#pragma unroll
+    for (int c = 0; c < kBK; ++c)
+      if (c >= n_ok) u[c >> 5][c & 31] = 0xff800000u;
+  }
+  float pm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < kBK; c += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pm[i] = fmax3(pm[i], __uint_as_float(u[c >> 5][(c & 31) + 2 * i]), __uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1]));
+  const float sc = MOD ? 1.0f : p.scale_log2;  // positive, so max(s) sc = max(s sc)
+  const float m_new = fmaxf(m_used, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sc);
+  const bool need = m_new > m_used + kRescaleThreshold;
+  if (__any_sync(0xffffffffu, need)) {
+    // The PV of the step before completed before S was posted, so O is at rest here.
+    if (have_o) {
+      const float f = need ? ex2_approx(m_used - m_new) : 1.0f;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(o_addr + (uint32_t)c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st_32x32b_x32(o_addr + (uint32_t)c, o);
+      }
+    }
+    if (need) {
+      l *= ex2_approx(m_used - m_new);
+      m_used = m_new;
+    }
+  }
+  if (!turn()) return false;
+  const float neg_m = (m_used == -INFINITY) ? 0.0f : -m_used;
+  const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
+  float2 psa = make_float2(0.0f, 0.0f), psb = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[16];
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const float2 z = make_float2(__uint_as_float(u[g][2 * c]), __uint_as_float(u[g][2 * c + 1]));
+      const float2 x = MOD ? fadd2(z, nm2) : ffma2(z, sc2, nm2);
+      const float e0 = ex2_approx(x.x), e1 = ex2_approx(x.y);
+      if (c & 1)
+        psb = fadd2(psb, make_float2(e0, e1));
+      else
+        psa = fadd2(psa, make_float2(e0, e1));
+      w[c] = Op<T>::pack(e0, e1);
+    }
+    tmem_st_32x32b_x16(s_addr + (uint32_t)(g * 16), w);
+    if (g == 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      half();
+    }
+  }
+  l += (psa.x + psb.x) + (psa.y + psb.y);
+  tmem_wait_st();
+  tc_fence_before();
+  __syncwarp();
+  return true;
+}
+
+// Stores n <= 32 fp32 values times inv as bf16 / fp16.
+__device__ __forceinline__ void store_out(const TcParams& p, int64_t at, const uint32_t (&o)[32], float inv, int n) {
+  uint16_t* dst = reinterpret_cast<uint16_t*>(p.a.out) + at;
+  const bool bf = p.a.out_type == kBF16;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = __uint_as_float(o[i + 2 * e]) * inv, b = __uint_as_float(o[i + 2 * e + 1]) * inv;
+      w[e] = bf ? Op<__nv_bfloat16>::pack(a, b) : Op<__half>::pack(a, b);
+    }
+    if (p.out_vec) {  // d % 8 == 0: whole 16-byte pieces
+      if (i < n) *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < n) dst[i + e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
+// A row computed again by one warp without the tensor core, lanes over channels, keys
+// [j0, j1) of the sequence one after another: for a row whose accumulator holds an
+// infinity or NaN. A masked key's probability is 0, but 0 times a value that is not finite
+// is NaN in a matrix product; here such keys are left out.
+template <class T>
+__device__ __noinline__ void slow_row(const TcParams& p, int64_t qrow, int head, int k0, int j0, int j1, float pos, float nslope,
+                                      float (&o)[4], float& m, float& l) {
+  const RaggedAttention& a = p.a;
+  const int lane = threadIdx.x & 31, kvh = head / p.G;
+  const T* q = reinterpret_cast<const T*>(a.q) + qrow * a.ldq + (int64_t)head * a.d;
+  float qv[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    qv[c] = lane + 32 * c < a.d ? to_f32(q[lane + 32 * c]) : 0.0f;
+    o[c] = 0.0f;
+  }
+  m = -INFINITY;
+  l = 0.0f;
+  for (int j = j0; j < j1; ++j) {
+    const T* k = reinterpret_cast<const T*>(a.k) + (int64_t)(k0 + j) * a.ldk + (int64_t)kvh * a.d;
+    const T* v = reinterpret_cast<const T*>(a.v) + (int64_t)(k0 + j) * a.ldv + (int64_t)kvh * a.d;
+    float z = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 32 * c < a.d) z = fmaf(qv[c], to_f32(k[lane + 32 * c]), z);
+    z = warp_add(z);
+    z = a.cap > 0.0f ? p.cap_log2 - 2.0f * p.cap_log2 * rcp_approx(1.0f + ex2_approx(z * p.cap_in)) : z * p.scale_log2;
+    z = fmaf(nslope, fabsf(pos - (float)j), z);
+    if (z == -INFINITY) continue;
+    const float mn = fmaxf(m, z), f = ex2_approx(m - mn), w = ex2_approx(z - mn);
+    m = mn;
+    l = l * f + w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 32 * c < a.d) o[c] = fmaf(w, to_f32(v[lane + 32 * c]), o[c] * f);
+  }
+}
+
+// The rows of a warp whose accumulators are not finite, again by slow_row: normalised into
+// out, or (m, l, O) into a piece.
+template <class T>
+__device__ __noinline__ void redo_rows(const TcParams& p, const Seq& q, const Row& w, bool bad, int j0, int j1, float* piece,
+                                       int r) {
+  const int lane = threadIdx.x & 31;
+  for (unsigned todo = __ballot_sync(0xffffffffu, bad); todo; todo &= todo - 1) {
+    const int src = __ffs(todo) - 1;
+    const int tok = __shfl_sync(0xffffffffu, w.tok, src), head = __shfl_sync(0xffffffffu, w.head, src);
+    const int lim = __shfl_sync(0xffffffffu, w.lim, src), row = __shfl_sync(0xffffffffu, r, src);
+    const float pos = __shfl_sync(0xffffffffu, w.pos, src), ns = __shfl_sync(0xffffffffu, w.nslope, src);
+    float o[4], m, l;
+    slow_row<T>(p, (int64_t)q.q0 + tok, head, q.k0, j0, min(j1, lim), pos, ns, o, m, l);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int ch = lane + 32 * c;
+      if (ch >= p.a.d) continue;
+      if (piece) {
+        piece[(int64_t)row * (p.a.d + 2) + ch] = o[c];
+      } else {
+        const int64_t at = ((int64_t)q.q0 + tok) * p.a.ldo + (int64_t)head * p.a.d + ch;
+        if (p.a.out_type == kBF16)
+          reinterpret_cast<__nv_bfloat16*>(p.a.out)[at] = from_f32<__nv_bfloat16>(o[c] * inv);
+        else
+          reinterpret_cast<__half*>(p.a.out)[at] = from_f32<__half>(o[c] * inv);
+      }
+    }
+    if (piece && lane == 0) {
+      piece[(int64_t)row * (p.a.d + 2) + p.a.d] = m;
+      piece[(int64_t)row * (p.a.d + 2) + p.a.d + 1] = l;
+    }
+  }
+}
+
+// O of one row from TMEM to out (normalised), or to a piece with m and l. all: no key of the
+// tile range but seen or zeroed ones entered the sum, so nothing needs redo_rows.
+template <int DP, class T>
+__device__ __forceinline__ void finish_rows(const TcParams& p, const Seq& q, const Row& w, uint32_t o_addr, bool have_o,
+                                            float m, float l, int j0, int j1, float* piece, int r) {
+  const bool none = !have_o || l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / l;
+  uint32_t big = 0;
+#pragma unroll 1
+  for (int c = 0; c < DP; c += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    if (have_o) {
+      tmem_ld_32x32b_x32(o_addr + (uint32_t)c, o);
+      tmem_wait_ld();
+    }
+    if (!w.valid || c >= p.a.d) continue;
+    if (none) {  // no key: zero, whatever TMEM holds
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (have_o) big = max(big, o[i] & 0x7fffffffu);
+        o[i] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) big = max(big, o[i] & 0x7fffffffu);
+    }
+    const int n = min(32, p.a.d - c);
+    if (piece) {
+      float* dst = piece + (int64_t)r * (p.a.d + 2) + c;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2)  // d is a multiple of 8, so pairs are 8-byte aligned
+        if (i < n) *reinterpret_cast<float2*>(dst + i) = make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+    } else {
+      store_out(p, ((int64_t)q.q0 + w.tok) * p.a.ldo + (int64_t)w.head * p.a.d + c, o, inv, n);
+    }
+  }
+  if (piece && w.valid)
+    *reinterpret_cast<float2*>(piece + (int64_t)r * (p.a.d + 2) + p.a.d) = make_float2(none ? -INFINITY : m, none ? 0.0f : l);
+  const bool bad = p.a.causal && w.valid && !none && big >= 0x7f800000u;
+  __syncwarp();
+  if (__any_sync(0xffffffffu, bad)) redo_rows<T>(p, q, w, bad, j0, j1, piece, r);
+}
+
+// Rows [valid, 128) of a V tile in shared memory to zero (the whole warp): keys past the
+// sequence belong to others, and 0 times what they hold need not be 0. The 128-byte
+// swizzle moves 16-byte pieces within a row only.
+template <int DP>
+__device__ __forceinline__ void zero_v_tail(uint8_t* v, int valid) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int a = 0; a < DP / 64; ++a)
+    for (int i = valid * 8 + lane; i < kBK * 8; i += 32)
+      *reinterpret_cast<uint4*>(v + a * (kBK * 128) + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// ------------------------------------------------------------------------------------
+// Two neighbouring tiles of one key head of one sequence.
+// ------------------------------------------------------------------------------------
+template <int DP>
+struct TilesCfg {
+  static constexpr int ATOM = kBQ * 128;
+  static constexpr int ATOMS = DP / 64;
+  static constexpr int Q_BYTES = ATOMS * ATOM;
+  static constexpr int KV_BYTES = ATOMS * ATOM;
+  static constexpr int SLOTS = DP == 128 ? 5 : 10;
+  static constexpr int SMEM = 2 * Q_BYTES + SLOTS * KV_BYTES + 1024 + 512;
+};
+constexpr uint32_t kOCol = 256;  // TMEM: S_A | S_B | O_A | O_B
+
+// The pair of tiles `want` (counted over all sequences) belongs to: sequence and first
+// pair, or -1. All threads; two barriers per 384 sequences.
+__device__ __forceinline__ int find_pair(const TcParams& p, int want, int* sh, int& pair) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  if (threadIdx.x == 0) sh[13] = -1;
+  for (int s0 = 0; s0 < p.a.n_seq; s0 += kThreads) {
+    const int s = s0 + threadIdx.x;
+    Seq q;
+    int n = 0;
+    if (s < p.a.n_seq) {
+      if (load_seq(p.a, s, q))
+        n = (q.ql + 2 * p.tpt - 1) / (2 * p.tpt);
+      else
+        atomicOr(p.a.err, kErrBadIndex);
+    }
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    int before = base, all = base;
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < warp) before += sh[i];
+      all += sh[i];
+    }
+    const int first = before + x - n;
+    if (want >= first && want < first + n) {
+      sh[13] = s;
+      sh[14] = want - first;
+    }
+    __syncthreads();
+    base = all;
+    if (sh[13] >= 0) break;
+  }
+  pair = sh[14];
+  return sh[13];
+}
+
+template <int DP, class T, int MOD>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_ragged_tiles(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcParams p) {
+  using C_ = TilesCfg<DP>;
+  constexpr uint32_t IDESC_S = make_idesc(Op<T>::kFmt, 0, 0, kBQ, kBK);
+  constexpr uint32_t IDESC_O = make_idesc(Op<T>::kFmt, 0, 1 /*V is MN-major*/, kBQ, DP);
+  constexpr int SLOTS = C_::SLOTS;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sR = sQ + 2 * C_::Q_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sR + SLOTS * C_::KV_BYTES);
+  uint64_t* q_full = bars;
+  uint64_t* s_full = bars + 1;   // [2] S_t(j) ready (and PV_t(j-1) done)
+  uint64_t* p_half = bars + 3;   // [2] keys 0..63 of P_t(j) stored, O_t rescaled
+  uint64_t* p_full = bars + 5;   // [2]
+  uint64_t* turn = bars + 7;     // [2] the tile finished its exp pass
+  uint64_t* o_final = bars + 9;  // [2]
+  uint64_t* drain = bars + 11;   // [2]
+  uint64_t* r_full = bars + 13;  // [SLOTS]
+  uint64_t* r_empty = r_full + SLOTS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + SLOTS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* scan = reinterpret_cast<int*>(tmem_slot + 2);  // [16]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x % p.a.kv_heads;
+  int pair;
+  const int s = find_pair(p, blockIdx.x / p.a.kv_heads, scan, pair);
+  if (s < 0) return;  // uniform: fewer pairs than the launch allowed for
+  Seq q;
+  load_seq(p.a, s, q);
+  // Late tiles first: with a causal mask they have the most keys.
+  const int pairs = (q.ql + 2 * p.tpt - 1) / (2 * p.tpt);
+  const int tok0 = (pairs - 1 - pair) * 2 * p.tpt;
+  const int pre = p.a.causal && p.a.prefix ? p.a.prefix[s] : 0;
+  // Key tiles of each of the two tiles (0: the tile has no token or no key).
+  auto tiles_of = [&](int t) {
+    const int first = tok0 + t * p.tpt;
+    if (first >= q.ql) return 0;
+    const int last = min(q.ql, first + p.tpt) - 1;
+    const int lim = p.a.causal ? min(q.kl, max(last + q.kl - q.ql + 1, pre)) : q.kl;
+    return (max(lim, 0) + kBK - 1) / kBK;
+  };
+  const int nA = tiles_of(0), nB = tiles_of(1);
+  const int nkv = max(nA, nB);
+  const bool two = nB > 0;  // nA <= nB then, tile limits grow with the tokens
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&r_full[i], 1);
+      mbar_init(&r_empty[i], two ? 2 : 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_half[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&turn[i], 4);
+      mbar_init(&o_final[i], 1);
+      mbar_init(&drain[i], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  int* err = p.a.err;
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    if (warp == 0) {
+      // ------------------------------ TMA producer ------------------------------
+      if (lane == 0 && nkv > 0) {
+        const int nq = two ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, nq * C_::ATOMS * p.G * p.tpt * 128);
+        for (int t = 0; t < nq; ++t)
+          for (int a = 0; a < C_::ATOMS; ++a)
+            tma_load_3d(sQ + t * C_::Q_BYTES + a * C_::ATOM, &tmQ, q_full, a * 64, kvh * p.G, q.q0 + tok0 + t * p.tpt);
+        int issued = -1;
+        for (int i = 0; i < 2 * nkv; ++i) {
+          const int sl = i % SLOTS, u = i / SLOTS;
+          if (!mbar_wait(&r_empty[sl], (u & 1) ^ 1u, abort_flag, err, kErrAttnWait)) break;
+          mbar_arrive_expect_tx(&r_full[sl], C_::KV_BYTES);
+          const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
+          for (int a = 0; a < C_::ATOMS; ++a)
+            tma_load_3d(sR + sl * C_::KV_BYTES + a * C_::ATOM, tm, &r_full[sl], a * 64, kvh, q.k0 + (i >> 1) * kBK);
+          issued = i;
+        }
+        if (issued < 2 * nkv - 1) {
+          // Aborted: wait (bounded) for the loads this CTA still has in flight.
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < kWaitLimitNs) {
+          }
+          for (int i = max(0, issued - SLOTS + 1); i <= issued; ++i)
+            while (!mbar_try_wait(&r_full[i % SLOTS], (i / SLOTS) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
+            }
+        }
+      }
+    } else if (warp == 1 || warp == 2) {
+      // ------------------------------ MMA issuers -------------------------------
+      // The whole warp runs the loop (it zeroes the last V tile's tail); lane 0 issues.
+      const int t = warp - 1, nt = t ? nB : nA;
+      if (nt > 0 || (t == 0 && two)) {
+        bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrAttnWait);
+        tc_fence_after();
+        const uint32_t q_addr = smem_u32(sQ + t * C_::Q_BYTES);
+        const uint32_t d_s = tmem + (uint32_t)(t * kBK);
+        const uint32_t d_o = tmem + kOCol + (uint32_t)(t * DP);
+        uint64_t qd[8] = {};
+        uint32_t pa[8];
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          if (ks < DP / 16) qd[ks] = sdesc_k_sw128(q_addr + (uint32_t)((ks >> 2) * C_::ATOM + (ks & 3) * 32));
+          pa[ks] = d_s + (uint32_t)(ks * 8);
+        }
+        for (int j = 0; ok && j <= nkv; ++j) {
+          const int vi = 2 * j - 1, ki = 2 * j;
+          const int vsl = (vi + SLOTS) % SLOTS, ksl = ki % SLOTS;
+          uint8_t* vp = sR + vsl * C_::KV_BYTES;
+          const uint32_t v_addr = smem_u32(vp), k_addr = smem_u32(sR + ksl * C_::KV_BYTES);
+          uint64_t vd[8], kd[8] = {};
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            vd[ks] = sdesc_mn_sw128(v_addr + (uint32_t)(ks * 16 * 128), C_::ATOM, 1024);
+            if (ks < DP / 16) kd[ks] = sdesc_k_sw128(k_addr + (uint32_t)((ks >> 2) * C_::ATOM + (ks & 3) * 32));
+          }
+          if (j > 0 && !mbar_wait(&r_full[vsl], (vi / SLOTS) & 1, abort_flag, err, kErrAttnWait)) break;
+          if (j < nkv && !mbar_wait(&r_full[ksl], (ki / SLOTS) & 1, abort_flag, err, kErrAttnWait)) break;
+          if (j > 0) {
+            if (j <= nt) {
+              if (j * kBK > q.kl) zero_v_tail<DP>(vp, q.kl - (j - 1) * kBK);
+              if (!mbar_wait(&p_half[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
+              tc_fence_after();
+              if (lane == 0) {
+                const uint32_t a4[4] = {pa[0], pa[1], pa[2], pa[3]};
+                const uint64_t b4[4] = {vd[0], vd[1], vd[2], vd[3]};
+                umma4_f16_ts(d_o, a4, b4, IDESC_O, j > 1 ? 1u : 0u);
+              }
+              if (!mbar_wait(&p_full[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
+              tc_fence_after();
+              if (lane == 0) {
+                const uint32_t a4[4] = {pa[4], pa[5], pa[6], pa[7]};
+                const uint64_t b4[4] = {vd[4], vd[5], vd[6], vd[7]};
+                umma4_f16_ts(d_o, a4, b4, IDESC_O, 1u);
+                umma_commit(&r_empty[vsl]);
+                if (j == nt) umma_commit(&o_final[t]);
+              }
+            } else if (lane == 0) {
+              mbar_arrive(&r_empty[vsl]);  // the other tile's keys
+            }
+          }
+          if (j < nkv && lane == 0) {
+            if (j < nt) {
+              tc_fence_after();
+              if constexpr (DP == 128)
+                umma8_f16_ss(d_s, qd, kd, IDESC_S, 0u);
+              else {
+                const uint64_t a4[4] = {qd[0], qd[1], qd[2], qd[3]};
+                const uint64_t b4[4] = {kd[0], kd[1], kd[2], kd[3]};
+                umma4_f16_ss(d_s, a4, b4, IDESC_S, 0u);
+              }
+              umma_commit(&s_full[t]);
+              umma_commit(&r_empty[ksl]);
+            } else {
+              mbar_arrive(&r_empty[ksl]);
+            }
+          }
+          __syncwarp();
+        }
+        if (lane == 0) {
+          umma_commit(&drain[t]);
+          const uint64_t t0 = globaltimer_ns();
+          while (!mbar_try_wait(&drain[t], 0))
+            if (globaltimer_ns() - t0 > kWaitLimitNs) {
+              atomicOr(err, kErrWaitDrain);
+              break;
+            }
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    // ------------------------------ softmax / epilogue ------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int t = (warp - 4) >> 2, qq = warp & 3;
+    const int r = qq * 32 + lane, nt = t ? nB : nA;
+    const Row w = make_row(p, q, s, kvh, tok0 + t * p.tpt, r);
+    const uint32_t lane_base = tmem + ((uint32_t)(qq * 32) << 16);
+    const uint32_t s_addr = lane_base + (uint32_t)(t * kBK);
+    const uint32_t o_addr = lane_base + kOCol + (uint32_t)(t * DP);
+    // The tile's first token has the smallest limit.
+    const int lim0 = p.a.causal ? min(q.kl, max(tok0 + t * p.tpt + q.kl - q.ql + 1, pre)) : q.kl;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      if (!mbar_wait(&s_full[t], j & 1, abort_flag, err, kErrAttnWait)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int kbase = j * kBK;
+      ok = softmax_step<DP, T, MOD>(
+          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.pos - (float)kbase, w.nslope, m, l,
+          [&]() {
+            // The tiles take turns (A(0), B(0), A(1), ...) while both have keys.
+            if (!two || (t == 0 ? j == 0 : j >= nA)) return true;
+            return mbar_wait(&turn[t ^ 1], (t == 0 ? j - 1 : j) & 1, abort_flag, err, kErrAttnWait);
+          },
+          [&]() {
+            if (lane == 0) mbar_arrive(&p_half[t]);
+          });
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive(&p_full[t]);
+        mbar_arrive(&turn[t]);
+      }
+    }
+    if (ok && (nt == 0 || mbar_wait(&o_final[t], 0, abort_flag, err, kErrAttnWait))) {
+      tc_fence_after();
+      finish_rows<DP, T>(p, q, w, o_addr, nt > 0, m, l, 0, q.kl, nullptr, r);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// Sequences of one tile each.
+// ------------------------------------------------------------------------------------
+// Shared list of the launch's sequences: first[s] is the number of key tiles (steps) of
+// the sequences before s over all key heads, first[n] the total. A sequence with queries has at
+// least one step per key head, so that rows without a key are written.
+struct StepList {
+  long long first[kMaxSeqs + 1];
+  Seq seq[kMaxSeqs];
+  int warp_sum[2][32];
+};
+__device__ __forceinline__ int steps_of(const Seq& q) { return max(1, (q.kl + kBK - 1) / kBK); }
+
+// All threads of the block (a multiple of 32, at most 1024); ends with a barrier.
+__device__ __forceinline__ void build_steps(const TcParams& p, StepList& L, int n) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  long long base = 0;
+  for (int s0 = 0; s0 < n; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x;
+    Seq q = {0, 0, 0, 0};
+    if (s < n && !load_seq(p.a, p.seq0 + s, q)) {
+      atomicOr(p.a.err, kErrBadIndex);
+      q = {0, 0, 0, 0};
+    }
+    long long x = q.ql > 0 ? (long long)steps_of(q) * p.a.kv_heads : 0;
+    const long long own = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) {
+      L.warp_sum[0][warp] = (int)(x & 0xffffffff);
+      L.warp_sum[1][warp] = (int)(x >> 32);
+    }
+    __syncthreads();
+    long long all = base;
+    for (int i = 0; i < nw; ++i) {
+      const long long v = ((long long)L.warp_sum[1][i] << 32) | (unsigned)L.warp_sum[0][i];
+      if (i < warp) x += v;
+      all += v;
+    }
+    if (s < n) {
+      L.first[s] = base + x - own;
+      L.seq[s] = q;
+    }
+    base = all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) L.first[n] = base;
+  __syncthreads();
+}
+// The sequence that step belongs to: the last one with first[s] <= step.
+__device__ __forceinline__ int find_step(const StepList& L, int n, long long step) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (L.first[mid] <= step)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+__device__ __forceinline__ long long part_begin(long long total, int workers, int w) { return total * w / workers; }
+
+// A worker's pieces in order: key tiles [kt0, kt1) of key head kvh of sequence s.
+struct Pieces {
+  const StepList& L;
+  int n;
+  long long at, end;
+  int s, kvh, kt0, kt1;
+  bool whole;
+  __device__ Pieces(const StepList& L_, int n_, int w, int workers)
+      : L(L_), n(n_), at(part_begin(L_.first[n_], workers, w)), end(part_begin(L_.first[n_], workers, w + 1)) {}
+  __device__ bool next() {
+    if (at >= end) return false;
+    s = find_step(L, n, at);
+    const int e = steps_of(L.seq[s]);
+    const long long rem = at - L.first[s];
+    kvh = (int)(rem / e);
+    kt0 = (int)(rem - (long long)kvh * e);
+    kt1 = (int)min((long long)e, kt0 + (end - at));
+    whole = kt0 == 0 && kt1 == e;
+    at += kt1 - kt0;
+    return true;
+  }
+  __device__ int tiles() const { return L.seq[s].kl > 0 ? kt1 - kt0 : 0; }  // to load
+};
+
+template <int DP, class T, int MOD>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_ragged_streams(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcParams p) {
+  constexpr int ATOM = kBK * 128, ATOMS = DP / 64, KV_BYTES = ATOMS * ATOM;
+  constexpr uint32_t IDESC_S = make_idesc(Op<T>::kFmt, 0, 0, kBQ, kBK);
+  constexpr uint32_t IDESC_O = make_idesc(Op<T>::kFmt, 0, 1, kBQ, DP);
+  constexpr int kMaxSlots = 8;
+
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ StepList steps;
+  __shared__ uint64_t bars[2][8 + 2 * kMaxSlots];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  // Q of worker 0 | Q of worker 1 | slots of worker 0 | of worker 1. A Q atom may be shorter
+  // than 128 rows: the MMA then reads rows of what follows, into rows that nobody uses.
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int SL = p.slots;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Worker of this warp: producers are warps 0 and 3, issuers 1 and 2, softmax 4-7 and 8-11.
+  const int t = warp < 4 ? (warp >= 2 ? 1 : 0) : (warp - 4) >> 2;
+  uint8_t* sQ = smem + t * ATOMS * p.q_atom;
+  uint8_t* sR = smem + 2 * ATOMS * p.q_atom + t * SL * KV_BYTES;
+  uint64_t* b = bars[t];
+  uint64_t *q_full = b, *q_empty = b + 1, *s_full = b + 2, *p_half = b + 3, *p_full = b + 4, *o_full = b + 5,
+           *drain = b + 6, *r_full = b + 8, *r_empty = b + 8 + kMaxSlots;
+  const int worker = t * gridDim.x + blockIdx.x, workers = 2 * gridDim.x;
+  const int n = min(p.a.n_seq - p.seq0, kMaxSeqs);
+
+  if (threadIdx.x < 2) {
+    uint64_t* z = bars[threadIdx.x];
+    mbar_init(z + 0, 1);
+    mbar_init(z + 1, 1);
+    mbar_init(z + 2, 1);
+    mbar_init(z + 3, 4);
+    mbar_init(z + 4, 4);
+    mbar_init(z + 5, 1);
+    mbar_init(z + 6, 1);
+    for (int i = 0; i < SL; ++i) {
+      mbar_init(z + 8 + i, 1);
+      mbar_init(z + 8 + kMaxSlots + i, 1);
+    }
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 2 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  tc_fence_before();
+  build_steps(p, steps, n);
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  int* err = p.a.err;
+  Pieces it(steps, n, worker, workers);
+  // The next launch (k_ragged_join) may be set up now; it waits for this grid's end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    if (warp == 0 || warp == 3) {
+      // ------------------------------ TMA producer ------------------------------
+      if (lane == 0) {
+        int ld = 0, nq = 0;  // loads and Q tiles so far: slot ld % SL, its use ld / SL
+        bool ok = true;
+        while (ok && it.next()) {
+          const int nt = it.tiles();
+          if (nt == 0) continue;
+          const Seq& q = steps.seq[it.s];
+          for (int i = 0; i < 2 * nt && ok; ++i) {
+            if (i == 0) {
+              ok = mbar_wait(q_empty, (nq & 1) ^ 1u, abort_flag, err, kErrAttnWait);
+              if (!ok) break;
+              mbar_arrive_expect_tx(q_full, ATOMS * p.G * p.tpt * 128);
+              for (int a = 0; a < ATOMS; ++a)
+                tma_load_3d(sQ + a * p.q_atom, &tmQ, q_full, a * 64, it.kvh * p.G, q.q0);
+              ++nq;
+            }
+            const int sl = ld % SL;
+            ok = mbar_wait(&r_empty[sl], ((ld / SL) & 1) ^ 1u, abort_flag, err, kErrAttnWait);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&r_full[sl], KV_BYTES);
+            const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
+            for (int a = 0; a < ATOMS; ++a)
+              tma_load_3d(sR + sl * KV_BYTES + a * ATOM, tm, &r_full[sl], a * 64, it.kvh, q.k0 + (it.kt0 + (i >> 1)) * kBK);
+            ++ld;
+          }
+        }
+        if (!ok) {
+          // Aborted: wait (bounded) for the loads this worker still has in flight.
+          const uint64_t t0 = globaltimer_ns();
+          if (nq > 0)
+            while (!mbar_try_wait(q_full, (nq - 1) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
+            }
+          for (int i = max(0, ld - SL); i < ld; ++i)
+            while (!mbar_try_wait(&r_full[i % SL], (i / SL) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
+            }
+        }
+      }
+    } else {
+      // ------------------------------ MMA issuer --------------------------------
+      const uint32_t q_addr = smem_u32(sQ);
+      const uint32_t d_s = tmem + (uint32_t)(t * kBK), d_o = tmem + kOCol + (uint32_t)(t * DP);
+      uint64_t qd[8] = {};
+      uint32_t pa[8];
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        if (ks < DP / 16) qd[ks] = sdesc_k_sw128(q_addr + (uint32_t)((ks >> 2) * p.q_atom + (ks & 3) * 32));
+        pa[ks] = d_s + (uint32_t)(ks * 8);
+      }
+      int ld = 0, nq = 0, step = 0;
+      bool ok = true;
+      while (ok && it.next()) {
+        const int nt = it.tiles();
+        if (nt == 0) continue;
+        const int kl = steps.seq[it.s].kl;
+        ok = mbar_wait(q_full, nq & 1, abort_flag, err, kErrAttnWait);
+        ++nq;
+        tc_fence_after();
+        // Loads ld + 2j (K_j) and ld + 2j + 1 (V_j) of this piece.
+        for (int j = 0; ok && j <= nt; ++j) {
+          const int vi = ld + 2 * j - 1, ki = ld + 2 * j;
+          if (j > 0) {
+            const int sl = vi % SL;
+            uint8_t* vp = sR + sl * KV_BYTES;
+            const uint32_t v_addr = smem_u32(vp);
+            ok = mbar_wait(&r_full[sl], (vi / SL) & 1, abort_flag, err, kErrAttnWait);
+            if (!ok) break;
+            const int left = kl - (it.kt0 + j - 1) * kBK;
+            if (left < kBK) zero_v_tail<DP>(vp, left);
+            uint64_t vd[8];
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) vd[ks] = sdesc_mn_sw128(v_addr + (uint32_t)(ks * 16 * 128), ATOM, 1024);
+            ok = mbar_wait(p_half, (step - 1) & 1, abort_flag, err, kErrAttnWait);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t a4[4] = {pa[0], pa[1], pa[2], pa[3]};
+              const uint64_t b4[4] = {vd[0], vd[1], vd[2], vd[3]};
+              umma4_f16_ts(d_o, a4, b4, IDESC_O, j > 1 ? 1u : 0u);
+            }
+            ok = mbar_wait(p_full, (step - 1) & 1, abort_flag, err, kErrAttnWait);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t a4[4] = {pa[4], pa[5], pa[6], pa[7]};
+              const uint64_t b4[4] = {vd[4], vd[5], vd[6], vd[7]};
+              umma4_f16_ts(d_o, a4, b4, IDESC_O, 1u);
+              umma_commit(&r_empty[sl]);
+              if (j == nt) umma_commit(o_full);
+            }
+          }
+          if (j < nt) {
+            const int sl = ki % SL;
+            const uint32_t k_addr = smem_u32(sR + sl * KV_BYTES);
+            ok = mbar_wait(&r_full[sl], (ki / SL) & 1, abort_flag, err, kErrAttnWait);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+              uint64_t kd[8] = {};
+#pragma unroll
+              for (int ks = 0; ks < DP / 16; ++ks)
+                kd[ks] = sdesc_k_sw128(k_addr + (uint32_t)((ks >> 2) * ATOM + (ks & 3) * 32));
+              if constexpr (DP == 128)
+                umma8_f16_ss(d_s, qd, kd, IDESC_S, 0u);
+              else {
+                const uint64_t a4[4] = {qd[0], qd[1], qd[2], qd[3]};
+                const uint64_t b4[4] = {kd[0], kd[1], kd[2], kd[3]};
+                umma4_f16_ss(d_s, a4, b4, IDESC_S, 0u);
+              }
+              umma_commit(s_full);
+              umma_commit(&r_empty[sl]);
+              if (j == nt - 1) umma_commit(q_empty);
+            }
+            ++step;
+          }
+          __syncwarp();
+        }
+        ld += 2 * nt;
+      }
+      if (lane == 0) {
+        umma_commit(drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0))
+          if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(err, kErrWaitDrain);
+            break;
+          }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------ softmax / epilogue ------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    const int qq = warp & 3, r = qq * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(qq * 32) << 16);
+    const uint32_t s_addr = lane_base + (uint32_t)(t * kBK);
+    const uint32_t o_addr = lane_base + kOCol + (uint32_t)(t * DP);
+    int step = 0, pieces = 0;
+    bool ok = true;
+    while (ok && it.next()) {
+      const Seq q = steps.seq[it.s];
+      const int nt = it.tiles();
+      const Row w = make_row(p, q, p.seq0 + it.s, it.kvh, 0, r);
+      const bool busy = qq * 32 < p.G * q.ql;  // the warp has rows (uniform)
+      const int lim0 = p.a.causal ? min(q.kl, max(q.kl - q.ql + 1, p.a.prefix ? p.a.prefix[p.seq0 + it.s] : 0)) : q.kl;
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < nt; ++j, ++step) {
+        if (!mbar_wait(s_full, step & 1, abort_flag, err, kErrAttnWait)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int kbase = (it.kt0 + j) * kBK;
+        if (busy) {
+          softmax_step<DP, T, MOD>(
+              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.pos - (float)kbase, w.nslope, m, l,
+              []() { return true; },
+              [&]() {
+                if (lane == 0) mbar_arrive(p_half);
+              });
+          if (lane == 0) mbar_arrive(p_full);
+        } else {
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_half);
+            mbar_arrive(p_full);
+          }
+        }
+      }
+      if (!ok) break;
+      if (nt > 0) {
+        if (!mbar_wait(o_full, pieces & 1, abort_flag, err, kErrAttnWait)) break;
+        ++pieces;
+        tc_fence_after();
+      }
+      if (busy) {
+        float* piece = nullptr;
+        if (!it.whole) piece = p.part + (int64_t)(2 * worker + (it.kt0 > 0 ? 0 : 1)) * p.part_rows * (p.a.d + 2);
+        finish_rows<DP, T>(p, q, w, o_addr, nt > 0, m, l, it.kt0 * kBK, it.kt1 * kBK, piece, r);
+      }
+      tc_fence_before();  // O is read before the next piece's P lets a PV write it
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The pieces of the rows that k_ragged_streams cut, joined: one warp per row (sequence,
+// token, head). Which workers hold them follows from the step list alone; rows that one
+// worker finished are already in out.
+template <class T>
+__global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcParams p, int workers) {
+  __shared__ StepList steps;
+  const int lane = threadIdx.x & 31, n = min(p.a.n_seq - p.seq0, kMaxSeqs);
+  build_steps(p, steps, n);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long total = steps.first[n];
+  const long long rows = (long long)n * p.a.max_q * p.a.heads;
+  const int pitch = p.a.d + 2;
+  for (long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); x < rows; x += (long long)gridDim.x * 8) {
+    const int h = (int)(x % p.a.heads);
+    const long long y = x / p.a.heads;
+    const int tok = (int)(y % p.a.max_q), s = (int)(y / p.a.max_q);
+    const Seq q = steps.seq[s];
+    if (tok >= q.ql) continue;
+    const int kvh = h / p.G, r = tok * p.G + (h - kvh * p.G), e = steps_of(q);
+    const long long a = steps.first[s] + (long long)kvh * e;
+    int w = (int)(a * workers / total);  // the worker that holds step a
+    while (w > 0 && part_begin(total, workers, w) > a) --w;
+    while (part_begin(total, workers, w + 1) <= a) ++w;
+    if (part_begin(total, workers, w + 1) >= a + e) continue;  // whole
+    const int w0 = w;
+    float top = -INFINITY;
+    for (; w < workers && part_begin(total, workers, w) < a + e; ++w) {
+      if (part_begin(total, workers, w + 1) == part_begin(total, workers, w)) continue;  // no steps
+      const float* piece = p.part + ((int64_t)(2 * w + (w == w0 ? 1 : 0)) * p.part_rows + r) * pitch;
+      top = fmaxf(top, piece[p.a.d]);
+    }
+    if (top == -INFINITY) top = 0.0f;
+    float l = 0.0f;
+    float2 o[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    const int w1 = w;
+    for (w = w0; w < w1; ++w) {
+      if (part_begin(total, workers, w + 1) == part_begin(total, workers, w)) continue;
+      const float* piece = p.part + ((int64_t)(2 * w + (w == w0 ? 1 : 0)) * p.part_rows + r) * pitch;
+      const float2 ml = *reinterpret_cast<const float2*>(piece + p.a.d);
+      const float f = ex2_approx(ml.x - top);
+      l = fmaf(f, ml.y, l);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (2 * lane + 64 * c < p.a.d) {
+          const float2 v = *reinterpret_cast<const float2*>(piece + 2 * lane + 64 * c);
+          o[c] = ffma2(make_float2(f, f), v, o[c]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = reinterpret_cast<T*>(p.a.out) + ((int64_t)q.q0 + tok) * p.a.ldo + (int64_t)h * p.a.d;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (2 * lane + 64 * c < p.a.d) {
+        out[2 * lane + 64 * c] = from_f32<T>(o[c].x * inv);
+        out[2 * lane + 64 * c + 1] = from_f32<T>(o[c].y * inv);
+      }
+  }
+}
+
+template <class K>
+void prepare_kernel(K kern, int smem, bool (&done)[64]) {
+  const int dev = ctx().device;
+  if (done[dev]) return;
+  // setmaxnreg.inc waits until the registers it asks for are free; the split only adds up if
+  // the kernel was compiled to exactly kRegsLaunch registers per thread.
+  cudaFuncAttributes fa{};
+  check_cuda(cudaFuncGetAttributes(&fa, kern), "cudaFuncGetAttributes(attention_ragged)");
+  if (fa.numRegs != kRegsLaunch)
+    fail(kErrUnsupported, "attention_ragged: compiled with " + std::to_string(fa.numRegs) + " registers per thread, the " +
+                              "register split needs " + std::to_string(kRegsLaunch));
+  check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+             "cudaFuncSetAttribute(attention_ragged)");
+  done[dev] = true;
+}
+
+template <int DP, class T, int MOD>
+void launch_mod(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool streams) {
+  DeviceContext& c = ctx();
+  if (!streams) {
+    static bool done[64] = {};
+    prepare_kernel(k_ragged_tiles<DP, T, MOD>, TilesCfg<DP>::SMEM, done);
+    // Pairs of tiles: at most one per sequence more than the rows make.
+    const int64_t pairs = std::min<int64_t>((int64_t)p.a.n_seq * ((p.a.max_q + 2 * p.tpt - 1) / (2 * p.tpt)),
+                                            p.a.Tq / (2 * p.tpt) + p.a.n_seq);
+    const int64_t grid = pairs * p.a.kv_heads;
+    if (grid >= ((int64_t)1 << 31)) fail(kErrInvalidArg, "attention_ragged: too many query tiles");
+    k_ragged_tiles<DP, T, MOD><<<(unsigned)grid, kThreads, TilesCfg<DP>::SMEM, c.stream>>>(tq, tk, tv, p);
+    check_launch("attention_ragged_tiles");
+    return;
+  }
+  constexpr int kKv = DP / 64 * kBK * 128;
+  const int room = kMaxSmem - (int)sizeof(StepList) - 1024 - 1024 - 2 * (DP / 64) * p.q_atom;
+  p.slots = std::min(8, room / (2 * kKv));
+  const int smem = 1024 + 2 * (DP / 64) * p.q_atom + 2 * p.slots * kKv;
+  static bool done[64] = {};
+  prepare_kernel(k_ragged_streams<DP, T, MOD>, kMaxSmem - (int)sizeof(StepList) - 1024, done);
+  for (p.seq0 = 0; p.seq0 < p.a.n_seq; p.seq0 += kMaxSeqs) {
+    k_ragged_streams<DP, T, MOD><<<(unsigned)c.num_sms, kThreads, smem, c.stream>>>(tq, tk, tv, p);
+    check_launch("attention_ragged_streams");
+    if (p.a.max_kv <= kBK) continue;  // every piece is a whole row
+    const int64_t rows = (int64_t)std::min(p.a.n_seq - p.seq0, kMaxSeqs) * p.a.max_q * p.a.heads;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)c.num_sms * 4));
+    cfg.blockDim = dim3(256);
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const int workers = 2 * c.num_sms;
+    if (p.a.out_type == kBF16)
+      check_cuda(cudaLaunchKernelEx(&cfg, k_ragged_join<__nv_bfloat16>, (const TcParams)p, workers), "attention_ragged_join");
+    else
+      check_cuda(cudaLaunchKernelEx(&cfg, k_ragged_join<__half>, (const TcParams)p, workers), "attention_ragged_join");
+    check_launch("attention_ragged_join");
+  }
+}
+
+template <int DP, class T>
+void launch_tc(TcParams p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool streams) {
+  const int mod = (p.a.cap > 0.0f ? 1 : 0) | (p.a.slopes ? 2 : 0);
+  if (mod == 0) return launch_mod<DP, T, 0>(p, tq, tk, tv, streams);
+  if (mod == 1) return launch_mod<DP, T, 1>(p, tq, tk, tv, streams);
+  if (mod == 2) return launch_mod<DP, T, 2>(p, tq, tk, tv, streams);
+  launch_mod<DP, T, 3>(p, tq, tk, tv, streams);
+}
+
+}  // namespace ragged
+}  // namespace sdb
