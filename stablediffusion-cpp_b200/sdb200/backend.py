@@ -230,11 +230,15 @@ def conv2d(x, w, bias, stride, pad):
 # Several requests at once: adapters, per-head norms with the rotation, ragged attention
 # ---------------------------------------------------------------------------------
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _check_args(op, like, **tensors):
-    """Every tensor on `like`'s device, which must be the current one. (name, dtype, shape)
-    triples; None tensors are skipped, a shape of None is not checked."""
+def _refuse_args(op, like, **tensors):
+    """Names what is wrong with the tensors, (tensor, dtype, shape or None) by name: all on
+    like's device, which must be the current one, and contiguous where a shape is given. The
+    operators below test all of it in one expression and come here only when it fails: at one
+    token a call's GPU time is that of a few tensor checks."""
     if not like.is_cuda or like.device.index != torch.cuda.current_device():
         raise ValueError(f"{op}: tensors must be on the current CUDA device, got {like.device}")
     for name, (t, dtype, shape) in tensors.items():
@@ -248,12 +252,35 @@ def _check_args(op, like, **tensors):
             raise ValueError(f"{op}: {name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
 
 
+def _fits(t, dtype, dev, shape):
+    """A None tensor, or one of that type, device and contiguous shape."""
+    return t is None or (t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous())
+
+
 def _head_pitch(op, name, t):
     """Row pitch (elements) of [T, heads, d] whose heads lie next to each other."""
     T, h, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+    row, head, one = t.stride()
+    if (one != 1 and d > 1) or (head != d and h > 1):
         raise ValueError(f"{op}: the heads of {name} must be dense within a row")
-    return t.stride(0) if T > 1 else max(t.stride(0), h * d)
+    return row if T > 1 else h * d
+
+
+def _row_pitch(op, name, t):
+    rows, cols = t.shape
+    row, one = t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"{op}: the rows of {name} must be dense")
+    return row if rows > 1 else cols
+
+
+def _stack_pitch(op, name, t):
+    n, rows, cols = t.shape
+    s0, s1, s2 = t.stride()
+    ld = s1 if rows > 1 else s0 if n > 1 else cols
+    if (s2 != 1 and cols > 1) or (n > 1 and s0 != rows * ld):
+        raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
+    return ld
 
 
 def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleaved=False, out_dtype=None, q_out=None,
@@ -263,36 +290,51 @@ def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleav
     row pos[t] (int32), or t % n_pos without pos. Returns (q, k) in out_dtype (default: as
     given), or in q_out / k_out, which may be q / k themselves. k may be None."""
     op = "qk_norm_rope"
-    if q.dtype not in _TYPES or q.dim() != 3:
-        raise TypeError(f"{op}: q must be [T, heads, d] fp32, bf16 or fp16, got {q.dtype} {tuple(q.shape)}")
+    dtype, dev = q.dtype, q.get_device()
+    if dtype not in _TYPES or q.dim() != 3:
+        raise TypeError(f"{op}: q must be [T, heads, d] fp32, bf16 or fp16, got {dtype} {tuple(q.shape)}")
     T, heads, d = q.shape
-    out_dtype = out_dtype or (q_out.dtype if q_out is not None else q.dtype)
+    out_dtype = out_dtype or (q_out.dtype if q_out is not None else dtype)
     if out_dtype not in _TYPES:
         raise TypeError(f"{op}: output type {out_dtype}")
-    if cos.dim() != 2:
+    table = cos.shape
+    if len(table) != 2:
         raise ValueError(f"{op}: cos must be [n_pos, rot]")
-    _check_args(op, q, k=(k, q.dtype, None), cos=(cos, torch.float32, cos.shape), sin=(sin, torch.float32, cos.shape),
-                gq=(gq, torch.float32, (d,)), gk=(gk, torch.float32, (d,)), pos=(pos, torch.int32, (T,)),
-                q_out=(q_out, out_dtype, None), k_out=(k_out, out_dtype, None))
+    if not (0 <= dev == _current() and _fits(cos, _F32, dev, table) and _fits(sin, _F32, dev, table)
+            and _fits(gq, _F32, dev, (d,)) and _fits(gk, _F32, dev, (d,)) and _fits(pos, _I32, dev, (T,))
+            and (k is None or (k.dtype is dtype and k.get_device() == dev))
+            and (q_out is None or (q_out.dtype is out_dtype and q_out.get_device() == dev))
+            and (k_out is None or (k_out.dtype is out_dtype and k_out.get_device() == dev))):
+        _refuse_args(op, q, k=(k, dtype, None), cos=(cos, _F32, table), sin=(sin, _F32, table), gq=(gq, _F32, (d,)),
+                     gk=(gk, _F32, (d,)), pos=(pos, _I32, (T,)), q_out=(q_out, out_dtype, None),
+                     k_out=(k_out, out_dtype, None))
+    ldqo, kv, ldk, ldko, kp, kop = heads * d, 0, 0, 0, None, None
     if q_out is None:
-        q_out = torch.empty((T, heads, d), device=q.device, dtype=out_dtype)
-    kv, ldk, ldko = 0, 0, 0
-    if k is not None:
+        q_out = q.new_empty((T, heads, d), dtype=out_dtype)
+    else:
+        if q_out.shape != q.shape:
+            raise ValueError(f"{op}: q_out must have the shape of q")
+        ldqo = _head_pitch(op, "q_out", q_out)
+    if k is None:
+        k_out = None
+    else:
         if k.dim() != 3 or k.shape[0] != T or k.shape[2] != d:
             raise ValueError(f"{op}: k must be [{T}, kv_heads, {d}], got {tuple(k.shape)}")
+        kv = k.shape[1]
+        ldk, ldko = _head_pitch(op, "k", k), kv * d
         if k_out is None:
-            k_out = torch.empty(k.shape, device=q.device, dtype=out_dtype)
-        if k_out.shape != k.shape:
-            raise ValueError(f"{op}: k_out must have the shape of k")
-        kv, ldk, ldko = k.shape[1], _head_pitch(op, "k", k), _head_pitch(op, "k_out", k_out)
-    if q_out.shape != q.shape:
-        raise ValueError(f"{op}: q_out must have the shape of q")
-    bind_stream()
-    check(lib().sdb200_qk_norm_rope(T, q.data_ptr(), _head_pitch(op, "q", q), heads, _p(k), ldk, kv, _TYPES[q.dtype],
-                                    d, cos.shape[1], _p(gq), _p(gk), eps, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-                                    _p(pos), int(interleaved), q_out.data_ptr(), _head_pitch(op, "q_out", q_out),
-                                    _p(k_out) if k is not None else None, ldko, _TYPES[out_dtype]))
-    return q_out, (k_out if k is not None else None)
+            k_out = q.new_empty((T, kv, d), dtype=out_dtype)
+        else:
+            if k_out.shape != k.shape:
+                raise ValueError(f"{op}: k_out must have the shape of k")
+            ldko = _head_pitch(op, "k_out", k_out)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    L = lib()
+    check(L.sdb200_set_stream(_raw_stream(dev)))
+    check(L.sdb200_qk_norm_rope(T, q.data_ptr(), _head_pitch(op, "q", q), heads, kp, ldk, kv, _TYPES[dtype], d, table[1],
+                                _p(gq), _p(gk), eps, cos.data_ptr(), sin.data_ptr(), table[0], _p(pos),
+                                1 if interleaved else 0, q_out.data_ptr(), ldqo, kop, ldko, _TYPES[out_dtype]))
+    return q_out, k_out
 
 
 def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32, out=None):
@@ -300,41 +342,38 @@ def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32
     adapter). x [T, K] bf16 or fp32 (rounded to bf16), W [N, K], A [n, r, K], B [n, N, r] bf16,
     scale [n] and bias [N] fp32. Returns [T, N] in out_dtype (fp32 or bf16), or out."""
     op = "linear_lora"
-    if x.dtype not in (torch.float32, torch.bfloat16) or x.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+    dtype, dev = x.dtype, x.get_device()
+    if dtype not in (_F32, _BF16) or x.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
         raise TypeError(f"{op}: x [T, K] fp32 or bf16, W [N, K], A [n, r, K], B [n, N, r]")
     T, K = x.shape
-    N, (n, r) = W.shape[0], A.shape[:2]
-    if W.shape[1] != K or A.shape[2] != K or B.shape != (n, N, r):
+    N, (n, r, Ka) = W.shape[0], A.shape
+    if W.shape[1] != K or Ka != K or B.shape != (n, N, r):
         raise ValueError(f"{op}: shapes {tuple(x.shape)}, {tuple(W.shape)}, {tuple(A.shape)}, {tuple(B.shape)}")
     if out is not None:
         out_dtype = out.dtype
-    if out_dtype not in (torch.float32, torch.bfloat16):
+    if out_dtype not in (_F32, _BF16):
         raise TypeError(f"{op}: output type {out_dtype}")
-    bf = torch.bfloat16
-    _check_args(op, x, W=(W, bf, None), A=(A, bf, None), B=(B, bf, None), rows=(rows, torch.int32, (T,)),
-                scale=(scale, torch.float32, (n,)), bias=(bias, torch.float32, (N,)), out=(out, out_dtype, None))
-    for name, t in (("x", x), ("W", W)):
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"{op}: the rows of {name} must be dense")
-    pitch = []
-    for name, t in (("A", A), ("B", B)):
-        ld = t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2])
-        if (t.shape[2] > 1 and t.stride(2) != 1) or (n > 1 and t.stride(0) != t.shape[1] * ld):
-            raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
-        pitch.append(ld)
+    if not (0 <= dev == _current() and W.dtype is _BF16 and A.dtype is _BF16 and B.dtype is _BF16 and W.get_device() == dev
+            and A.get_device() == dev and B.get_device() == dev and _fits(rows, _I32, dev, (T,))
+            and _fits(scale, _F32, dev, (n,)) and _fits(bias, _F32, dev, (N,))
+            and (out is None or out.get_device() == dev)):
+        _refuse_args(op, x, W=(W, _BF16, None), A=(A, _BF16, None), B=(B, _BF16, None), rows=(rows, _I32, (T,)),
+                     scale=(scale, _F32, (n,)), bias=(bias, _F32, (N,)), out=(out, out_dtype, None))
     if out is None:
-        out = torch.empty((T, N), device=x.device, dtype=out_dtype)
-    if out.shape != (T, N) or (N > 1 and out.stride(1) != 1):
-        raise ValueError(f"{op}: out must be [{T}, {N}] with dense rows")
-    ldx, ldw, ldy = (t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1]) for t in (x, W, out))
+        out, ldy = x.new_empty((T, N), dtype=out_dtype), N
+    else:
+        if out.shape != (T, N):
+            raise ValueError(f"{op}: out must be [{T}, {N}]")
+        ldy = _row_pitch(op, "out", out)
+    operands = (T, N, K, x.data_ptr(), _row_pitch(op, "x", x), 1 if dtype is _BF16 else 0, W.data_ptr(),
+                _row_pitch(op, "W", W))
+    adapters = (n, r, A.data_ptr(), _stack_pitch(op, "A", A), B.data_ptr(), _stack_pitch(op, "B", B))
     L = lib()
-    need = L.sdb200_linear_lora_workspace(T, N, K, x.data_ptr(), ldx, int(x.dtype == bf), W.data_ptr(), ldw, n, r,
-                                          A.data_ptr(), pitch[0], B.data_ptr(), pitch[1])
-    ws = torch.empty(max(need, 1), device=x.device, dtype=torch.uint8)
-    bind_stream()
-    check(L.sdb200_linear_lora(T, N, K, x.data_ptr(), ldx, int(x.dtype == bf), W.data_ptr(), ldw, _p(bias),
-                               rows.data_ptr(), n, r, A.data_ptr(), pitch[0], B.data_ptr(), pitch[1], _p(scale),
-                               out.data_ptr(), ldy, int(out_dtype == bf), ws.data_ptr(), need))
+    need = L.sdb200_linear_lora_workspace(*operands, *adapters)
+    ws = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    check(L.sdb200_set_stream(_raw_stream(dev)))
+    check(L.sdb200_linear_lora(*operands, _p(bias), rows.data_ptr(), *adapters, _p(scale), out.data_ptr(), ldy,
+                               1 if out_dtype is _BF16 else 0, _p(ws), need))
     return out
 
 
@@ -348,34 +387,41 @@ def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, s
     slope * distance. scale defaults to 1 / sqrt(d). Returns out [Tq, heads, d] in out_dtype
     (bf16 or fp16, default as q); rows of no sequence keep what out held (zeros without out)."""
     op = "attention_ragged"
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.dim() != 3 or k.dim() != 3:
-        raise TypeError(f"{op}: q, k, v must be [T, heads, d] bf16 or fp16, got {q.dtype}")
+    dtype, dev = q.dtype, q.get_device()
+    if dtype not in (_BF16, torch.float16) or q.dim() != 3 or k.dim() != 3:
+        raise TypeError(f"{op}: q, k, v must be [T, heads, d] bf16 or fp16, got {dtype}")
     (Tq, heads, d), (Tkv, kv_heads, dk) = q.shape, k.shape
     if dk != d or v.shape != k.shape:
         raise ValueError(f"{op}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    out_dtype = out.dtype if out is not None else (out_dtype or q.dtype)
-    if out_dtype not in (torch.bfloat16, torch.float16):
+    out_dtype = out.dtype if out is not None else (out_dtype or dtype)
+    if out_dtype not in (_BF16, torch.float16):
         raise TypeError(f"{op}: output type {out_dtype}")
     n = q_begin.numel()
-    i32 = torch.int32
-    _check_args(op, q, k=(k, q.dtype, None), v=(v, q.dtype, None), q_begin=(q_begin, i32, (n,)),
-                q_len=(q_len, i32, (n,)), kv_begin=(kv_begin, i32, (n,)), kv_len=(kv_len, i32, (n,)),
-                prefix=(prefix, i32, (n,)), slopes=(slopes, torch.float32, (heads,)), out=(out, out_dtype, None))
+    one = (n,)
+    if not (0 <= dev == _current() and k.dtype is dtype and v.dtype is dtype and k.get_device() == dev
+            and v.get_device() == dev and _fits(q_begin, _I32, dev, one) and _fits(q_len, _I32, dev, one)
+            and _fits(kv_begin, _I32, dev, one) and _fits(kv_len, _I32, dev, one) and _fits(prefix, _I32, dev, one)
+            and _fits(slopes, _F32, dev, (heads,)) and (out is None or out.get_device() == dev)):
+        _refuse_args(op, q, k=(k, dtype, None), v=(v, dtype, None), q_begin=(q_begin, _I32, one), q_len=(q_len, _I32, one),
+                     kv_begin=(kv_begin, _I32, one), kv_len=(kv_len, _I32, one), prefix=(prefix, _I32, one),
+                     slopes=(slopes, _F32, (heads,)), out=(out, out_dtype, None))
     if out is None:
-        out = torch.zeros((Tq, heads, d), device=q.device, dtype=out_dtype)
-    if out.shape != q.shape:
-        raise ValueError(f"{op}: out must have the shape of q")
+        out, ldo = q.new_zeros((Tq, heads, d), dtype=out_dtype), heads * d
+    else:
+        if out.shape != q.shape:
+            raise ValueError(f"{op}: out must have the shape of q")
+        ldo = _head_pitch(op, "out", out)
     L = lib()
     max_q, max_kv = min(max_q, Tq), min(max_kv, Tkv)
     need = L.sdb200_attention_ragged_workspace(n, max_q, max_kv, heads, kv_heads, d)
-    ws = torch.empty(max(need, 1), device=q.device, dtype=torch.uint8)
-    bind_stream()
+    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    check(L.sdb200_set_stream(_raw_stream(dev)))
     check(L.sdb200_attention_ragged(q.data_ptr(), _head_pitch(op, "q", q), k.data_ptr(), _head_pitch(op, "k", k),
-                                    v.data_ptr(), _head_pitch(op, "v", v), _TYPES[q.dtype], out.data_ptr(),
-                                    _head_pitch(op, "out", out), _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(),
-                                    q_len.data_ptr(), kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads,
-                                    kv_heads, d, d ** -0.5 if scale is None else scale, cap, _p(slopes), int(causal),
-                                    _p(prefix), ws.data_ptr(), need))
+                                    v.data_ptr(), _head_pitch(op, "v", v), _TYPES[dtype], out.data_ptr(), ldo,
+                                    _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(), q_len.data_ptr(),
+                                    kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads, kv_heads, d,
+                                    d ** -0.5 if scale is None else scale, cap, _p(slopes), 1 if causal else 0,
+                                    _p(prefix), _p(ws), need))
     return out
 
 
