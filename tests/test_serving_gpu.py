@@ -208,6 +208,8 @@ LORA = [  # T, N, K, r, adapters, rows: each | runs | random | one | none, in, o
     (31, 40, 3, 1, 2, "random", BF16, F32, True, True),
     (200, 8, 24, 2, 3, "random", BF16, BF16, True, True),
     (257, 2048, 2048, 16, 2, "runs", BF16, BF16, True, False),
+    (4300, 2056, 128, 16, 6, "runs", BF16, BF16, True, True),          # tiles of pairs of processors
+    (4100, 2048, 192, 40, 5, "random", BF16, F32, True, False),
 ]
 
 
@@ -253,12 +255,12 @@ def test_linear_lora_strided_operands(sdb, T):
     assert (out[:, :2] == 3.0).all() and (out[:, N + 2:] == 3.0).all()
 
 
-@pytest.mark.parametrize("T", [4, 30, 130, 400])
+@pytest.mark.parametrize("T,N", [(4, 320), (30, 320), (130, 320), (400, 320), (4200, 2048)])
 @pytest.mark.parametrize("to", [BF16, F32])
-def test_linear_lora_keeps_requests_apart(sdb, T, to):
+def test_linear_lora_keeps_requests_apart(sdb, T, N, to):
     """NaN and infinities of one adapter or of one row stay in the rows that use them."""
     g = gen(11 * T)
-    N, K, r, n = 320, 256, 16, 4
+    K, r, n = 256, 16, 4
     x, W, A, B, scale, bias = lora_inputs(g, T, N, K, r, n)
     rows = torch.arange(T, device="cuda", dtype=torch.int32) % (n + 1) - 1
     clean = (rows != 1) & (rows != 2)
