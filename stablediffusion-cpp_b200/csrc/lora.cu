@@ -2,8 +2,8 @@
 //   y[t, n] = sum_k x[t, k] W[n, k] + bias[n] + sum_j h[t, j] B_a[n, j],
 //   h[t, j] = s_a sum_k x[t, k] A_a[j, k],   a = row_adapter[t] (no second term for a < 0).
 //
-// Up to 64 rows the work is reading W and the adapters once (k_lora_down_rows, k_lora_rows);
-// above, it is a GEMM (k_lora_down and the adapter form of gemm_tc.cu).
+// Up to 128 rows the work is reading W and the adapters once (k_lora_down_rows, k_lora_rows);
+// above, it is a GEMM (k_lora_down, k_lora_gemm).
 #include <algorithm>
 
 #include "elem.cuh"
@@ -18,84 +18,187 @@ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int kMaxRowsSmall = 64;
+constexpr int kMaxRowsSmall = 128;
+
+// The adapter term rides on the same tensor-core product as W: next to the K blocks of X and
+// W, an accumulator runs through the chunks of H and B, where H holds h in the columns of the
+// row's own adapter and zeros in those of the other adapters among the rows it is multiplied with.
+// A chunk is cw = 16, 32 or 64 ranks of one adapter; for an fp32 output h is kept in two bf16
+// parts, high and low, and each chunk has one of either.
+// K-major operand rows of `pitch` = 32, 64 or 128 bytes in the swizzle of that width.
+__device__ __forceinline__ uint64_t sdesc_k(uint32_t saddr, int pitch) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)1u << 16;
+  d |= (uint64_t)((uint32_t)(8 * pitch) >> 4) << 32;  // 8 rows
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)(pitch == 128 ? 2u : pitch == 64 ? 4u : 6u) << 61;
+  return d;
+}
+// Two bf16 of a word, the low half first.
+__device__ __forceinline__ float2 bf16x2_to_f32(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// h in bf16 (part 0), and what that lost (part 1): together h to 2^-16.
+__device__ __forceinline__ uint32_t h_part(float h, int part) {
+  const uint32_t hi = f32_to_bf16_rne(h);
+  if (!part) return hi;
+  const float v = bf16_to_f32((uint16_t)hi);
+  return f32_to_bf16_rne(fabsf(v) < INFINITY ? h - v : 0.0f);
+}
+inline int chunk_width(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : 64; }
+inline CUtensorMapSwizzle swizzle_of(int cw) {
+  return cw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : cw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+}
+
 
 // ------------------------------------------------------------------------------------
 // Few rows
 // ------------------------------------------------------------------------------------
-// h[t, j], one warp per value, 16-byte loads of both rows (pitches multiples of 8, packed
-// where they were not; elements past K are masked). Bound by the adapters' bytes.
+// H: [f][part][rc][TN][cw] bf16 for every row f that is the first of its adapter.
+struct RowsK {
+  uint16_t* H;
+  int cw, rc, parts;
+  __host__ __device__ int per() const { return parts * rc; }  // chunks of an adapter
+};
+
+// Whether row i is the first of its adapter (ids of the T rows in shared memory).
+__device__ __forceinline__ bool is_first(const int* ids, int i) {
+  const int a = ids[i];
+  bool first = a >= 0;
+  for (int j = 0; j < i; ++j) first &= ids[j] != a;
+  return first;
+}
+
+// h[t, 8 jb .. + 8] with one warp per value and 16-byte loads of both rows (pitches are
+// multiples of 8, elements past K masked), then row t of every adapter's chunks: its own
+// values, or zeros. Bound by the adapters' bytes.
 __global__ void __launch_bounds__(256) k_lora_down_rows(const LoraLinear p, const uint16_t* __restrict__ X, int64_t ldx,
-                                                        const uint16_t* __restrict__ A, int64_t lda, float* __restrict__ h) {
+                                                        const uint16_t* __restrict__ A, int64_t lda, RowsK rk, int TN) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31, t = blockIdx.x;
-  const int64_t j = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (j >= p.r) return;
-  const int a = p.row_adapter[t];
-  if (a >= p.n_adapters && lane == 0 && j == 0) atomicOr(p.err, kErrBadIndex);
+  __shared__ int ids[kMaxRowsSmall];
+  __shared__ float sh[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x, T = (int)p.T;
+  const int j = blockIdx.y * 8 + warp;
+  if (threadIdx.x < T) {
+    const int a = p.row_adapter[threadIdx.x];
+    if (a >= p.n_adapters && threadIdx.x == t && blockIdx.y == 0) atomicOr(p.err, kErrBadIndex);
+    ids[threadIdx.x] = a < p.n_adapters ? a : -1;
+  }
+  __syncthreads();
+  const int a = ids[t];
   float s = 0.0f;
-  if (a >= 0 && a < p.n_adapters) {
+  if (a >= 0 && j < p.r) {
+    const float scale = p.scale ? p.scale[a] : 1.0f;
     const uint16_t* x = X + (int64_t)t * ldx;
     const uint16_t* w = A + ((int64_t)a * p.r + j) * lda;
     float2 s2 = make_float2(0.0f, 0.0f);
-    const int64_t whole = p.K / 8;
-#pragma unroll 4
-    for (int64_t c = lane; c < whole; c += 32) {
+    const int whole = (int)(p.K / 8);
+#pragma unroll 8
+    for (int c = lane; c < whole; c += 32) {
       const uint4 u = *reinterpret_cast<const uint4*>(x + 8 * c), v = __ldg(reinterpret_cast<const uint4*>(w + 8 * c));
-      const uint32_t ux[4] = {u.x, u.y, u.z, u.w}, vx[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s2 = ffma2(make_float2(__uint_as_float(ux[i] << 16), __uint_as_float(ux[i] & 0xffff0000u)),
-                   make_float2(__uint_as_float(vx[i] << 16), __uint_as_float(vx[i] & 0xffff0000u)), s2);
+      s2 = ffma2(bf16x2_to_f32(u.x), bf16x2_to_f32(v.x), s2);
+      s2 = ffma2(bf16x2_to_f32(u.y), bf16x2_to_f32(v.y), s2);
+      s2 = ffma2(bf16x2_to_f32(u.z), bf16x2_to_f32(v.z), s2);
+      s2 = ffma2(bf16x2_to_f32(u.w), bf16x2_to_f32(v.w), s2);
     }
     s = s2.x + s2.y;
-    for (int64_t k = whole * 8 + lane; k < p.K; k += 32) s = fmaf(bf16_to_f32(x[k]), bf16_to_f32(w[k]), s);
-    s = warp_add(s) * (p.scale ? p.scale[a] : 1.0f);
+    for (int k = whole * 8 + lane; k < p.K; k += 32) s = fmaf(bf16_to_f32(x[k]), bf16_to_f32(w[k]), s);
+    s = warp_add(s) * scale;
   }
-  if (lane == 0) h[t * p.r + j] = s;
+  if (lane == 0) sh[warp] = s;
+  __syncthreads();
+  if (threadIdx.x < T && is_first(ids, threadIdx.x)) {
+    const bool own = ids[threadIdx.x] == a;
+    const int j0 = blockIdx.y * 8, c = j0 / rk.cw;
+    for (int part = 0; part < rk.parts; ++part) {
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (own)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(sh[e], part) << (16 * (e & 1));
+      uint16_t* dst = rk.H + ((((int64_t)threadIdx.x * rk.parts + part) * rk.rc + c) * TN + t) * rk.cw + j0 % rk.cw;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
 }
 
-// All rows in one tile of N_mma columns: D[n, t] = sum_k W[n, k] x[t, k] on tcgen05, 128
-// rows of W (the M of the MMA) per cluster, K split over the cluster's CTAs, so that every
-// processor streams W. While the copies run, the epilogue warps add up the adapter term in
-// fp32 for the CTA's share of the rows n; then the CTAs' partial sums are read from their
-// shared memory in rank order (the result does not depend on timing).
+struct LoraRows {
+  LoraLinear p;
+  RowsK rk;
+  const uint16_t *X, *W, *B;
+  int64_t ldx, ldw, ldb;
+  int splits;
+};
+__device__ __noinline__ int spoilt_feature(const LoraRows& g, const int* ids, const int* list, int count, int64_t n) {
+  for (int i = 0; i < count; ++i) {
+    const uint16_t* b = g.B + ((int64_t)ids[list[i]] * g.p.N + n) * g.ldb;
+    for (int c = 0; c < g.p.r; ++c)
+      if ((b[c] & 0x7f80u) == 0x7f80u) return 1;
+  }
+  return 0;
+}
+__device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int t, int64_t n, int TN) {
+  const uint16_t *x = g.X + t * g.ldx, *w = g.W + n * g.ldw;
+  float s = g.p.bias ? g.p.bias[n] : 0.0f;
+  for (int64_t k = 0; k < g.p.K; ++k) s = fmaf(bf16_to_f32(x[k]), bf16_to_f32(w[k]), s);
+  const int a = ids[t];
+  if (a < 0) return s;
+  int f = 0;
+  while (ids[f] != a) ++f;
+  const uint16_t* b = g.B + ((int64_t)a * g.p.N + n) * g.ldb;
+  for (int c = 0; c < g.p.r; ++c)
+    for (int part = 0; part < g.rk.parts; ++part) {
+      const uint16_t hv =
+          g.rk.H[((((int64_t)f * g.rk.parts + part) * g.rk.rc + c / g.rk.cw) * TN + t) * g.rk.cw + c % g.rk.cw];
+      s = fmaf(bf16_to_f32(hv), bf16_to_f32(b[c]), s);
+    }
+  return s;
+}
+
+// The rows are the N of one MMA tile: D[n, t] = sum_k W[n, k] x[t, k] (+ the chunks of B and
+// H) on tcgen05, 128 rows of W (the M of the MMA) per cluster. K blocks and chunks are split
+// over the cluster's CTAs, so that every processor streams W; the CTAs' partial sums are read
+// from their shared memory in rank order (the result does not depend on timing).
 template <int TN>
 struct RowsCfg {
   static constexpr int W_BYTES = 128 * 128, X_BYTES = TN * 128, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = 4;
-  static constexpr int PITCH = TN + 1;  // floats of a row of partial sums: spreads banks
-  static constexpr int SUM_BYTES = 128 * PITCH * 4;
-  static_assert(STAGES * STAGE >= SUM_BYTES, "partial sums reuse the stages");
+  static constexpr int STAGES = TN >= 64 ? 3 : 4;  // two CTAs fit a processor
+  static_assert(STAGES * STAGE >= 128 * TN * 4, "partial sums reuse the stages");
+  static constexpr int SMEM = 1024 + STAGES * STAGE;
 };
 constexpr int kRowThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kSumThreads = 256;  // k_lora_rows: eight
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
 }
 
 template <int TN>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(64 + kSumThreads, 2)
     k_lora_rows(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                const __grid_constant__ LoraLinear p, const float* __restrict__ h, const uint16_t* __restrict__ B,
-                int64_t ldb, int splits, int b_vec) {
+                const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmH,
+                const __grid_constant__ LoraRows g) {
   using C_ = RowsCfg<TN>;
   constexpr uint32_t IDESC = make_idesc(1u, 0, 0, 128, TN);
   constexpr uint32_t COLS = TN < 32 ? 32 : TN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sums = reinterpret_cast<float*>(smem);                               // [128][PITCH], after the MMAs
-  float* delta = reinterpret_cast<float*>(smem + C_::STAGES * C_::STAGE);    // [128 / splits][PITCH]
-  float* sh = delta + (128 / splits) * C_::PITCH;                            // [T][r]
-  __shared__ uint64_t full[C_::STAGES], empty[C_::STAGES], acc_full;
+  float* sums = reinterpret_cast<float*>(smem);  // [TN][128] after the MMAs: features side by side, for reads of whole lines
+  __shared__ uint64_t full[C_::STAGES], empty[C_::STAGES], acc_full, list_full;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int abort_word, ids[kMaxRowsSmall], list[kMaxRowsSmall], in_warp[4], mixed;
   volatile int* abort_flag = &abort_word;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const LoraLinear& p = g.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = g.splits;
   const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
-  const int T = (int)p.T, r = (int)p.r;
+  const int T = (int)p.T, per_stage = 64 / g.rk.cw, cwb = 2 * g.rk.cw;
   const int64_t n0 = (int64_t)tile * 128;
   const int kblocks = (int)((p.K + 63) / 64);
   const int kb0 = (int)((int64_t)kblocks * rank / splits), kb1 = (int)((int64_t)kblocks * (rank + 1) / splits);
@@ -106,7 +209,9 @@ __global__ void __launch_bounds__(kRowThreads)
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
+    mbar_init(&list_full, 1);
     abort_word = 0;
+    mixed = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -117,17 +222,39 @@ __global__ void __launch_bounds__(kRowThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // This CTA's chunks: those of the listed adapters whose number is rank modulo splits.
+  auto my_chunks = [&]() { return (in_warp[0] * g.rk.per() - rank + splits - 1) / splits; };
   if (warp == 0) {
     if (lane == 0) {
       int done = 0;
+      bool ok = true;
+      auto stage = [&](int bytes) {
+        ok = mbar_wait(&empty[done % C_::STAGES], ((done / C_::STAGES) & 1) ^ 1u, abort_flag, p.err, kErrWaitEmpty);
+        if (ok) mbar_arrive_expect_tx(&full[done % C_::STAGES], bytes);
+        return smem + done % C_::STAGES * C_::STAGE;
+      };
       for (int kb = kb0; kb < kb1; ++kb, ++done) {
-        const int s = done % C_::STAGES;
-        if (!mbar_wait(&empty[s], ((done / C_::STAGES) & 1) ^ 1u, abort_flag, p.err, kErrWaitEmpty)) break;
-        mbar_arrive_expect_tx(&full[s], C_::STAGE);
-        tma_load_2d(smem + s * C_::STAGE, &tmW, &full[s], kb * 64, (int)n0);
-        tma_load_2d(smem + s * C_::STAGE + C_::W_BYTES, &tmX, &full[s], kb * 64, 0);
+        uint8_t* st = stage(C_::STAGE);
+        if (!ok) break;
+        tma_load_2d(st, &tmW, &full[done % C_::STAGES], kb * 64, (int)n0);
+        tma_load_2d(st + C_::W_BYTES, &tmX, &full[done % C_::STAGES], kb * 64, 0);
       }
-      if (done < kb1 - kb0) {
+      if (ok && g.rk.rc > 0) {
+        ok = mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int nq = ok ? my_chunks() : 0;
+        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
+          const int n = min(per_stage, nq - q0);
+          uint8_t* st = stage(n * (128 + TN) * cwb);
+          if (!ok) break;
+          for (int i = 0; i < n; ++i) {
+            const int q = (q0 + i) * splits + rank, f = list[q / g.rk.per()], sub = q % g.rk.per();
+            tma_load_3d(st + i * 128 * cwb, &tmB, &full[done % C_::STAGES], sub % g.rk.rc * g.rk.cw, (int)n0, ids[f]);
+            tma_load_2d(st + C_::W_BYTES + i * TN * cwb, &tmH, &full[done % C_::STAGES], 0, (f * g.rk.per() + sub) * TN);
+          }
+        }
+      }
+      if (!ok) {
         // Aborted: wait (bounded) for the loads in flight.
         const uint64_t t0 = globaltimer_ns();
         for (int i = max(0, done - C_::STAGES); i < done; ++i)
@@ -137,15 +264,32 @@ __global__ void __launch_bounds__(kRowThreads)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      for (int i = 0; i < kb1 - kb0; ++i) {
-        const int s = i % C_::STAGES;
-        if (!mbar_wait(&full[s], (i / C_::STAGES) & 1, abort_flag, p.err, kErrWaitFull)) break;
+      int done = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb, ++done) {
+        const int s = done % C_::STAGES;
+        ok = mbar_wait(&full[s], (done / C_::STAGES) & 1, abort_flag, p.err, kErrWaitFull);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_f16_ss(tmem, sdesc_k_sw128(a0 + k * 32), sdesc_k_sw128(b0 + k * 32), IDESC, (i | k) != 0);
+          umma_f16_ss(tmem, sdesc_k_sw128(a0 + k * 32), sdesc_k_sw128(b0 + k * 32), IDESC, kb > kb0 || k > 0);
         umma_commit(&empty[s]);
+      }
+      if (ok && g.rk.rc > 0 && mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull)) {
+        const int nq = my_chunks();
+        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
+          const int s = done % C_::STAGES;
+          if (!mbar_wait(&full[s], (done / C_::STAGES) & 1, abort_flag, p.err, kErrWaitFull)) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
+          for (int i = 0; i < min(per_stage, nq - q0); ++i)
+            for (int k = 0; k < g.rk.cw / 16; ++k)
+              umma_f16_ss(tmem, sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), sdesc_k(b0 + i * TN * cwb + k * 32, cwb), IDESC,
+                          kb1 > kb0 || q0 + i + k > 0);
+          umma_commit(&empty[s]);
+        }
       }
       umma_commit(&acc_full);
       const uint64_t t0 = globaltimer_ns();
@@ -156,75 +300,94 @@ __global__ void __launch_bounds__(kRowThreads)
         }
     }
   } else {
-    // The adapter term of rows [rank R, + R) of the tile, one output feature n and every
-    // `splits`-th token per thread.
-    const int tid = threadIdx.x - 64, R = 128 / splits;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int i = tid; i < T * r; i += 128) sh[i] = h[i];
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    const int row = tid % R;
-    const int64_t n = n0 + rank * R + row;
-    for (int t = tid / R; t < T; t += splits) {
-      const int a = p.row_adapter ? p.row_adapter[t] : -1;
-      float d = 0.0f;
-      if (r > 0 && a >= 0 && a < p.n_adapters && n < p.N) {
-        const uint16_t* b = B + ((int64_t)a * p.N + n) * ldb;
-        const float* ht = sh + t * r;
-        if (b_vec) {  // 16-byte rows of B, r a multiple of 8
-          float2 d2 = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-          for (int c = 0; c < r; c += 8) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(b + c));
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              d2 = ffma2(make_float2(ht[c + 2 * i], ht[c + 2 * i + 1]),
-                         make_float2(__uint_as_float(x[i] << 16), __uint_as_float(x[i] & 0xffff0000u)), d2);
-          }
-          d = d2.x + d2.y;
-        } else {
-          for (int c = 0; c < r; ++c) d = fmaf(ht[c], bf16_to_f32(b[c]), d);
-        }
+    const int tid = threadIdx.x - 64;
+    if (g.rk.rc > 0) {
+      // The adapters among the rows, in the order of their first rows.
+      if (tid < T) {
+        const int a = p.row_adapter[tid];
+        ids[tid] = a < p.n_adapters ? a : -1;
       }
-      delta[row * C_::PITCH + t] = d;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const bool first = tid < T && is_first(ids, tid);
+      if (tid < T && max(ids[tid], -1) != max(ids[0], -1)) mixed = 1;
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+      if (tid < 128 && lane == 0) in_warp[tid >> 5] = __popc(firsts);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      int at = __popc(firsts & ((1u << lane) - 1)), all = 0;
+      for (int w = 0; w < 4; ++w) {
+        if (w < tid >> 5) at += in_warp[w];
+        all += in_warp[w];
+      }
+      if (first) list[at] = tid;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tid == 0) {
+        in_warp[0] = all;
+        mbar_arrive(&list_full);
+      }
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int q = warp & 3;  // TMEM lane quarter
-    if (mbar_wait(&acc_full, 0, abort_flag, p.err, kErrWaitAccFull)) {
+    if (warp < 6 && mbar_wait(&acc_full, 0, abort_flag, p.err, kErrWaitAccFull)) {
       tc_fence_after();
-      float* mine = sums + (q * 32 + lane) * C_::PITCH;
+      const bool any = kb1 > kb0 || (g.rk.rc > 0 && my_chunks() > 0);
+      float* mine = sums + q * 32 + lane;
 #pragma unroll
       for (int c = 0; c < TN; c += 16) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mine[c + i] = kb1 > kb0 ? __uint_as_float(v[i]) : 0.0f;
+        for (int i = 0; i < 16; ++i) mine[(c + i) * 128] = any ? __uint_as_float(v[i]) : 0.0f;
       }
     }
   }
   tc_fence_before();
   __syncwarp();
   cluster_sync();  // every CTA's partial sums are in its shared memory
-  tc_fence_after();
   if (warp >= 2) {
-    const int tid = threadIdx.x - 64, R = 128 / splits;
-    const int row = tid % R;
+    // Rows [rank R, + R) of the tile, neighbouring threads neighbouring features: a warp reads
+    // 128 contiguous bytes of a peer (16-byte reads of 32 different rows took ten times as
+    // long). Four tokens of up to eight parts are in flight.
+    const int tid = threadIdx.x - 64, R = 128 / splits, row = tid % R, step = kSumThreads / R;
     const int64_t n = n0 + rank * R + row;
     if (n < p.N) {
       const float bias = p.bias ? p.bias[n] : 0.0f;
-      for (int t = tid / R; t < T; t += splits) {
-        const uint32_t at = smem_u32(sums + (rank * R + row) * C_::PITCH + t);
-        float y = 0.0f;
-        for (int s = 0; s < splits; ++s) {
-          uint32_t peer;
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(s));
-          y += ld_cluster_f32(peer);
+      const uint32_t base = smem_u32(sums + rank * R + row);
+      int spoilt = -1;  // whether an adapter's B is not finite in this feature
+      for (int t0 = tid / R; t0 < T; t0 += 4 * step) {
+        float y[4] = {bias, bias, bias, bias};
+#pragma unroll
+        for (int s0 = 0; s0 < 8; s0 += 4) {
+          if (s0 >= splits) break;
+          float part[4][4];
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            if (s0 + s < splits) {
+              const uint32_t peer = peer_addr(base, s0 + s);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) part[s][u] = ld_cluster_f32(peer + 512 * min(t0 + u * step, TN - 1));
+            }
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            if (s0 + s < splits)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) y[u] += part[s][u];
         }
-        y += bias + delta[row * C_::PITCH + t];
-        if (p.y_bf16)
-          ((uint16_t*)p.Y)[t * p.ldy + n] = f32_to_bf16_rne(y);
-        else
-          ((float*)p.Y)[t * p.ldy + n] = y;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int t = t0 + u * step;
+          if (t >= T) break;
+          if (mixed && !(fabsf(y[u]) < INFINITY)) {
+            // Zero times what is not finite in another row's adapter is NaN: such a value is
+            // computed again without the tensor core.
+            if (spoilt < 0) spoilt = spoilt_feature(g, ids, list, in_warp[0], n);
+            if (spoilt) y[u] = redo_value(g, ids, t, n, TN);
+          }
+          if (p.y_bf16)
+            ((uint16_t*)p.Y)[t * p.ldy + n] = f32_to_bf16_rne(y[u]);
+          else
+            ((float*)p.Y)[t * p.ldy + n] = y[u];
+        }
       }
     }
   }
@@ -240,7 +403,7 @@ __global__ void __launch_bounds__(kRowThreads)
 struct Operands {
   bool pack_x, pack_w, pack_a, pack_b;
   int64_t Kp, rb;  // pitches of packed rows
-  size_t x_at, w_at, a_at, b_at, h_at, bytes;
+  size_t x_at, w_at, a_at, b_at, h_at;
 };
 Operands lay_out(const LoraLinear& p) {
   Operands o{};
@@ -250,7 +413,7 @@ Operands lay_out(const LoraLinear& p) {
   o.pack_x = !p.x_bf16 || !aligned16(p.X) || p.ldx % 8 != 0;
   o.pack_w = !aligned16(p.W) || p.ldw % 8 != 0;
   o.pack_a = adapters && (!aligned16(p.A) || p.lda % 8 != 0);
-  o.pack_b = adapters && p.T > kMaxRowsSmall && (!aligned16(p.B) || p.ldb % 8 != 0);
+  o.pack_b = adapters && (!aligned16(p.B) || p.ldb % 8 != 0);
   size_t at = 0;
   auto take = [&](bool need, int64_t rows, int64_t pitch) {
     const size_t here = at;
@@ -262,68 +425,92 @@ Operands lay_out(const LoraLinear& p) {
   o.a_at = take(o.pack_a, p.n_adapters * p.r, o.Kp);
   o.b_at = take(o.pack_b, p.n_adapters * p.N, o.rb);
   o.h_at = at;
-  o.bytes = at + align256((size_t)(p.T * p.r) * 4);
   return o;
 }
 
+int rows_tile(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128; }
+RowsK lay_out_rows(const LoraLinear& p, uint8_t* at, size_t* bytes) {
+  RowsK k{};
+  k.cw = 64;
+  *bytes = 0;
+  if (p.n_adapters <= 0 || p.r <= 0) return k;
+  k.H = reinterpret_cast<uint16_t*>(at);
+  k.cw = chunk_width(p.r);
+  k.rc = (int)((p.r + k.cw - 1) / k.cw);
+  k.parts = p.y_bf16 ? 1 : 2;
+  *bytes = align256((size_t)(p.T * k.per() * rows_tile(p.T) * k.cw) * 2);
+  return k;
+}
+
+void map_2d(CUtensorMap* m, const void* x, int64_t k, int64_t rows, int64_t ld, int box_k, int box_rows,
+            CUtensorMapSwizzle sw) {
+  const uint64_t dims[2] = {(uint64_t)k, (uint64_t)rows};
+  const uint64_t str[1] = {(uint64_t)ld * 2};
+  const uint32_t box[2] = {(uint32_t)box_k, (uint32_t)box_rows};
+  encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, dims, str, box, sw);
+}
+// `rows` x `cols` of every adapter, one adapter at a time.
+void map_adapters(CUtensorMap* m, const void* x, int64_t cols, int64_t rows, int64_t n, int64_t ld, int box_cols, int box_rows,
+                  CUtensorMapSwizzle sw) {
+  const uint64_t dims[3] = {(uint64_t)cols, (uint64_t)rows, (uint64_t)n};
+  const uint64_t str[2] = {(uint64_t)ld * 2, (uint64_t)(rows * ld) * 2};
+  const uint32_t box[3] = {(uint32_t)box_cols, (uint32_t)box_rows, 1};
+  encode_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, x, dims, str, box, sw);
+}
+
 template <int TN>
-void launch_rows(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, const float* h) {
+void launch_rows(LoraRows g) {
   using C_ = RowsCfg<TN>;
   DeviceContext& c = ctx();
-  CUtensorMap tw, tx;
-  {
-    const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)p.N};
-    const uint64_t str[1] = {(uint64_t)ldw * 2};
-    const uint32_t box[2] = {64, 128};
-    encode_tmap(&tw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, W, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-  }
-  {
-    const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)p.T};
-    const uint64_t str[1] = {(uint64_t)ldx * 2};
-    const uint32_t box[2] = {64, (uint32_t)TN};
-    encode_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, X, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const LoraLinear& p = g.p;
+  const bool adapters = g.rk.rc > 0;
+  CUtensorMap tw, tx, tb, th;
+  map_2d(&tw, g.W, p.K, p.N, g.ldw, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  map_2d(&tx, g.X, p.K, p.T, g.ldx, 64, TN, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (adapters) {
+    map_adapters(&tb, g.B, p.r, p.N, p.n_adapters, g.ldb, g.rk.cw, 128, swizzle_of(g.rk.cw));
+    map_2d(&th, g.rk.H, g.rk.cw, p.T * g.rk.per() * TN, g.rk.cw, g.rk.cw, TN, swizzle_of(g.rk.cw));
+  } else {
+    tb = th = tx;  // no chunk is read
   }
   const int64_t tiles = (p.N + 127) / 128;
   const int kblocks = (int)((p.K + 63) / 64);
-  auto smem_of = [&](int s) {
-    return 1024 + C_::STAGES * C_::STAGE + 128 / s * C_::PITCH * 4 + (int)(p.T * p.r) * 4;
-  };
-  // K splits until two CTAs a processor (where they fit) have a part, of two K blocks at least.
-  int splits = 1;
-  while (splits < 8 && kblocks >= 4 * splits &&
-         tiles * splits * 2 <= (int64_t)c.num_sms * (smem_of(2 * splits) <= 113 * 1024 ? 2 : 1))
-    splits *= 2;
-  const int smem = smem_of(splits);
+  // K splits until two CTAs a processor have a part, of two K blocks at least.
+  g.splits = 1;
+  while (g.splits < 8 && kblocks >= 4 * g.splits && tiles * g.splits * 2 <= (int64_t)c.num_sms * 2) g.splits *= 2;
   static bool done[64] = {};
   if (!done[c.device]) {
-    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024),
+    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM),
+               "cudaFuncSetAttribute(linear_lora)");
+    // The default carve-out would hold one CTA a processor, and the rest would run after it.
+    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared),
                "cudaFuncSetAttribute(linear_lora)");
     done[c.device] = true;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * splits));
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3((unsigned)(tiles * g.splits));
+  cfg.blockDim = dim3(64 + kSumThreads);
+  cfg.dynamicSmemBytes = C_::SMEM;
   cfg.stream = c.stream;
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.x = (unsigned)g.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.r > 0 ? 2 : 1;  // only k_lora_down_rows may be overtaken
-  const int b_vec = p.r % 8 == 0 && p.ldb % 8 == 0 && aligned16(p.B);
-  check_cuda(cudaLaunchKernelEx(&cfg, k_lora_rows<TN>, tw, tx, p, h, p.B, p.ldb, splits, b_vec), "linear_lora");
+  cfg.numAttrs = adapters ? 2 : 1;  // only k_lora_down_rows may be overtaken
+  check_cuda(cudaLaunchKernelEx(&cfg, k_lora_rows<TN>, tw, tx, tb, th, (const LoraRows)g), "linear_lora");
   check_launch("linear_lora");
 }
 
 // ------------------------------------------------------------------------------------
-// Many rows: Y = [X | H] [W | B]^T as one GEMM, where H holds h in the columns of the row's
-// own adapter and zeros in those of the other adapters of its tile.
+// Many rows: Y = [X | H] [W | B]^T as one GEMM.
 // ------------------------------------------------------------------------------------
 constexpr int kGroup = 256;     // rows that share a list of adapters and a block of H
 constexpr int kMaxPass = 256;   // accumulator columns of k_lora_down
+constexpr int kHash = 512;
 
 struct GroupList {
   int count;            // distinct adapters of the rows
@@ -339,20 +526,6 @@ struct LoraK {
   __host__ __device__ int chunks(int count) const { return count * parts * rc; }
 };
 
-// K-major operand rows of `pitch` = 32, 64 or 128 bytes in the swizzle of that width.
-__device__ __forceinline__ uint64_t sdesc_k(uint32_t saddr, int pitch) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)1u << 16;
-  d |= (uint64_t)((uint32_t)(8 * pitch) >> 4) << 32;  // 8 rows
-  d |= (uint64_t)1u << 46;
-  d |= (uint64_t)(pitch == 128 ? 2u : pitch == 64 ? 4u : 6u) << 61;
-  return d;
-}
-inline CUtensorMapSwizzle swizzle_of(int cw) {
-  return cw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : cw == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-}
-
 // H of one tile of 128 rows: x A_a^T on tcgen05 for every adapter a of the group (an N of
 // rpr = round_up(r, 16) columns each, at most 256 a pass), K split over the cluster's CTAs.
 // Each row keeps the columns of its own adapter; the CTAs' parts are added in rank order.
@@ -360,7 +533,7 @@ inline CUtensorMapSwizzle swizzle_of(int cw) {
 struct DownCfg {
   static constexpr int X_BYTES = 128 * 128, A_BYTES = kMaxPass * 128, STAGE = X_BYTES + A_BYTES;
   static constexpr int MAX_STAGES = 4;
-  static int stages(int rpr) { return std::min(MAX_STAGES, (222 * 1024 - 128 * (rpr + 1) * 4) / STAGE); }
+  static int stages(int rpr) { return std::min(MAX_STAGES, (216 * 1024 - 128 * (rpr + 1) * 4) / STAGE); }
   static int smem(int rpr) { return 1024 + stages(rpr) * STAGE + 128 * (rpr + 1) * 4; }
 };
 
@@ -374,7 +547,7 @@ __global__ void __launch_bounds__(kRowThreads)
   float* sums = reinterpret_cast<float*>(smem + stages * C_::STAGE);  // [128][pitch]
   const int pitch = rpr + 1;
   __shared__ uint64_t full[C_::MAX_STAGES], empty[C_::MAX_STAGES], acc_full[2], acc_empty[2], drain;
-  __shared__ int ids[kGroup], slot[kGroup], rank_of[kGroup], list[kGroup], wsum[8], count, mixed;
+  __shared__ int ids[kGroup], slot[kGroup], rank_of[kGroup], list[kGroup], hash_key[kHash], hash_row[kHash], count, mixed;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -414,16 +587,31 @@ __global__ void __launch_bounds__(kRowThreads)
     if (t >= rows) a = -2;
     ids[i] = a;
   }
+  for (int i = threadIdx.x; i < kHash; i += kRowThreads) {
+    hash_key[i] = -1;
+    hash_row[i] = kGroup;
+  }
   __syncthreads();
+  // slot[i]: the first row with row i's adapter, through a hash table of the group's ids.
   for (int i = threadIdx.x; i < kGroup; i += kRowThreads) {
     const int a = ids[i];
-    int f = 0;
-    while (ids[f] != a) ++f;  // ends at i at the latest
-    slot[i] = f;
+    uint32_t at = ((uint32_t)a * 2654435761u) >> 23;
+    if (a >= 0) {
+      for (;; at = (at + 1) % kHash) {
+        const int k = atomicCAS(&hash_key[at], -1, a);
+        if (k == -1 || k == a) break;  // at most kGroup of kHash places are taken
+      }
+      atomicMin(&hash_row[at], i);
+    }
+    slot[i] = (int)at;
     if (a != -2 && a != ids[0]) mixed = 1;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kGroup; i += kRowThreads) rank_of[i] = slot[i] == i && ids[i] >= 0;
+  for (int i = threadIdx.x; i < kGroup; i += kRowThreads) {
+    const int f = ids[i] >= 0 ? hash_row[slot[i]] : i;
+    rank_of[i] = f == i && ids[i] >= 0;
+    slot[i] = f;
+  }
   __syncthreads();
   if (warp < 1) {  // exclusive prefix over the 256 flags, 8 per lane
     int n = 0, f[8];
@@ -545,38 +733,43 @@ __global__ void __launch_bounds__(kRowThreads)
   __syncwarp();
   cluster_sync();
   if (warp >= 2) {
-    // This CTA's share of the rows: 8 ranks of one chunk per step and thread.
-    const int share = 128 / splits, pieces = lk.cw / 8, nq = lk.chunks(m);
-    for (int i = threadIdx.x - 64; i < share * pieces * nq; i += 128) {
-      const int pc = i % pieces, rr = rank * share + i / pieces % share, qi = i / (pieces * share);
-      const int c = qi % lk.rc, part = qi / lk.rc % lk.parts, sl = qi / (lk.rc * lk.parts);
-      const int me = half * 128 + rr, a = ids[me];
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (a >= 0 && rank_of[slot[me]] == sl) {
-        const float scale = p.scale ? p.scale[a] : 1.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = c * lk.cw + pc * 8 + e;
-          float v = 0.0f;
-          if (j < p.r) {
-            const uint32_t at = smem_u32(sums + rr * pitch + j);
-            for (int s = 0; s < splits; ++s) {
-              uint32_t peer;
-              asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(s));
-              v += ld_cluster_f32(peer);
-            }
-            v *= scale;
-          }
-          uint32_t b = f32_to_bf16_rne(v);
-          if (part) {  // what bf16 lost: h = high + low to 2^-16
-            const float hi = bf16_to_f32((uint16_t)b);
-            b = f32_to_bf16_rne(fabsf(hi) < INFINITY ? v - hi : 0.0f);
-          }
-          w[e >> 1] |= b << (16 * (e & 1));
+    // This CTA's share of the rows. First their sums over the cluster, scaled, into the
+    // stages' memory (every copy and MMA is done), then H: 16 bytes per store.
+    const int share = 128 / splits, tid = threadIdx.x - 64;
+    float* fin = reinterpret_cast<float*>(smem);  // [share][pitch]
+    for (int rr = tid / 32; rr < share; rr += 4) {
+      const int me = half * 128 + rank * share + rr, a = ids[me];
+      if (a < 0) continue;
+      const float scale = p.scale ? p.scale[a] : 1.0f;
+      for (int j = lane; j < rpr; j += 32) {
+        const uint32_t at = smem_u32(sums + (rank * share + rr) * pitch + j);
+        float v = 0.0f;
+        for (int s = 0; s < splits; ++s) {
+          uint32_t peer;
+          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(s));
+          v += ld_cluster_f32(peer);
         }
+        fin[rr * pitch + j] = v * scale;
       }
-      uint16_t* dst = lk.H + (((int64_t)group * lk.q_max + qi) * kGroup + me) * lk.cw + pc * 8;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int lgp = lk.cw == 16 ? 1 : lk.cw == 32 ? 2 : 3, nq = lk.chunks(m), per = lk.parts * lk.rc;
+    for (int x = tid; x < share << lgp; x += 128) {
+      const int rr = x >> lgp, pc = x & ((1 << lgp) - 1), me = half * 128 + rank * share + rr;
+      const int q0 = ids[me] >= 0 ? rank_of[slot[me]] * per : -per;
+      uint16_t* dst = lk.H + ((int64_t)group * lk.q_max * kGroup + me) * lk.cw + pc * 8;
+      for (int qi = 0; qi < nq; ++qi, dst += (int64_t)kGroup * lk.cw) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (qi >= q0 && qi < q0 + per) {
+          const int part = qi - q0 >= lk.rc, c = qi - q0 - part * lk.rc;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = c * lk.cw + pc * 8 + e;
+            w[e >> 1] |= h_part(j < p.r ? fin[rr * pitch + j] : 0.0f, part) << (16 * (e & 1));
+          }
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
   __syncwarp();
@@ -944,27 +1137,16 @@ template <int BN, bool PAIR>
 void launch_lora_gemm(LoraGemm g, int64_t r, bool overlap) {
   using C_ = LoraGemmCfg<BN, PAIR>;
   DeviceContext& c = ctx();
-  const CUtensorMapDataType bf = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tx, tw, th, tb;
-  auto map2 = [&](CUtensorMap* m, const void* x, int64_t k, int64_t rows, int64_t ld, int box_k, int box_rows,
-                  CUtensorMapSwizzle sw) {
-    const uint64_t dims[2] = {(uint64_t)k, (uint64_t)rows};
-    const uint64_t str[1] = {(uint64_t)ld * 2};
-    const uint32_t box[2] = {(uint32_t)box_k, (uint32_t)box_rows};
-    encode_tmap(m, bf, 2, x, dims, str, box, sw);
-  };
-  map2(&tx, g.X, g.p.K, g.p.T, g.ldx, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-  map2(&tw, g.W, g.p.K, g.p.N, g.ldw, 64, C_::B_ROWS, CU_TENSOR_MAP_SWIZZLE_128B);
+  map_2d(&tx, g.X, g.p.K, g.p.T, g.ldx, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  map_2d(&tw, g.W, g.p.K, g.p.N, g.ldw, 64, C_::B_ROWS, CU_TENSOR_MAP_SWIZZLE_128B);
   g.m_tiles = (int)((g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
   g.n_tiles = (int)((g.p.N + BN - 1) / BN);
   g.k_blocks = (int)((g.p.K + 63) / 64);
   if (overlap) {
     const int64_t groups = (g.rows + kGroup - 1) / kGroup;
-    map2(&th, g.lk.H, g.lk.cw, groups * g.lk.q_max * kGroup, g.lk.cw, g.lk.cw, 128, swizzle_of(g.lk.cw));
-    const uint64_t dims[3] = {(uint64_t)r, (uint64_t)g.p.N, (uint64_t)g.p.n_adapters};
-    const uint64_t str[2] = {(uint64_t)g.ldb * 2, (uint64_t)g.p.N * g.ldb * 2};
-    const uint32_t box[3] = {(uint32_t)g.lk.cw, (uint32_t)C_::B_ROWS, 1};
-    encode_tmap(&tb, bf, 3, g.B, dims, str, box, swizzle_of(g.lk.cw));
+    map_2d(&th, g.lk.H, g.lk.cw, groups * g.lk.q_max * kGroup, g.lk.cw, g.lk.cw, 128, swizzle_of(g.lk.cw));
+    map_adapters(&tb, g.B, r, g.p.N, g.p.n_adapters, g.ldb, g.lk.cw, C_::B_ROWS, swizzle_of(g.lk.cw));
   } else {
     th = tb = tx;  // no chunk is read
   }
@@ -1017,7 +1199,7 @@ Big lay_out_big(const LoraLinear& p, size_t at) {
   b.lk.cw = 64;
   if (p.n_adapters <= 0 || p.r <= 0) return b;
   b.lk.parts = p.y_bf16 ? 1 : 2;
-  b.lk.cw = p.r <= 16 ? 16 : p.r <= 32 ? 32 : 64;
+  b.lk.cw = chunk_width(p.r);
   b.lk.rc = (int)((p.r + b.lk.cw - 1) / b.lk.cw);
   b.lk.q_max = b.lk.chunks((int)std::min<int64_t>(p.n_adapters, kGroup));
   // H holds every chunk a group could need; blocks of rows keep it within 128 MB.
@@ -1050,25 +1232,15 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
     if (adapters) {
       const int rpr = (int)round_up(p.r, 16), stages = DownCfg::stages(rpr);
       CUtensorMap tx, ta;
-      {
-        const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)p.T};
-        const uint64_t str[1] = {(uint64_t)ldx * 2};
-        const uint32_t box[2] = {64, 128};
-        encode_tmap(&tx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, X, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-      }
-      {
-        const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.r, (uint64_t)p.n_adapters};
-        const uint64_t str[2] = {(uint64_t)lda * 2, (uint64_t)p.r * lda * 2};
-        const uint32_t box[3] = {64, (uint32_t)rpr, 1};
-        encode_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, A, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-      }
+      map_2d(&tx, X, p.K, p.T, ldx, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+      map_adapters(&ta, A, p.K, p.r, p.n_adapters, lda, 64, rpr, CU_TENSOR_MAP_SWIZZLE_128B);
       const int64_t tiles = 2 * ((g.rows + kGroup - 1) / kGroup);
       const int kblocks = (int)((p.K + 63) / 64);
       int splits = 1;
       while (splits < 8 && tiles * splits * 2 <= c.num_sms && kblocks >= 4 * splits) splits *= 2;
       static bool done[64] = {};
       if (!done[c.device]) {
-        check_cuda(cudaFuncSetAttribute(k_lora_down, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024),
+        check_cuda(cudaFuncSetAttribute(k_lora_down, cudaFuncAttributeMaxDynamicSharedMemorySize, 218 * 1024),
                    "cudaFuncSetAttribute(lora_down)");
         done[c.device] = true;
       }
@@ -1089,24 +1261,36 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
       check_launch("lora_down");
     }
     // Tile shape by waves, as gemm_tc.cu prices them: a tile costs its width and 48 columns
-    // of fixed cost, a 256 x 256 pair tile 8% less.
-    auto waves = [&](int bm, int bn, int64_t units) {
+    // of fixed cost, a pair tile (256 rows over two processors) 8% less. Several pair widths,
+    // because a few rows of tiles leave the last wave nearly empty: 2397 x 4096 outputs are
+    // 2.2 waves of 256 columns (3 x 280) but 3.0 waves of 192 (3 x 221).
+    auto cost = [&](int bm, int bn, int64_t units) {
       const int64_t t = ((g.rows + bm - 1) / bm) * ((p.N + bn - 1) / bn);
-      return (double)((t + units - 1) / units);
+      return (double)((t + units - 1) / units) * (bn + 48) * (bm == 256 ? 0.92 : 1.0);
     };
-    double best = g.rows > 128 ? waves(256, 256, c.num_sms / 2) * (256 + 48) * 0.92 : 1e30;
-    int bn = 0;
-    for (int cand : {256, 128, 64}) {
-      const double cost = waves(128, cand, c.num_sms) * (cand + 48);
-      if (cost < best) {
-        best = cost;
-        bn = cand;
+    double best = 1e30;
+    int bm = 128, bn = 64;
+    for (int cand : {256, 224, 192, 160, 128, 64})
+      for (int rows : {256, 128}) {
+        if (rows == 256 ? cand == 64 || g.rows <= 128 : cand != 256 && cand != 128 && cand != 64) continue;
+        const double x = cost(rows, cand, rows == 256 ? c.num_sms / 2 : c.num_sms);
+        if (x < best - 1e-9) {
+          best = x;
+          bm = rows;
+          bn = cand;
+        }
       }
+    if (bm == 256) {
+      if (bn == 256) launch_lora_gemm<256, true>(g, p.r, adapters);
+      if (bn == 224) launch_lora_gemm<224, true>(g, p.r, adapters);
+      if (bn == 192) launch_lora_gemm<192, true>(g, p.r, adapters);
+      if (bn == 160) launch_lora_gemm<160, true>(g, p.r, adapters);
+      if (bn == 128) launch_lora_gemm<128, true>(g, p.r, adapters);
+    } else {
+      if (bn == 256) launch_lora_gemm<256, false>(g, p.r, adapters);
+      if (bn == 128) launch_lora_gemm<128, false>(g, p.r, adapters);
+      if (bn == 64) launch_lora_gemm<64, false>(g, p.r, adapters);
     }
-    if (bn == 0) launch_lora_gemm<256, true>(g, p.r, adapters);
-    if (bn == 256) launch_lora_gemm<256, false>(g, p.r, adapters);
-    if (bn == 128) launch_lora_gemm<128, false>(g, p.r, adapters);
-    if (bn == 64) launch_lora_gemm<64, false>(g, p.r, adapters);
   }
 }
 
@@ -1114,7 +1298,10 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
 
 size_t lora_linear_workspace(const LoraLinear& p) {
   const Operands o = lay_out(p);
-  return p.T <= kMaxRowsSmall ? o.bytes : lay_out_big(p, o.h_at).bytes;
+  if (p.T > kMaxRowsSmall) return lay_out_big(p, o.h_at).bytes;
+  size_t h;
+  lay_out_rows(p, nullptr, &h);
+  return o.h_at + h;
 }
 
 void launch_lora_linear(LoraLinear p, void* ws_) {
@@ -1149,17 +1336,17 @@ void launch_lora_linear(LoraLinear p, void* ws_) {
     ldb = o.rb;
   }
   if (p.T > kMaxRowsSmall) return launch_big(p, X, ldx, W, ldw, A, lda, B, ldb, ws, lay_out_big(p, o.h_at));
-  float* h = reinterpret_cast<float*>(ws + o.h_at);
-  if (p.n_adapters <= 0 || p.r <= 0) {
-    p.n_adapters = p.r = 0;
-    p.row_adapter = nullptr;
-  } else {
-    k_lora_down_rows<<<dim3((unsigned)p.T, (unsigned)((p.r + 7) / 8)), 256, 0, c.stream>>>(p, X, ldx, A, lda, h);
+  size_t h;
+  LoraRows g{p, lay_out_rows(p, ws + o.h_at, &h), X, W, B, ldx, ldw, ldb, 1};
+  const int tn = rows_tile(p.T);
+  if (g.rk.rc > 0) {
+    k_lora_down_rows<<<dim3((unsigned)p.T, (unsigned)(g.rk.rc * g.rk.cw / 8)), 256, 0, c.stream>>>(p, X, ldx, A, lda, g.rk, tn);
     check_launch("lora_down_rows");
   }
-  if (p.T <= 16) return launch_rows<16>(p, X, ldx, W, ldw, h);
-  if (p.T <= 32) return launch_rows<32>(p, X, ldx, W, ldw, h);
-  launch_rows<64>(p, X, ldx, W, ldw, h);
+  if (tn == 16) return launch_rows<16>(g);
+  if (tn == 32) return launch_rows<32>(g);
+  if (tn == 64) return launch_rows<64>(g);
+  launch_rows<128>(g);
 }
 
 }  // namespace sdb
