@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {  // the whole warp: an elected lane issues
       int done = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb, ++done) {
@@ -272,10 +272,8 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
         if (!ok) break;
         tc_fence_after();
         const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f16_ss(tmem, sdesc_k_sw128(a0 + k * 32), sdesc_k_sw128(b0 + k * 32), IDESC, kb > kb0 || k > 0);
-        umma_commit(&empty[s]);
+        umma4_elect(tmem, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb > kb0);
+        umma_commit_elect(&empty[s]);
       }
       if (ok && g.rk.rc > 0 && mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull)) {
         const int nq = my_chunks();
@@ -286,16 +284,16 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
           const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
           for (int i = 0; i < min(per_stage, nq - q0); ++i)
             for (int k = 0; k < g.rk.cw / 16; ++k)
-              umma_f16_ss(tmem, sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), sdesc_k(b0 + i * TN * cwb + k * 32, cwb), IDESC,
+              umma_elect(tmem, sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), sdesc_k(b0 + i * TN * cwb + k * 32, cwb), IDESC,
                           kb1 > kb0 || q0 + i + k > 0);
-          umma_commit(&empty[s]);
+          umma_commit_elect(&empty[s]);
         }
       }
-      umma_commit(&acc_full);
+      umma_commit_elect(&acc_full);
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(&acc_full, 0))
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
-          atomicOr(p.err, kErrWaitDrain);
+          if (lane == 0) atomicOr(p.err, kErrWaitDrain);
           break;
         }
     }
@@ -971,20 +969,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {  // the whole warp: an elected lane issues
       int done = 0, n = 0;
       bool ok = true;
-      auto mma = [&](uint32_t d, uint64_t a, uint64_t b, bool acc) {
-        if constexpr (PAIR)
-          umma_f16_ss_pair(d, a, b, IDESC, acc);
-        else
-          umma_f16_ss(d, a, b, IDESC, acc);
-      };
       auto commit = [&](uint64_t* bar) {
         if constexpr (PAIR)
-          umma_commit_pair(bar, 0x3);
+          umma_commit_pair_elect(bar, 0x3);
         else
-          umma_commit(bar);
+          umma_commit_elect(bar);
       };
       for (int t = unit; t < tiles && ok; t += units, ++n) {
         const int acc = n & 1;
@@ -1000,8 +992,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma(d, sdesc_k_sw128(a0 + k * 32), sdesc_k_sw128(b0 + k * 32), (kb | k) != 0);
+          if constexpr (PAIR)
+            umma4_pair_elect(d, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb != 0);
+          else
+            umma4_elect(d, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb != 0);
           commit(&empty[s]);
         }
         if (!ok) break;
@@ -1014,8 +1008,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
           for (int i = 0; i < min(per_stage, nq - q0); ++i)
-            for (int k = 0; k < cw / 16; ++k)
-              mma(d, sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), sdesc_k(b0 + i * C_::B_ROWS * cwb + k * 32, cwb), true);
+            for (int k = 0; k < cw / 16; ++k) {
+              const uint64_t ad = sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), bd = sdesc_k(b0 + i * C_::B_ROWS * cwb + k * 32, cwb);
+              if constexpr (PAIR)
+                umma_pair_elect(d, ad, bd, IDESC, 1u);
+              else
+                umma_elect(d, ad, bd, IDESC, 1u);
+            }
           commit(&empty[s]);
         }
         if (!ok) break;

@@ -373,6 +373,81 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
                : "memory");
 }
 
+// ---- issue by one elected lane of a converged warp -------------------------------------
+// The descriptors of an MMA are read from uniform registers. Where the issuing code runs under
+// `if (lane == 0)`, ptxas must move every descriptor there first; here the whole warp runs
+// the code, values stay uniform, and only the instruction itself is predicated on the
+// elected lane (the same one every time, so its commits cover its MMAs). Measured in a
+// 256 x 256 pair GEMM: about 390 cycles to issue a K block of four MMAs from one lane, which
+// is more than the tensor core needs for 128 columns.
+//
+// Four kind::f16 MMAs along K, both operands K-major in a 128-byte swizzle (32 bytes = 2
+// descriptor units per step); the first accumulates iff acc_first.
+__device__ __forceinline__ void umma4_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first) {
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc_first)
+      : "memory");
+}
+__device__ __forceinline__ void umma4_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first) {
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc_first)
+      : "memory");
+}
+// One MMA.
+__device__ __forceinline__ void umma_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred q, p;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred q, p;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// umma_commit / umma_commit_pair by the elected lane.
+__device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_pair_elect(uint64_t* bar, uint16_t cta_mask) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "h"(cta_mask)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
