@@ -3,8 +3,9 @@
 //   h[t, j] = s_a sum_k x[t, k] A_a[j, k],   a = row_adapter[t] (no second term for a < 0).
 //
 // Up to 128 rows the work is reading W and the adapters once (k_lora_down_rows, k_lora_rows);
-// above, it is a GEMM (k_lora_down, k_lora_gemm).
+// above, it is a GEMM (k_lora_lists, k_lora_gemm).
 #include <algorithm>
+#include <cmath>
 
 #include "elem.cuh"
 #include "internal.h"
@@ -225,32 +226,37 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
   // This CTA's chunks: those of the listed adapters whose number is rank modulo splits.
   auto my_chunks = [&]() { return (in_warp[0] * g.rk.per() - rank + splits - 1) / splits; };
   if (warp == 0) {
-    if (lane == 0) {
+    {  // the whole warp: an elected lane issues
+      RingPos at;
       int done = 0;
       bool ok = true;
+      const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(&full[0]);
       auto stage = [&](int bytes) {
-        ok = mbar_wait(&empty[done % C_::STAGES], ((done / C_::STAGES) & 1) ^ 1u, abort_flag, p.err, kErrWaitEmpty);
-        if (ok) mbar_arrive_expect_tx(&full[done % C_::STAGES], bytes);
-        return smem + done % C_::STAGES * C_::STAGE;
+        ok = mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, p.err, kErrWaitEmpty);
+        if (ok) {
+          mbar_expect_tx_elect(full0 + (uint32_t)(at.slot * 8), (uint32_t)bytes);
+          ++done;
+        }
+        return smem0 + (uint32_t)(at.slot * C_::STAGE);
       };
-      for (int kb = kb0; kb < kb1; ++kb, ++done) {
-        uint8_t* st = stage(C_::STAGE);
+      for (int kb = kb0; kb < kb1; ++kb, at.next(C_::STAGES)) {
+        const uint32_t st = stage(C_::STAGE);
         if (!ok) break;
-        tma_load_2d(st, &tmW, &full[done % C_::STAGES], kb * 64, (int)n0);
-        tma_load_2d(st + C_::W_BYTES, &tmX, &full[done % C_::STAGES], kb * 64, 0);
+        tma_load_2d_elect(st, &tmW, full0 + (uint32_t)(at.slot * 8), kb * 64, (int)n0);
+        tma_load_2d_elect(st + C_::W_BYTES, &tmX, full0 + (uint32_t)(at.slot * 8), kb * 64, 0);
       }
       if (ok && g.rk.rc > 0) {
         ok = mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull);
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int nq = ok ? my_chunks() : 0;
-        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
+        for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(C_::STAGES)) {
           const int n = min(per_stage, nq - q0);
-          uint8_t* st = stage(n * (128 + TN) * cwb);
+          const uint32_t st = stage(n * (128 + TN) * cwb), bar = full0 + (uint32_t)(at.slot * 8);
           if (!ok) break;
           for (int i = 0; i < n; ++i) {
             const int q = (q0 + i) * splits + rank, f = list[q / g.rk.per()], sub = q % g.rk.per();
-            tma_load_3d(st + i * 128 * cwb, &tmB, &full[done % C_::STAGES], sub % g.rk.rc * g.rk.cw, (int)n0, ids[f]);
-            tma_load_2d(st + C_::W_BYTES + i * TN * cwb, &tmH, &full[done % C_::STAGES], 0, (f * g.rk.per() + sub) * TN);
+            tma_load_3d_elect(st + i * 128 * cwb, &tmB, bar, sub % g.rk.rc * g.rk.cw, (int)n0, ids[f]);
+            tma_load_2d_elect(st + C_::W_BYTES + i * TN * cwb, &tmH, bar, 0, (f * g.rk.per() + sub) * TN);
           }
         }
       }
@@ -264,22 +270,22 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
     }
   } else if (warp == 1) {
     {  // the whole warp: an elected lane issues
-      int done = 0;
+      RingPos at;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb, ++done) {
-        const int s = done % C_::STAGES;
-        ok = mbar_wait(&full[s], (done / C_::STAGES) & 1, abort_flag, p.err, kErrWaitFull);
+      const uint64_t ad0 = sdesc_k_sw128(smem_u32(smem)), bd0 = sdesc_k_sw128(smem_u32(smem) + C_::W_BYTES);
+      const uint32_t empty0 = smem_u32(&empty[0]);
+      for (int kb = kb0; kb < kb1; ++kb, at.next(C_::STAGES)) {
+        ok = mbar_wait(&full[at.slot], at.phase, abort_flag, p.err, kErrWaitFull);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
-        umma4_elect(tmem, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb > kb0);
-        umma_commit_elect(&empty[s]);
+        const uint64_t off = (uint64_t)(at.slot * (C_::STAGE >> 4));
+        umma4_elect(tmem, ad0 + off, bd0 + off, IDESC, kb > kb0, empty0 + 8 * at.slot);
       }
       if (ok && g.rk.rc > 0 && mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull)) {
         const int nq = my_chunks();
-        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
-          const int s = done % C_::STAGES;
-          if (!mbar_wait(&full[s], (done / C_::STAGES) & 1, abort_flag, p.err, kErrWaitFull)) break;
+        for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(C_::STAGES)) {
+          const int s = at.slot;
+          if (!mbar_wait(&full[s], at.phase, abort_flag, p.err, kErrWaitFull)) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
           for (int i = 0; i < min(per_stage, nq - q0); ++i)
@@ -506,273 +512,95 @@ void launch_rows(LoraRows g) {
 // ------------------------------------------------------------------------------------
 // Many rows: Y = [X | H] [W | B]^T as one GEMM.
 // ------------------------------------------------------------------------------------
-constexpr int kGroup = 256;     // rows that share a list of adapters and a block of H
-constexpr int kMaxPass = 256;   // accumulator columns of k_lora_down
+constexpr int kGroup = 256;  // rows that share a list of adapters and a block of H
 constexpr int kHash = 512;
 
 struct GroupList {
-  int count;            // distinct adapters of the rows
-  int mixed;            // rows of different adapters, or some of none
-  int adapter[kGroup];  // in the order of their first rows
+  int count;             // distinct adapters of the rows
+  int mixed;             // rows of different adapters, or some of none
+  int adapter[kGroup];   // in the order of their first rows
+  int16_t slot[kGroup];  // each row's place in that order, -1: no adapter
 };
-// H: [groups][q_max][kGroup][cw] bf16. A chunk q of a group is cw ranks of one adapter (and,
-// with two parts, of the high or low half of h): q = (slot * parts + part) * rc + c.
+// H: [groups][q_max][kGroup][cw] bf16, chunk q = (slot * parts + part) * rc + c of a group.
 struct LoraK {
-  const GroupList* lists;
+  GroupList* lists;
+  int* done;  // warps of k_lora_gemm that have stored their part of H
   uint16_t* H;
   int cw, rc, parts, q_max;
   __host__ __device__ int chunks(int count) const { return count * parts * rc; }
 };
 
-// H of one tile of 128 rows: x A_a^T on tcgen05 for every adapter a of the group (an N of
-// rpr = round_up(r, 16) columns each, at most 256 a pass), K split over the cluster's CTAs.
-// Each row keeps the columns of its own adapter; the CTAs' parts are added in rank order.
-// Reading X bounds it: 128 x K bf16 per tile, once per 256 columns of adapters.
-struct DownCfg {
-  static constexpr int X_BYTES = 128 * 128, A_BYTES = kMaxPass * 128, STAGE = X_BYTES + A_BYTES;
-  static constexpr int MAX_STAGES = 4;
-  static int stages(int rpr) { return std::min(MAX_STAGES, (216 * 1024 - 128 * (rpr + 1) * 4) / STAGE); }
-  static int smem(int rpr) { return 1024 + stages(rpr) * STAGE + 128 * (rpr + 1) * 4; }
-};
-
-__global__ void __launch_bounds__(kRowThreads)
-    k_lora_down(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmA,
-                const __grid_constant__ LoraLinear p, const LoraK lk, GroupList* __restrict__ lists, int rpr, int stages,
-                int splits, int64_t row0, int64_t rows) {
-  using C_ = DownCfg;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sums = reinterpret_cast<float*>(smem + stages * C_::STAGE);  // [128][pitch]
-  const int pitch = rpr + 1;
-  __shared__ uint64_t full[C_::MAX_STAGES], empty[C_::MAX_STAGES], acc_full[2], acc_empty[2], drain;
-  __shared__ int ids[kGroup], slot[kGroup], rank_of[kGroup], list[kGroup], hash_key[kHash], hash_row[kHash], count, mixed;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
-  volatile int* abort_flag = &abort_word;
+// The distinct adapters of a group's rows, through a hash table.
+__global__ void __launch_bounds__(kGroup) k_lora_lists(const LoraLinear p, const LoraK lk, int64_t row0, int64_t rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits, group = tile >> 1, half = tile & 1;
-  const int kblocks = (int)((p.K + 63) / 64);
-  const int kb0 = (int)((int64_t)kblocks * rank / splits), kb1 = (int)((int64_t)kblocks * (rank + 1) / splits);
+  __shared__ int hash_key[kHash], hash_row[kHash], first_at[kGroup], in_warp[kGroup / 32], mixed;
+  const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
+  const int64_t t = (int64_t)blockIdx.x * kGroup + i;
+  GroupList& L = lk.lists[blockIdx.x];
+  for (int h = i; h < kHash; h += kGroup) {
+    hash_key[h] = -1;
+    hash_row[h] = kGroup;
+  }
+  if (i == 0) mixed = 0;
+  if (i == 0 && blockIdx.x == 0) *lk.done = 0;
+  int a = t < rows ? p.row_adapter[row0 + t] : -1;
+  if (a >= p.n_adapters) {
+    atomicOr(p.err, kErrBadIndex);
+    a = -1;
+  }
+  a = max(a, -1);
+  __syncthreads();
+  uint32_t at = ((uint32_t)a * 2654435761u) >> 23;
+  if (a >= 0) {
+    for (;; at = (at + 1) % kHash) {
+      const int k = atomicCAS(&hash_key[at], -1, a);
+      if (k == -1 || k == a) break;  // at most kGroup of kHash places are taken
+    }
+    atomicMin(&hash_row[at], i);
+  }
+  first_at[i] = a;
+  __syncthreads();
+  if (t < rows && a != first_at[0]) mixed = 1;
+  const int f = a >= 0 ? hash_row[at] : -1;  // the first row of this adapter
+  const bool first = f == i;
+  const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) in_warp[warp] = __popc(firsts);
+  __syncthreads();
+  int place = __popc(firsts & ((1u << lane) - 1)), all = 0;
+  for (int w = 0; w < kGroup / 32; ++w) {
+    if (w < warp) place += in_warp[w];
+    all += in_warp[w];
+  }
+  if (first) {
+    first_at[i] = place;
+    L.adapter[place] = a;
+  }
+  __syncthreads();
+  L.slot[i] = (int16_t)(a >= 0 ? first_at[f] : -1);
+  if (i == 0) {
+    L.count = all;
+    L.mixed = mixed;
+  }
+}
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
-    }
-    mbar_init(&drain, 1);
-    abort_word = 0;
-    mixed = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(&tmem_slot, 512);
-    tmem_relinquish();
-  }
-  // The group's distinct adapters, in the order of their first rows.
-  for (int i = threadIdx.x; i < kGroup; i += kRowThreads) {
-    const int64_t t = (int64_t)group * kGroup + i;
-    int a = t < rows ? p.row_adapter[row0 + t] : -2;  // -2: no row
-    if (a >= p.n_adapters) {
-      if (rank == 0 && half == 0) atomicOr(p.err, kErrBadIndex);
-      a = -1;
-    }
-    if (a < 0 && a != -2) a = -1;
-    if (t >= rows) a = -2;
-    ids[i] = a;
-  }
-  for (int i = threadIdx.x; i < kHash; i += kRowThreads) {
-    hash_key[i] = -1;
-    hash_row[i] = kGroup;
-  }
-  __syncthreads();
-  // slot[i]: the first row with row i's adapter, through a hash table of the group's ids.
-  for (int i = threadIdx.x; i < kGroup; i += kRowThreads) {
-    const int a = ids[i];
-    uint32_t at = ((uint32_t)a * 2654435761u) >> 23;
-    if (a >= 0) {
-      for (;; at = (at + 1) % kHash) {
-        const int k = atomicCAS(&hash_key[at], -1, a);
-        if (k == -1 || k == a) break;  // at most kGroup of kHash places are taken
-      }
-      atomicMin(&hash_row[at], i);
-    }
-    slot[i] = (int)at;
-    if (a != -2 && a != ids[0]) mixed = 1;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kGroup; i += kRowThreads) {
-    const int f = ids[i] >= 0 ? hash_row[slot[i]] : i;
-    rank_of[i] = f == i && ids[i] >= 0;
-    slot[i] = f;
-  }
-  __syncthreads();
-  if (warp < 1) {  // exclusive prefix over the 256 flags, 8 per lane
-    int n = 0, f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = rank_of[lane * 8 + i];
-      n += f[i];
-    }
-    int x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    int at = x - n;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (f[i]) list[at] = ids[lane * 8 + i];
-      rank_of[lane * 8 + i] = at;
-      at += f[i];
-    }
-    if (lane == 31) count = x;
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const int m = count, per_pass = kMaxPass / rpr, passes = (m + per_pass - 1) / per_pass;
-  if (rank == 0 && half == 0) {
-    for (int i = threadIdx.x; i < m; i += kRowThreads) lists[group].adapter[i] = list[i];
-    if (threadIdx.x == 0) {
-      lists[group].count = m;
-      lists[group].mixed = mixed;
+// Waits (bounded) until *flag, counted up by other CTAs of this launch, reaches want.
+__device__ __forceinline__ int ld_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool wait_count(const int* flag, int want, volatile int* abort_flag, int* err) {
+  if (ld_acquire(flag) >= want) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    if (ld_acquire(flag) >= want) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      atomicOr(err, kErrWaitFull);
+      return false;
     }
   }
-  if (warp == 0) {
-    if (lane == 0) {
-      int done = 0;
-      bool ok = true;
-      for (int ps = 0; ps < passes && ok; ++ps) {
-        const int s0 = ps * per_pass, used = min(per_pass, m - s0);
-        for (int kb = kb0; kb < kb1; ++kb, ++done) {
-          const int s = done % stages;
-          ok = mbar_wait(&empty[s], ((done / stages) & 1) ^ 1u, abort_flag, p.err, kErrWaitEmpty);
-          if (!ok) break;
-          uint8_t* st = smem + s * C_::STAGE;
-          mbar_arrive_expect_tx(&full[s], C_::X_BYTES + used * rpr * 128);
-          tma_load_2d(st, &tmX, &full[s], kb * 64, (int)(row0 + (int64_t)tile * 128));
-          for (int i = 0; i < used; ++i)
-            tma_load_3d(st + C_::X_BYTES + i * rpr * 128, &tmA, &full[s], kb * 64, 0, list[s0 + i]);
-        }
-      }
-      if (!ok) {
-        const uint64_t t0 = globaltimer_ns();
-        for (int i = max(0, done - stages); i < done; ++i)
-          while (!mbar_try_wait(&full[i % stages], (i / stages) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
-          }
-      }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int done = 0;
-      bool ok = true;
-      for (int ps = 0; ps < passes && ok; ++ps) {
-        const int acc = ps & 1, used = min(per_pass, m - ps * per_pass);
-        const uint32_t idesc = make_idesc(1u, 0, 0, 128, (uint32_t)(used * rpr)), d = tmem + (uint32_t)(acc * kMaxPass);
-        ok = mbar_wait(&acc_empty[acc], ((ps >> 1) & 1) ^ 1u, abort_flag, p.err, kErrWaitAccEmpty);
-        if (!ok) break;
-        tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++done) {
-          const int s = done % stages;
-          ok = mbar_wait(&full[s], (done / stages) & 1, abort_flag, p.err, kErrWaitFull);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::X_BYTES;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ss(d, sdesc_k_sw128(a0 + k * 32), sdesc_k_sw128(b0 + k * 32), idesc, kb > kb0 || k > 0);
-          umma_commit(&empty[s]);
-        }
-        if (!ok) break;
-        umma_commit(&acc_full[acc]);
-      }
-      umma_commit(&drain);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(&drain, 0))
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
-          atomicOr(p.err, kErrWaitDrain);
-          break;
-        }
-    }
-  } else {
-    const int q = warp & 3, rr = q * 32 + lane, me = half * 128 + rr;
-    const int mine = ids[me] >= 0 ? rank_of[slot[me]] : -1;
-    float* row = sums + rr * pitch;
-    for (int ps = 0; ps < passes; ++ps) {
-      const int acc = ps & 1, s0 = ps * per_pass, used = min(per_pass, m - s0);
-      if (!mbar_wait(&acc_full[acc], (ps >> 1) & 1, abort_flag, p.err, kErrWaitAccFull)) break;
-      tc_fence_after();
-      for (int i = 0; i < used; ++i) {
-        if (!__any_sync(0xffffffffu, mine == s0 + i)) continue;
-        for (int c = 0; c < rpr; c += 16) {
-          uint32_t v[16];
-          __syncwarp();
-          tmem_ld_32x32b_x16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * kMaxPass + i * rpr + c), v);
-          tmem_wait_ld();
-          if (mine == s0 + i) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) row[c + e] = kb1 > kb0 ? __uint_as_float(v[e]) : 0.0f;
-          }
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[acc]);
-    }
-  }
-  tc_fence_before();
-  __syncwarp();
-  cluster_sync();
-  if (warp >= 2) {
-    // This CTA's share of the rows. First their sums over the cluster, scaled, into the
-    // stages' memory (every copy and MMA is done), then H: 16 bytes per store.
-    const int share = 128 / splits, tid = threadIdx.x - 64;
-    float* fin = reinterpret_cast<float*>(smem);  // [share][pitch]
-    for (int rr = tid / 32; rr < share; rr += 4) {
-      const int me = half * 128 + rank * share + rr, a = ids[me];
-      if (a < 0) continue;
-      const float scale = p.scale ? p.scale[a] : 1.0f;
-      for (int j = lane; j < rpr; j += 32) {
-        const uint32_t at = smem_u32(sums + (rank * share + rr) * pitch + j);
-        float v = 0.0f;
-        for (int s = 0; s < splits; ++s) {
-          uint32_t peer;
-          asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer) : "r"(at), "r"(s));
-          v += ld_cluster_f32(peer);
-        }
-        fin[rr * pitch + j] = v * scale;
-      }
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    const int lgp = lk.cw == 16 ? 1 : lk.cw == 32 ? 2 : 3, nq = lk.chunks(m), per = lk.parts * lk.rc;
-    for (int x = tid; x < share << lgp; x += 128) {
-      const int rr = x >> lgp, pc = x & ((1 << lgp) - 1), me = half * 128 + rank * share + rr;
-      const int q0 = ids[me] >= 0 ? rank_of[slot[me]] * per : -per;
-      uint16_t* dst = lk.H + ((int64_t)group * lk.q_max * kGroup + me) * lk.cw + pc * 8;
-      for (int qi = 0; qi < nq; ++qi, dst += (int64_t)kGroup * lk.cw) {
-        uint32_t w[4] = {0, 0, 0, 0};
-        if (qi >= q0 && qi < q0 + per) {
-          const int part = qi - q0 >= lk.rc, c = qi - q0 - part * lk.rc;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = c * lk.cw + pc * 8 + e;
-            w[e >> 1] |= h_part(j < p.r ? fin[rr * pitch + j] : 0.0f, part) << (16 * (e & 1));
-          }
-        }
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-  }
-  __syncwarp();
-  cluster_sync();
-  if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
 // The elements of one 32-column chunk of a warp's rows whose sums are not finite, again
@@ -783,6 +611,7 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
                                         int local, int64_t col0, uint32_t bad) {
   const int lane = threadIdx.x & 31;
   const GroupList& L = lk.lists[local / kGroup];
+  ld_acquire(lk.done);  // H is complete: the tile's MMAs have read it
   for (uint32_t cols = __reduce_or_sync(0xffffffffu, bad); cols; cols &= cols - 1) {
     const int j = __ffs(cols) - 1;
     const int64_t n = col0 + j;
@@ -798,9 +627,9 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
       const uint16_t* w = W + n * ldw;
       float s = 0.0f;
       for (int64_t k = lane; k < p.K; k += 32) s = fmaf(bf16_to_f32(x[k]), bf16_to_f32(w[k]), s);
-      int a = p.row_adapter[row0 + t], sl = 0;
-      if (a >= 0 && a < p.n_adapters) {
-        while (L.adapter[sl] != a) ++sl;
+      const int sl = L.slot[t % kGroup];
+      if (sl >= 0) {
+        const int a = L.adapter[sl];
         const uint16_t* b = B + ((int64_t)a * p.N + n) * ldb;
         for (int c = lane; c < p.r; c += 32)
           for (int part = 0; part < lk.parts; ++part) {
@@ -824,9 +653,16 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
 // The GEMM: persistent, TMA warp / MMA warp / four epilogue warps, accumulators double
 // buffered in TMEM, as gemm_tc.cu. PAIR: clusters of two CTAs share 256 x BN tiles
 // (cta_group::2 MMAs, each CTA loads its 128 rows of X and its half of W's rows); else
-// 128 x BN tiles. After the K blocks of X and W a tile runs through the chunks of H and B
-// of its group's list, 64 / cw of them a stage; they are read only once k_lora_down has
-// ended (griddepcontrol.wait), so the base product of the first tiles overlaps it.
+// 128 x BN tiles.
+//
+// The first items of the launch, one per row of tiles, make H: X A_a^T for the adapters of
+// the group's list, their ranks side by side as the columns of an accumulator (BN at a
+// time); the epilogue keeps each row's own, scaled, and counts up `done`. The other items are
+// the tiles of Y: the K blocks of X and W first, then, once `done` says that H is complete,
+// the chunks of H and B, 64 / cw of them a stage. Every unit runs its items of the first kind
+// before those of the second, and only the second kind waits, so the wait ends. In a kernel of its
+// own the adapter product cost a pass over X that nothing overlapped: 827 instead of
+// us at 33792 x 3840 x 3840 with one adapter of rank 16 (640 without).
 template <int BN, bool PAIR>
 struct LoraGemmCfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
@@ -843,7 +679,13 @@ struct LoraGemm {
   int64_t row0, rows;
   int m_tiles, n_tiles, k_blocks;
   int y_vec, bias_vec;
+  __device__ int down_items() const { return lk.q_max ? m_tiles : 0; }
 };
+// Columns of the accumulator that `n` ranks take: a pair's MMA has a multiple of 32.
+template <int CTAS>
+__device__ __forceinline__ int down_columns(int n) {
+  return CTAS == 2 ? (n + 31) / 32 * 32 : n;
+}
 constexpr int kGroupM = 16;  // M tiles walked together, for reuse in L2
 __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& mb, int& nb) {
   const int per = kGroupM * n_tiles, g = t / per, first = g * kGroupM;
@@ -856,7 +698,7 @@ template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kRowThreads, 1)
     k_lora_gemm(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                 const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ LoraGemm g) {
+                const __grid_constant__ CUtensorMap tmA, const __grid_constant__ LoraGemm g) {
   using C_ = LoraGemmCfg<BN, PAIR>;
   constexpr int STAGES = C_::STAGES, CTAS = PAIR ? 2 : 1;
   constexpr uint32_t IDESC = make_idesc(1u, 0, 0, PAIR ? 256 : 128, BN);
@@ -864,13 +706,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int abort_word, pass_ids[BN / 16];  // adapters of the chunks of a pass
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
-  const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS, tiles = g.m_tiles * g.n_tiles;
+  const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
+  const int downs = g.down_items(), items = downs + g.m_tiles * g.n_tiles;
   int* err = g.p.err;
-  const int cw = g.lk.cw, cwb = 2 * cw, per_stage = 64 / cw;
+  const int cw = g.lk.cw, cwb = 2 * cw, per_stage = 64 / cw, per_pass = BN / cw;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -905,58 +748,87 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any signal crosses
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // The list of tile row mb's group, complete once k_lora_down has ended (without adapters
-  // there is none).
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // k_lora_lists
+  // The list of tile row mb's group (without adapters there is none), its adapters and the
+  // passes over them that make H.
   auto list_of = [&](int mb) { return g.lk.lists + (PAIR ? mb : mb >> 1); };
-  auto chunks_of = [&](int mb) { return g.lk.q_max ? g.lk.chunks(__ldcg(&list_of(mb)->count)) : 0; };
+  auto count_of = [&](int mb) { return g.lk.q_max ? __ldcg(&list_of(mb)->count) : 0; };
+  auto passes_of = [&](int mb) { return (count_of(mb) * g.lk.rc + per_pass - 1) / per_pass; };
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full0 = PAIR ? mapa_shared(&full[0], 0) : 0;
-      int done = 0;
-      bool ok = true;
-      auto stage = [&](int bytes, uint8_t*& st) {
-        const int s = done % STAGES;
-        ok = mbar_wait(&empty[s], ((done / STAGES) & 1) ^ 1u, abort_flag, err, kErrWaitEmpty);
+    {  // the whole warp: an elected lane issues
+      const uint32_t smem0 = smem_u32(smem), full_own = smem_u32(&full[0]);
+      const uint32_t full0 = PAIR ? mapa_shared(&full[0], 0) : full_own;  // the leader's
+      RingPos at;
+      int done = 0;  // stages filled
+      bool ok = true, have_h = false;
+      auto stage = [&](int bytes, uint32_t& st) {
+        ok = mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrWaitEmpty);
         if (!ok) return false;
-        st = smem + s * C_::STAGE;
-        if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * bytes);
+        st = smem0 + (uint32_t)(at.slot * C_::STAGE);
+        if (rank == 0) mbar_expect_tx_elect(full_own + (uint32_t)(at.slot * 8), (uint32_t)(CTAS * bytes));
+        ++done;
         return true;
       };
-      auto load2 = [&](uint8_t* dst, const CUtensorMap* m, int x, int y) {
-        const int s = done % STAGES;
+      auto load2 = [&](uint32_t dst, const CUtensorMap* m, int x, int y) {
         if constexpr (PAIR)
-          tma_load_2d_pair(dst, m, full0 + (uint32_t)(s * 8), x, y);
+          tma_load_2d_pair_elect(dst, m, full0 + (uint32_t)(at.slot * 8), x, y);
         else
-          tma_load_2d(dst, m, &full[s], x, y);
+          tma_load_2d_elect(dst, m, full0 + (uint32_t)(at.slot * 8), x, y);
       };
-      auto load3 = [&](uint8_t* dst, const CUtensorMap* m, int x, int y, int z) {
-        const int s = done % STAGES;
+      auto load3 = [&](uint32_t dst, const CUtensorMap* m, int x, int y, int z) {
         if constexpr (PAIR)
-          tma_load_3d_pair(dst, m, full0 + (uint32_t)(s * 8), x, y, z);
+          tma_load_3d_pair_elect(dst, m, full0 + (uint32_t)(at.slot * 8), x, y, z);
         else
-          tma_load_3d(dst, m, &full[s], x, y, z);
+          tma_load_3d_elect(dst, m, full0 + (uint32_t)(at.slot * 8), x, y, z);
       };
-      for (int t = unit; t < tiles && ok; t += units) {
+      for (int it = unit; it < items && ok; it += units) {
+        uint32_t st;
+        if (it < downs) {
+          const int y0 = (it * CTAS + (int)rank) * 128, nch = count_of(it) * g.lk.rc;
+          for (int c0 = 0; c0 < nch && ok; c0 += per_pass) {
+            const int n = min(per_pass, nch - c0);
+            __syncwarp();
+            if (lane < n) pass_ids[lane] = __ldcg(&list_of(it)->adapter[(c0 + lane) / g.lk.rc]);
+            __syncwarp();
+            const int c_first = c0 % g.lk.rc;
+            for (int kb = 0; kb < g.k_blocks; ++kb, at.next(STAGES)) {
+              if (!stage(C_::A_BYTES + n * (cw / CTAS) * 128, st)) break;
+              load2(st, &tmX, kb * 64, (int)g.row0 + y0);
+              for (int i = 0, c = c_first; i < n; ++i, c = c + 1 == g.lk.rc ? 0 : c + 1)
+                load3(st + C_::A_BYTES + i * (cw / CTAS) * 128, &tmA, kb * 64, c * cw + (int)rank * (cw / CTAS), pass_ids[i]);
+            }
+          }
+          continue;
+        }
         int mb, nb;
-        tile_at(t, g.m_tiles, g.n_tiles, mb, nb);
+        tile_at(it - downs, g.m_tiles, g.n_tiles, mb, nb);
         const int y0 = (mb * CTAS + (int)rank) * 128, n0 = nb * BN + (int)rank * C_::B_ROWS;
-        uint8_t* st;
-        for (int kb = 0; kb < g.k_blocks; ++kb, ++done) {
+        // Read ahead: the loads arrive while the K blocks are on their way.
+        const int count = count_of(mb), adapter0 = downs ? __ldcg(&list_of(mb)->adapter[0]) : 0;
+        const int adapter1 = downs ? __ldcg(&list_of(mb)->adapter[1]) : 0;
+        for (int kb = 0; kb < g.k_blocks; ++kb, at.next(STAGES)) {
           if (!stage(C_::STAGE, st)) break;
           load2(st, &tmX, kb * 64, (int)g.row0 + y0);
           load2(st + C_::A_BYTES, &tmW, kb * 64, n0);
         }
         if (!ok) break;
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int nq = chunks_of(mb), group = y0 / kGroup;
-        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
+        if (!downs) continue;
+        const int nq = g.lk.chunks(count), group = y0 / kGroup;
+        if (!have_h) {
+          ok = wait_count(g.lk.done, 4 * CTAS * g.m_tiles, abort_flag, err);
+          if (!ok) break;
+          asm volatile("fence.proxy.async;" ::: "memory");  // H was stored by other CTAs, TMA reads it
+          have_h = true;
+        }
+        for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(STAGES)) {
           const int n = min(per_stage, nq - q0);
           if (!stage(n * (128 + C_::B_ROWS) * cwb, st)) break;
           for (int i = 0; i < n; ++i) {
             const int q = q0 + i, c = q % g.lk.rc, sl = q / (g.lk.rc * g.lk.parts);
             load2(st + i * 128 * cwb, &tmH, 0, (group * g.lk.q_max + q) * kGroup + y0 % kGroup);
-            load3(st + C_::A_BYTES + i * C_::B_ROWS * cwb, &tmB, c * cw, n0, __ldcg(&list_of(mb)->adapter[sl]));
+            load3(st + C_::A_BYTES + i * C_::B_ROWS * cwb, &tmB, c * cw, n0,
+                  sl == 0 ? adapter0 : sl == 1 ? adapter1 : __ldcg(&list_of(mb)->adapter[sl]));
           }
         }
       }
@@ -970,7 +842,10 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {  // the whole warp: an elected lane issues
-      int done = 0, n = 0;
+      RingPos at;
+      int n = 0;
+      const uint64_t ad0 = sdesc_k_sw128(smem_u32(smem)), bd0 = sdesc_k_sw128(smem_u32(smem) + C_::A_BYTES);
+      const uint32_t empty0 = smem_u32(&empty[0]);
       bool ok = true;
       auto commit = [&](uint64_t* bar) {
         if constexpr (PAIR)
@@ -978,47 +853,60 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         else
           umma_commit_elect(bar);
       };
-      for (int t = unit; t < tiles && ok; t += units, ++n) {
-        const int acc = n & 1;
-        ok = mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1u, abort_flag, err, kErrWaitAccEmpty);
-        if (!ok) break;
-        tc_fence_after();
-        int mb, nb;
-        tile_at(t, g.m_tiles, g.n_tiles, mb, nb);
-        const uint32_t d = tmem + (uint32_t)(acc * BN);
-        for (int kb = 0; kb < g.k_blocks; ++kb, ++done) {
-          const int s = done % STAGES;
-          ok = mbar_wait(&full[s], (done / STAGES) & 1, abort_flag, err, kErrWaitFull);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
-          if constexpr (PAIR)
-            umma4_pair_elect(d, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb != 0);
-          else
-            umma4_elect(d, sdesc_k_sw128(a0), sdesc_k_sw128(b0), IDESC, kb != 0);
-          commit(&empty[s]);
+      for (int it = unit; it < items && ok; it += units) {
+        const bool down = it < downs;
+        int mb = it, nb = 0, nch = 0, passes = 1;
+        if (down) {
+          nch = count_of(it) * g.lk.rc;
+          passes = passes_of(it);
+        } else {
+          tile_at(it - downs, g.m_tiles, g.n_tiles, mb, nb);
         }
-        if (!ok) break;
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int nq = chunks_of(mb);
-        for (int q0 = 0; q0 < nq; q0 += per_stage, ++done) {
-          const int s = done % STAGES;
-          ok = mbar_wait(&full[s], (done / STAGES) & 1, abort_flag, err, kErrWaitFull);
+        const int count = count_of(mb);
+        for (int ps = 0; ps < passes; ++ps, ++n) {
+          const int acc = n & 1;
+          ok = mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1u, abort_flag, err, kErrWaitAccEmpty);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
-          for (int i = 0; i < min(per_stage, nq - q0); ++i)
-            for (int k = 0; k < cw / 16; ++k) {
-              const uint64_t ad = sdesc_k(a0 + i * 128 * cwb + k * 32, cwb), bd = sdesc_k(b0 + i * C_::B_ROWS * cwb + k * 32, cwb);
-              if constexpr (PAIR)
-                umma_pair_elect(d, ad, bd, IDESC, 1u);
-              else
-                umma_elect(d, ad, bd, IDESC, 1u);
+          const uint32_t d = tmem + (uint32_t)(acc * BN);
+          // A pair's MMA takes a multiple of 32 columns; what the last ones hold is not read.
+          const int N = down ? down_columns<CTAS>(min(per_pass, nch - ps * per_pass) * cw) : BN;
+          const uint32_t idesc = down ? make_idesc(1u, 0, 0, 128 * CTAS, (uint32_t)N) : IDESC;
+          const uint32_t d_step = 4 * N <= BN ? (uint32_t)N : 0;  // four accumulators where they fit
+          for (int kb = 0; kb < g.k_blocks; ++kb, at.next(STAGES)) {
+            ok = mbar_wait(&full[at.slot], at.phase, abort_flag, err, kErrWaitFull);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t off = (uint64_t)(at.slot * (C_::STAGE >> 4));
+            if constexpr (PAIR)
+              umma4_pair_elect(d, ad0 + off, bd0 + off, idesc, kb != 0, empty0 + 8 * at.slot, d_step);
+            else
+              umma4_elect(d, ad0 + off, bd0 + off, idesc, kb != 0, empty0 + 8 * at.slot, d_step);
+          }
+          if (!ok) break;
+          if (!down && downs) {
+              const int nq = g.lk.chunks(count);
+            for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(STAGES)) {
+              const int s = at.slot;
+              ok = mbar_wait(&full[s], at.phase, abort_flag, err, kErrWaitFull);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
+              for (int i = 0; i < min(per_stage, nq - q0); ++i)
+                for (int k = 0; k < cw / 16; ++k) {
+                  const uint64_t ad = sdesc_k(a0 + i * 128 * cwb + k * 32, cwb);
+                  const uint64_t bd = sdesc_k(b0 + i * C_::B_ROWS * cwb + k * 32, cwb);
+                  if constexpr (PAIR)
+                    umma_pair_elect(d, ad, bd, IDESC, 1u);
+                  else
+                    umma_elect(d, ad, bd, IDESC, 1u);
+                }
+              commit(&empty[s]);
             }
-          commit(&empty[s]);
+            if (!ok) break;
+          }
+          commit(&acc_full[acc]);
         }
-        if (!ok) break;
-        commit(&acc_full[acc]);
       }
       commit(&drain);
     }
@@ -1033,13 +921,80 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   } else {
     const int q = warp & 3;
     const uint32_t acc_empty0 = PAIR ? mapa_shared(&acc_empty[0], 0) : 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     int n = 0;
-    for (int t = unit; t < tiles; t += units, ++n) {
+    bool ok = true;
+    auto release = [&](int acc) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_cluster(acc_empty0 + (uint32_t)(acc * 8));
+        else
+          mbar_arrive(&acc_empty[acc]);
+      }
+    };
+    for (int it = unit; it < items && ok; it += units) {
+      if (it < downs) {
+        // H of this warp's rows: their own adapter's columns, zeros in the others' chunks.
+        const int me = (it * CTAS + (int)rank) * 128 % kGroup + q * 32 + lane, nch = count_of(it) * g.lk.rc;
+        const GroupList* L = list_of(it);
+        const int mine = L->slot[me];
+        const float scale = mine >= 0 && g.p.scale ? g.p.scale[L->adapter[mine]] : 1.0f;
+        uint16_t* rowH = g.lk.H + ((int64_t)(L - g.lk.lists) * g.lk.q_max * kGroup + me) * cw;
+        for (int c0 = 0; c0 < nch; c0 += per_pass, ++n) {
+          const int acc = n & 1, used = min(per_pass, nch - c0), N = down_columns<CTAS>(used * cw);
+          ok = mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+          for (int i = 0; i < used; ++i) {
+            const int sl = (c0 + i) / g.lk.rc, c = (c0 + i) % g.lk.rc;
+            for (int e0 = 0; e0 < cw; e0 += 8) {
+              // A pair's two CTAs hold the two halves of each chunk's ranks.
+              const int half = e0 >= cw / CTAS;
+              const int col = half * (N / CTAS) + i * (cw / CTAS) + e0 - half * (cw / CTAS);
+              uint32_t v[8];
+              __syncwarp();
+              tmem_ld_32x32b_x8(base + (uint32_t)col, v);
+              if (4 * N <= BN) {  // four accumulators
+                uint32_t u[3][8];
+#pragma unroll
+                for (int a = 0; a < 3; ++a) tmem_ld_32x32b_x8(base + (uint32_t)(col + (a + 1) * N), u[a]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  v[e] = __float_as_uint((__uint_as_float(v[e]) + __uint_as_float(u[0][e])) +
+                                         (__uint_as_float(u[1][e]) + __uint_as_float(u[2][e])));
+              } else {
+                tmem_wait_ld();
+              }
+              for (int part = 0; part < g.lk.parts; ++part) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                if (sl == mine) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(__uint_as_float(v[e]) * scale, part) << (16 * (e & 1));
+                }
+                const int64_t qi = (int64_t)(sl * g.lk.parts + part) * g.lk.rc + c;
+                *reinterpret_cast<uint4*>(rowH + qi * kGroup * cw + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+          }
+          release(acc);
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");  // for the TMA loads of other CTAs
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          __threadfence();
+          atomicAdd(g.lk.done, 1);
+        }
+        continue;
+      }
       const int acc = n & 1;
       int mb, nb;
-      tile_at(t, g.m_tiles, g.n_tiles, mb, nb);
+      tile_at(it - downs, g.m_tiles, g.n_tiles, mb, nb);
       if (!mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull)) break;
+      ++n;
       tc_fence_after();
       const int local = (mb * CTAS + (int)rank) * 128 + q * 32 + lane;
       const bool row_ok = local < g.rows, mixed = g.lk.q_max && __ldcg(&list_of(mb)->mixed);
@@ -1109,14 +1064,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             redo_chunk(g.p, g.lk, g.X, g.ldx, g.W, g.ldw, g.B, g.ldb, g.row0, local, col0, bad);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (PAIR)
-          mbar_arrive_cluster(acc_empty0 + (uint32_t)(acc * 8));
-        else
-          mbar_arrive(&acc_empty[acc]);
-      }
+      release(acc);
     }
   }
   tc_fence_before();
@@ -1133,10 +1081,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 }
 
 template <int BN, bool PAIR>
-void launch_lora_gemm(LoraGemm g, int64_t r, bool overlap) {
+void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) {
+  const int64_t r = g.p.r;
   using C_ = LoraGemmCfg<BN, PAIR>;
   DeviceContext& c = ctx();
-  CUtensorMap tx, tw, th, tb;
+  CUtensorMap tx, tw, th, tb, ta;
   map_2d(&tx, g.X, g.p.K, g.p.T, g.ldx, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
   map_2d(&tw, g.W, g.p.K, g.p.N, g.ldw, 64, C_::B_ROWS, CU_TENSOR_MAP_SWIZZLE_128B);
   g.m_tiles = (int)((g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
@@ -1146,8 +1095,9 @@ void launch_lora_gemm(LoraGemm g, int64_t r, bool overlap) {
     const int64_t groups = (g.rows + kGroup - 1) / kGroup;
     map_2d(&th, g.lk.H, g.lk.cw, groups * g.lk.q_max * kGroup, g.lk.cw, g.lk.cw, 128, swizzle_of(g.lk.cw));
     map_adapters(&tb, g.B, r, g.p.N, g.p.n_adapters, g.ldb, g.lk.cw, C_::B_ROWS, swizzle_of(g.lk.cw));
+    map_adapters(&ta, A, g.p.K, r, g.p.n_adapters, lda, 64, PAIR ? g.lk.cw / 2 : g.lk.cw, CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
-    th = tb = tx;  // no chunk is read
+    th = tb = ta = tx;  // not read
   }
   static int clusters[64] = {};
   auto kern = k_lora_gemm<BN, PAIR>;
@@ -1181,7 +1131,7 @@ void launch_lora_gemm(LoraGemm g, int64_t r, bool overlap) {
   }
   cfg.numAttrs = n;
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(clusters[c.device], (int64_t)g.m_tiles * g.n_tiles) * (PAIR ? 2 : 1)));
-  check_cuda(cudaLaunchKernelEx(&cfg, kern, tx, tw, th, tb, g), "linear_lora");
+  check_cuda(cudaLaunchKernelEx(&cfg, kern, tx, tw, th, tb, ta, g), "linear_lora");
   check_launch("linear_lora");
 }
 
@@ -1204,7 +1154,7 @@ Big lay_out_big(const LoraLinear& p, size_t at) {
   // H holds every chunk a group could need; blocks of rows keep it within 128 MB.
   const int64_t group = (int64_t)b.lk.q_max * kGroup * b.lk.cw * 2;
   b.rows = std::min(b.rows, std::max<int64_t>(1, ((int64_t)128 << 20) / group) * kGroup);
-  b.h_at = at + align256((size_t)(b.rows / kGroup) * sizeof(GroupList));
+  b.h_at = at + 256 + align256((size_t)(b.rows / kGroup) * sizeof(GroupList));  // `done`, the lists, H
   b.bytes = b.h_at + align256((size_t)(b.rows / kGroup) * group);
   return b;
 }
@@ -1216,7 +1166,8 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   LoraGemm g{};
   g.p = p;
   g.lk = big.lk;
-  g.lk.lists = reinterpret_cast<const GroupList*>(ws + big.lists_at);
+  g.lk.done = reinterpret_cast<int*>(ws + big.lists_at);
+  g.lk.lists = reinterpret_cast<GroupList*>(ws + big.lists_at + 256);
   g.lk.H = reinterpret_cast<uint16_t*>(ws + big.h_at);
   g.X = X;
   g.W = W;
@@ -1229,43 +1180,17 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   for (g.row0 = 0; g.row0 < p.T; g.row0 += big.rows) {
     g.rows = std::min(big.rows, p.T - g.row0);
     if (adapters) {
-      const int rpr = (int)round_up(p.r, 16), stages = DownCfg::stages(rpr);
-      CUtensorMap tx, ta;
-      map_2d(&tx, X, p.K, p.T, ldx, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-      map_adapters(&ta, A, p.K, p.r, p.n_adapters, lda, 64, rpr, CU_TENSOR_MAP_SWIZZLE_128B);
-      const int64_t tiles = 2 * ((g.rows + kGroup - 1) / kGroup);
-      const int kblocks = (int)((p.K + 63) / 64);
-      int splits = 1;
-      while (splits < 8 && tiles * splits * 2 <= c.num_sms && kblocks >= 4 * splits) splits *= 2;
-      static bool done[64] = {};
-      if (!done[c.device]) {
-        check_cuda(cudaFuncSetAttribute(k_lora_down, cudaFuncAttributeMaxDynamicSharedMemorySize, 218 * 1024),
-                   "cudaFuncSetAttribute(lora_down)");
-        done[c.device] = true;
-      }
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3((unsigned)(tiles * splits));
-      cfg.blockDim = dim3(kRowThreads);
-      cfg.dynamicSmemBytes = DownCfg::smem(rpr);
-      cfg.stream = c.stream;
-      cudaLaunchAttribute attr{};
-      attr.id = cudaLaunchAttributeClusterDimension;
-      attr.val.clusterDim.x = (unsigned)splits;
-      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-      cfg.attrs = &attr;
-      cfg.numAttrs = 1;
-      check_cuda(cudaLaunchKernelEx(&cfg, k_lora_down, tx, ta, p, (const LoraK)g.lk, const_cast<GroupList*>(g.lk.lists), rpr,
-                                    stages, splits, g.row0, g.rows),
-                 "lora_down");
-      check_launch("lora_down");
+      k_lora_lists<<<(unsigned)((g.rows + kGroup - 1) / kGroup), kGroup, 0, c.stream>>>(p, g.lk, g.row0, g.rows);
+      check_launch("lora_lists");
     }
     // Tile shape by waves, as gemm_tc.cu prices them: a tile costs its width and 48 columns
     // of fixed cost, a pair tile (256 rows over two processors) 8% less. Several pair widths,
     // because a few rows of tiles leave the last wave nearly empty: 2397 x 4096 outputs are
     // 2.2 waves of 256 columns (3 x 280) but 3.0 waves of 192 (3 x 221).
     auto cost = [&](int bm, int bn, int64_t units) {
-      const int64_t t = ((g.rows + bm - 1) / bm) * ((p.N + bn - 1) / bn);
-      return (double)((t + units - 1) / units) * (bn + 48) * (bm == 256 ? 0.92 : 1.0);
+      const int64_t rows = (g.rows + bm - 1) / bm, t = rows * ((p.N + bn - 1) / bn);
+      const double down = adapters ? 0.3 * (double)rows : 0.0;  // the items that make H
+      return std::ceil(((double)t + down) / (double)units) * (bn + 48) * (bm == 256 ? 0.92 : 1.0);
     };
     double best = 1e30;
     int bm = 128, bn = 64;
@@ -1280,15 +1205,15 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
         }
       }
     if (bm == 256) {
-      if (bn == 256) launch_lora_gemm<256, true>(g, p.r, adapters);
-      if (bn == 224) launch_lora_gemm<224, true>(g, p.r, adapters);
-      if (bn == 192) launch_lora_gemm<192, true>(g, p.r, adapters);
-      if (bn == 160) launch_lora_gemm<160, true>(g, p.r, adapters);
-      if (bn == 128) launch_lora_gemm<128, true>(g, p.r, adapters);
+      if (bn == 256) launch_lora_gemm<256, true>(g, A, lda, adapters);
+      if (bn == 224) launch_lora_gemm<224, true>(g, A, lda, adapters);
+      if (bn == 192) launch_lora_gemm<192, true>(g, A, lda, adapters);
+      if (bn == 160) launch_lora_gemm<160, true>(g, A, lda, adapters);
+      if (bn == 128) launch_lora_gemm<128, true>(g, A, lda, adapters);
     } else {
-      if (bn == 256) launch_lora_gemm<256, false>(g, p.r, adapters);
-      if (bn == 128) launch_lora_gemm<128, false>(g, p.r, adapters);
-      if (bn == 64) launch_lora_gemm<64, false>(g, p.r, adapters);
+      if (bn == 256) launch_lora_gemm<256, false>(g, A, lda, adapters);
+      if (bn == 128) launch_lora_gemm<128, false>(g, A, lda, adapters);
+      if (bn == 64) launch_lora_gemm<64, false>(g, A, lda, adapters);
     }
   }
 }

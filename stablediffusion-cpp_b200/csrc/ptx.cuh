@@ -69,6 +69,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// A position in a ring of `n` slots: the slot, and the parity of its current use.
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // Waits until the phase with the given parity has completed. Returns false (after
 // recording `code` in *err and raising the CTA abort flag) if the wait exceeds
 // kWaitLimitNs, or if another role of the CTA has already aborted.
@@ -185,15 +197,6 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
       "[%2];" ::"r"(smem_u32(smem_dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
-      : "memory");
-}
-// 3-D form of tma_load_2d_pair.
-__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster, int x,
-                                                 int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
-      "%5}], [%2];" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 // 4-D form of tma_load_2d_pair (x innermost, 16-byte aligned; no multicast).
@@ -382,35 +385,43 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 // is more than the tensor core needs for 128 columns.
 //
 // Four kind::f16 MMAs along K, both operands K-major in a 128-byte swizzle (32 bytes = 2
-// descriptor units per step); the first accumulates iff acc_first.
-__device__ __forceinline__ void umma4_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first) {
+// descriptor units per step), and a commit of them to the mbarrier at shared address `bar`
+// (of both CTAs of a pair); the first accumulates iff acc_first. With d_step they go to four
+// accumulators d_step columns apart, each accumulating iff acc_first: MMAs of a few columns on
+// one accumulator wait for one another (a pair's four of 32 columns took 0.65 us).
+__device__ __forceinline__ void umma4_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first,
+                                            uint32_t bar, uint32_t d_step = 0) {
   asm volatile(
-      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t"
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t.reg .b32 z;\n\t"
       "elect.sync _|q, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.or.b32 t, %6, 0, p;\n\t"
       "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
-      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
-      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc_first)
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\tadd.s32 z, %0, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [z], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\tadd.s32 z, z, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [z], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\tadd.s32 z, z, %6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [z], x, y, %3, t;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc_first), "r"(bar), "r"(d_step)
       : "memory");
 }
-__device__ __forceinline__ void umma4_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first) {
+__device__ __forceinline__ void umma4_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc_first,
+                                            uint32_t bar, uint32_t d_step = 0) {
   asm volatile(
-      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t"
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\t.reg .b32 z;\n\t"
       "elect.sync _|q, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.or.b32 t, %6, 0, p;\n\t"
       "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t"
-      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t"
-      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], x, y, %3, t;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc_first)
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\tadd.s32 z, %0, %6;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [z], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\tadd.s32 z, z, %6;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [z], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\tadd.s32 z, z, %6;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [z], x, y, %3, t;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%5], %7;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc_first), "r"(bar), "r"(d_step),
+      "h"((uint16_t)0x3)
       : "memory");
 }
 // One MMA.
@@ -448,6 +459,50 @@ __device__ __forceinline__ void umma_commit_pair_elect(uint64_t* bar, uint16_t c
       : "memory");
 }
 
+// The loads above, and the arrival that announces their bytes, by the elected lane of a
+// converged warp (see umma4_elect). From one lane under `if (lane == 0)` a load took 150 to
+// 200 cycles to issue, so that two loads a K block bounded GEMMs of up to 192 columns.
+__device__ __forceinline__ void mbar_expect_tx_elect(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_elect(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}\n" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_elect(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair_elect(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair_elect(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y,
+                                                       int z) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -471,6 +526,12 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+// 32 lanes x 8 columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 // 32 lanes x 16 columns store (thread i writes lane base+i).
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
