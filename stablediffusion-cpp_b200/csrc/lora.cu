@@ -524,7 +524,10 @@ struct GroupList {
 // H: [groups][q_max][kGroup][cw] bf16, chunk q = (slot * parts + part) * rc + c of a group.
 struct LoraK {
   GroupList* lists;
-  int* done;  // warps of k_lora_gemm that have stored their part of H
+  int* done;     // warps of k_lora_gemm that have stored their part of H
+  int* arrived;  // [groups][8]: K splits that have stored their part, for 32 rows each
+  float* part;   // [rows][ksplit][rc cw]: the splits' parts of a row's own h
+  int ksplit;
   uint16_t* H;
   int cw, rc, parts, q_max;
   __host__ __device__ int chunks(int count) const { return count * parts * rc; }
@@ -543,6 +546,7 @@ __global__ void __launch_bounds__(kGroup) k_lora_lists(const LoraLinear p, const
   }
   if (i == 0) mixed = 0;
   if (i == 0 && blockIdx.x == 0) *lk.done = 0;
+  if (i < 8) lk.arrived[blockIdx.x * 8 + i] = 0;
   int a = t < rows ? p.row_adapter[row0 + t] : -1;
   if (a >= p.n_adapters) {
     atomicOr(p.err, kErrBadIndex);
@@ -657,7 +661,8 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
 //
 // The first items of the launch, one per row of tiles, make H: X A_a^T for the adapters of
 // the group's list, their ranks side by side as the columns of an accumulator (BN at a
-// time); the epilogue keeps each row's own, scaled, and counts up `done`. The other items are
+// time), K split over several items where there are more units than rows of tiles; the
+// epilogue keeps each row's own, scaled, and counts up `done`. The other items are
 // the tiles of Y: the K blocks of X and W first, then, once `done` says that H is complete,
 // the chunks of H and B, 64 / cw of them a stage. Every unit runs its items of the first kind
 // before those of the second, and only the second kind waits, so the wait ends. In a kernel of its
@@ -679,13 +684,14 @@ struct LoraGemm {
   int64_t row0, rows;
   int m_tiles, n_tiles, k_blocks;
   int y_vec, bias_vec;
-  __device__ int down_items() const { return lk.q_max ? m_tiles : 0; }
+  __device__ int down_items() const { return lk.q_max ? m_tiles * lk.ksplit : 0; }
 };
 // Columns of the accumulator that `n` ranks take: a pair's MMA has a multiple of 32.
 template <int CTAS>
 __device__ __forceinline__ int down_columns(int n) {
   return CTAS == 2 ? (n + 31) / 32 * 32 : n;
 }
+__device__ __forceinline__ int split_begin(int k_blocks, int splits, int s) { return (int)((int64_t)k_blocks * s / splits); }
 constexpr int kGroupM = 16;  // M tiles walked together, for reuse in L2
 __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& mb, int& nb) {
   const int per = kGroupM * n_tiles, g = t / per, first = g * kGroupM;
@@ -785,14 +791,16 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       for (int it = unit; it < items && ok; it += units) {
         uint32_t st;
         if (it < downs) {
-          const int y0 = (it * CTAS + (int)rank) * 128, nch = count_of(it) * g.lk.rc;
+          const int mb = it % g.m_tiles, sp = it / g.m_tiles;
+          const int y0 = (mb * CTAS + (int)rank) * 128, nch = count_of(mb) * g.lk.rc;
+          const int kb0 = split_begin(g.k_blocks, g.lk.ksplit, sp), kb1 = split_begin(g.k_blocks, g.lk.ksplit, sp + 1);
           for (int c0 = 0; c0 < nch && ok; c0 += per_pass) {
             const int n = min(per_pass, nch - c0);
             __syncwarp();
-            if (lane < n) pass_ids[lane] = __ldcg(&list_of(it)->adapter[(c0 + lane) / g.lk.rc]);
+            if (lane < n) pass_ids[lane] = __ldcg(&list_of(mb)->adapter[(c0 + lane) / g.lk.rc]);
             __syncwarp();
             const int c_first = c0 % g.lk.rc;
-            for (int kb = 0; kb < g.k_blocks; ++kb, at.next(STAGES)) {
+            for (int kb = kb0; kb < kb1; ++kb, at.next(STAGES)) {
               if (!stage(C_::A_BYTES + n * (cw / CTAS) * 128, st)) break;
               load2(st, &tmX, kb * 64, (int)g.row0 + y0);
               for (int i = 0, c = c_first; i < n; ++i, c = c + 1 == g.lk.rc ? 0 : c + 1)
@@ -855,10 +863,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       };
       for (int it = unit; it < items && ok; it += units) {
         const bool down = it < downs;
-        int mb = it, nb = 0, nch = 0, passes = 1;
+        int mb = it % g.m_tiles, nb = 0, nch = 0, passes = 1, kb0 = 0, kb1 = g.k_blocks;
         if (down) {
-          nch = count_of(it) * g.lk.rc;
-          passes = passes_of(it);
+          nch = count_of(mb) * g.lk.rc;
+          passes = passes_of(mb);
+          kb0 = split_begin(g.k_blocks, g.lk.ksplit, it / g.m_tiles);
+          kb1 = split_begin(g.k_blocks, g.lk.ksplit, it / g.m_tiles + 1);
         } else {
           tile_at(it - downs, g.m_tiles, g.n_tiles, mb, nb);
         }
@@ -873,15 +883,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           const int N = down ? down_columns<CTAS>(min(per_pass, nch - ps * per_pass) * cw) : BN;
           const uint32_t idesc = down ? make_idesc(1u, 0, 0, 128 * CTAS, (uint32_t)N) : IDESC;
           const uint32_t d_step = 4 * N <= BN ? (uint32_t)N : 0;  // four accumulators where they fit
-          for (int kb = 0; kb < g.k_blocks; ++kb, at.next(STAGES)) {
+          for (int kb = kb0; kb < kb1; ++kb, at.next(STAGES)) {
             ok = mbar_wait(&full[at.slot], at.phase, abort_flag, err, kErrWaitFull);
             if (!ok) break;
             tc_fence_after();
             const uint64_t off = (uint64_t)(at.slot * (C_::STAGE >> 4));
             if constexpr (PAIR)
-              umma4_pair_elect(d, ad0 + off, bd0 + off, idesc, kb != 0, empty0 + 8 * at.slot, d_step);
+              umma4_pair_elect(d, ad0 + off, bd0 + off, idesc, kb != kb0, empty0 + 8 * at.slot, d_step);
             else
-              umma4_elect(d, ad0 + off, bd0 + off, idesc, kb != 0, empty0 + 8 * at.slot, d_step);
+              umma4_elect(d, ad0 + off, bd0 + off, idesc, kb != kb0, empty0 + 8 * at.slot, d_step);
           }
           if (!ok) break;
           if (!down && downs) {
@@ -936,11 +946,25 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     for (int it = unit; it < items && ok; it += units) {
       if (it < downs) {
         // H of this warp's rows: their own adapter's columns, zeros in the others' chunks.
-        const int me = (it * CTAS + (int)rank) * 128 % kGroup + q * 32 + lane, nch = count_of(it) * g.lk.rc;
-        const GroupList* L = list_of(it);
+        const int mb = it % g.m_tiles, sp = it / g.m_tiles, nch = count_of(mb) * g.lk.rc;
+        const int me = (mb * CTAS + (int)rank) * 128 % kGroup + q * 32 + lane;
+        const GroupList* L = list_of(mb);
         const int mine = L->slot[me];
         const float scale = mine >= 0 && g.p.scale ? g.p.scale[L->adapter[mine]] : 1.0f;
         uint16_t* rowH = g.lk.H + ((int64_t)(L - g.lk.lists) * g.lk.q_max * kGroup + me) * cw;
+        const int rp = g.lk.rc * cw;
+        float* part = g.lk.part + ((int64_t)(mb * CTAS + (int)rank) * 128 + q * 32 + lane) * g.lk.ksplit * rp;
+        auto store_h = [&](int sl, int c, int e0, const float (&v)[8]) {
+          for (int pt = 0; pt < g.lk.parts; ++pt) {
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (sl == mine) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(v[e] * scale, pt) << (16 * (e & 1));
+            }
+            const int64_t qi = (int64_t)(sl * g.lk.parts + pt) * g.lk.rc + c;
+            *reinterpret_cast<uint4*>(rowH + qi * kGroup * cw + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        };
         for (int c0 = 0; c0 < nch; c0 += per_pass, ++n) {
           const int acc = n & 1, used = min(per_pass, nch - c0), N = down_columns<CTAS>(used * cw);
           ok = mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
@@ -949,44 +973,75 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
           for (int i = 0; i < used; ++i) {
             const int sl = (c0 + i) / g.lk.rc, c = (c0 + i) % g.lk.rc;
+            if (g.lk.ksplit > 1 && !__any_sync(0xffffffffu, sl == mine)) continue;
             for (int e0 = 0; e0 < cw; e0 += 8) {
               // A pair's two CTAs hold the two halves of each chunk's ranks.
               const int half = e0 >= cw / CTAS;
               const int col = half * (N / CTAS) + i * (cw / CTAS) + e0 - half * (cw / CTAS);
-              uint32_t v[8];
+              uint32_t r[4][8];
+              float v[8];
               __syncwarp();
-              tmem_ld_32x32b_x8(base + (uint32_t)col, v);
+              tmem_ld_32x32b_x8(base + (uint32_t)col, r[0]);
               if (4 * N <= BN) {  // four accumulators
-                uint32_t u[3][8];
 #pragma unroll
-                for (int a = 0; a < 3; ++a) tmem_ld_32x32b_x8(base + (uint32_t)(col + (a + 1) * N), u[a]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  v[e] = __float_as_uint((__uint_as_float(v[e]) + __uint_as_float(u[0][e])) +
-                                         (__uint_as_float(u[1][e]) + __uint_as_float(u[2][e])));
-              } else {
-                tmem_wait_ld();
+                for (int a = 1; a < 4; ++a) tmem_ld_32x32b_x8(base + (uint32_t)(col + a * N), r[a]);
               }
-              for (int part = 0; part < g.lk.parts; ++part) {
-                uint32_t w[4] = {0, 0, 0, 0};
-                if (sl == mine) {
+              tmem_wait_ld();
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(__uint_as_float(v[e]) * scale, part) << (16 * (e & 1));
-                }
-                const int64_t qi = (int64_t)(sl * g.lk.parts + part) * g.lk.rc + c;
-                *reinterpret_cast<uint4*>(rowH + qi * kGroup * cw + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int e = 0; e < 8; ++e) {
+                v[e] = __uint_as_float(r[0][e]);
+                if (4 * N <= BN)
+                  v[e] = (v[e] + __uint_as_float(r[1][e])) + (__uint_as_float(r[2][e]) + __uint_as_float(r[3][e]));
+              }
+              if (g.lk.ksplit == 1) {
+                store_h(sl, c, e0, v);
+              } else if (sl == mine) {
+                float4* dst = reinterpret_cast<float4*>(part + sp * rp + c * cw + e0);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
               }
             }
           }
           release(acc);
         }
-        asm volatile("fence.proxy.async;" ::: "memory");  // for the TMA loads of other CTAs
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) {
+        bool last = true;
+        if (g.lk.ksplit > 1) {
+          // The last split to arrive adds the parts in their order.
           __threadfence();
-          atomicAdd(g.lk.done, 1);
+          __syncwarp();
+          int before = 0;
+          if (lane == 0) before = atomicAdd(&g.lk.arrived[(mb * CTAS + (int)rank) * 4 + q], 1);
+          last = __shfl_sync(0xffffffffu, before, 0) == g.lk.ksplit - 1;
+          __threadfence();
+          if (last)
+            for (int i = 0; i < nch; ++i)
+              for (int e0 = 0; e0 < cw; e0 += 8) {
+                const int sl = i / g.lk.rc, c = i % g.lk.rc;
+                float v[8] = {};
+                if (sl == mine)
+                  for (int s = 0; s < g.lk.ksplit; ++s) {
+                    const float4* src = reinterpret_cast<const float4*>(part + s * rp + c * cw + e0);
+                    const float4 x = __ldcg(src), y = __ldcg(src + 1);
+                    v[0] += x.x;
+                    v[1] += x.y;
+                    v[2] += x.z;
+                    v[3] += x.w;
+                    v[4] += y.x;
+                    v[5] += y.y;
+                    v[6] += y.z;
+                    v[7] += y.w;
+                  }
+                store_h(sl, c, e0, v);
+              }
+        }
+        if (last) {
+          asm volatile("fence.proxy.async;" ::: "memory");  // for the TMA loads of other CTAs
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) {
+            __threadfence();
+            atomicAdd(g.lk.done, 1);
+          }
         }
         continue;
       }
@@ -1091,6 +1146,9 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   g.m_tiles = (int)((g.rows + (PAIR ? 255 : 127)) / (PAIR ? 256 : 128));
   g.n_tiles = (int)((g.p.N + BN - 1) / BN);
   g.k_blocks = (int)((g.p.K + 63) / 64);
+  // Units that would wait for H take part in making it: up to 8 K splits of 2 blocks at least.
+  const int units = c.num_sms / (PAIR ? 2 : 1);
+  g.lk.ksplit = std::max(1, std::min({8, units / g.m_tiles, g.k_blocks / 2}));
   if (overlap) {
     const int64_t groups = (g.rows + kGroup - 1) / kGroup;
     map_2d(&th, g.lk.H, g.lk.cw, groups * g.lk.q_max * kGroup, g.lk.cw, g.lk.cw, 128, swizzle_of(g.lk.cw));
@@ -1139,7 +1197,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
 struct Big {
   LoraK lk;
   int64_t rows;  // rows of a block, a multiple of kGroup
-  size_t lists_at, h_at, bytes;
+  size_t lists_at, arrived_at, part_at, h_at, bytes;
 };
 Big lay_out_big(const LoraLinear& p, size_t at) {
   Big b{};
@@ -1154,8 +1212,13 @@ Big lay_out_big(const LoraLinear& p, size_t at) {
   // H holds every chunk a group could need; blocks of rows keep it within 128 MB.
   const int64_t group = (int64_t)b.lk.q_max * kGroup * b.lk.cw * 2;
   b.rows = std::min(b.rows, std::max<int64_t>(1, ((int64_t)128 << 20) / group) * kGroup);
-  b.h_at = at + 256 + align256((size_t)(b.rows / kGroup) * sizeof(GroupList));  // `done`, the lists, H
-  b.bytes = b.h_at + align256((size_t)(b.rows / kGroup) * group);
+  // `done`, the lists, `arrived`, the K splits' parts (splits x rows of tiles <= units), H.
+  const int64_t groups = b.rows / kGroup;
+  b.arrived_at = at + 256 + align256((size_t)groups * sizeof(GroupList));
+  b.part_at = b.arrived_at + align256((size_t)groups * 32);
+  const int64_t part_rows = std::min<int64_t>(8 * b.rows, std::max<int64_t>(b.rows, (int64_t)ctx().num_sms * 128 + kGroup));
+  b.h_at = b.part_at + align256((size_t)(part_rows * b.lk.rc * b.lk.cw) * 4);
+  b.bytes = b.h_at + align256((size_t)groups * group);
   return b;
 }
 
@@ -1168,6 +1231,8 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   g.lk = big.lk;
   g.lk.done = reinterpret_cast<int*>(ws + big.lists_at);
   g.lk.lists = reinterpret_cast<GroupList*>(ws + big.lists_at + 256);
+  g.lk.arrived = reinterpret_cast<int*>(ws + big.arrived_at);
+  g.lk.part = reinterpret_cast<float*>(ws + big.part_at);
   g.lk.H = reinterpret_cast<uint16_t*>(ws + big.h_at);
   g.X = X;
   g.W = W;
