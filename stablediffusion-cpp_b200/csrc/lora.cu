@@ -432,6 +432,42 @@ Operands lay_out(const LoraLinear& p) {
   return o;
 }
 
+// Up to four matrices in one launch: rows of `cols` values, bf16 or fp32 (rounded to bf16),
+// to rows of `pitch` bf16, zero past cols. Eight values a thread: 16-byte stores, loads that a
+// warp's lines cover. Bound by memory; the copies of packed operands would otherwise cost more
+// than the product of a few rows (46 us for a 455 x 8276 W with one value a thread).
+struct PackOne {
+  const void* src;
+  uint16_t* dst;
+  int64_t ld, rows;
+  int cols, pitch, f32;
+};
+struct PackAll {
+  PackOne m[4];
+  int64_t end[4];  // chunks up to and with matrix i
+  int n;
+};
+__global__ void __launch_bounds__(256) k_lora_pack(const __grid_constant__ PackAll all) {
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < all.end[all.n - 1]; u += (int64_t)gridDim.x * 256) {
+    int i = 0;
+    while (u >= all.end[i]) ++i;
+    const PackOne& m = all.m[i];
+    const int64_t x = i ? u - all.end[i - 1] : u;
+    const int per = m.pitch / 8;
+    const int64_t r = x / per;
+    const int c = (int)(x - r * per) * 8;
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < m.cols) {
+        const int64_t at = r * m.ld + c + e;
+        const uint32_t v = m.f32 ? f32_to_bf16_rne(((const float*)m.src)[at]) : ((const uint16_t*)m.src)[at];
+        w[e >> 1] |= v << (16 * (e & 1));
+      }
+    *reinterpret_cast<uint4*>(m.dst + r * m.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 int rows_tile(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128; }
 RowsK lay_out_rows(const LoraLinear& p, uint8_t* at, size_t* bytes) {
   RowsK k{};
@@ -512,6 +548,7 @@ void launch_rows(LoraRows g) {
 // ------------------------------------------------------------------------------------
 // Many rows: Y = [X | H] [W | B]^T as one GEMM.
 // ------------------------------------------------------------------------------------
+constexpr int kMaxSmem = 232448;
 constexpr int kGroup = 256;  // rows that share a list of adapters and a block of H
 constexpr int kHash = 512;
 
@@ -526,7 +563,7 @@ struct LoraK {
   GroupList* lists;
   int* done;     // warps of k_lora_gemm that have stored their part of H
   int* arrived;  // [groups][8]: K splits that have stored their part, for 32 rows each
-  float* part;   // [rows][ksplit][rc cw]: the splits' parts of a row's own h
+  float4* part;  // [32-row blocks][ksplit][rc cw / 4][32]: the splits' parts of the rows' own h, for whole lines
   int ksplit;
   uint16_t* H;
   int cw, rc, parts, q_max;
@@ -672,8 +709,10 @@ template <int BN, bool PAIR>
 struct LoraGemmCfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = 208 * 1024 / STAGE > 8 ? 8 : 208 * 1024 / STAGE;
-  static constexpr int SMEM = 1024 + STAGES * STAGE;
+  static constexpr int STG_BYTES = 4 * 2 * 32 * 128;  // two 32 x 32 blocks of Y per epilogue warp
+  static constexpr int FIT = (kMaxSmem - 1024 - STG_BYTES - 2560) / STAGE;  // 2560: barriers, bias
+  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + STG_BYTES;
   static constexpr uint32_t COLS = 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
 };
 struct LoraGemm {
@@ -683,7 +722,7 @@ struct LoraGemm {
   int64_t ldx, ldw, ldb;
   int64_t row0, rows;
   int m_tiles, n_tiles, k_blocks;
-  int y_vec, bias_vec;
+  int y_tma;
   __device__ int down_items() const { return lk.q_max ? m_tiles * lk.ksplit : 0; }
 };
 // Columns of the accumulator that `n` ranks take: a pair's MMA has a multiple of 32.
@@ -704,7 +743,8 @@ template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kRowThreads, 1)
     k_lora_gemm(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                 const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmB,
-                const __grid_constant__ CUtensorMap tmA, const __grid_constant__ LoraGemm g) {
+                const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmY,
+                const __grid_constant__ LoraGemm g) {
   using C_ = LoraGemmCfg<BN, PAIR>;
   constexpr int STAGES = C_::STAGES, CTAS = PAIR ? 2 : 1;
   constexpr uint32_t IDESC = make_idesc(1u, 0, 0, PAIR ? 256 : 128, BN);
@@ -713,6 +753,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word, pass_ids[BN / 16];  // adapters of the chunks of a pass
+  __shared__ float4 sbias[2][BN / 4];            // bias of the tile's columns, by accumulator
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -895,7 +936,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           }
           if (!ok) break;
           if (!down && downs) {
-              const int nq = g.lk.chunks(count);
+            const int nq = g.lk.chunks(count);
             for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(STAGES)) {
               const int s = at.slot;
               ok = mbar_wait(&full[s], at.phase, abort_flag, err, kErrWaitFull);
@@ -931,6 +972,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   } else {
     const int q = warp & 3;
     const uint32_t acc_empty0 = PAIR ? mapa_shared(&acc_empty[0], 0) : 0;
+    uint8_t* const stg = smem + STAGES * C_::STAGE + q * 8192;
+    uint8_t* buf = stg;
     int n = 0;
     bool ok = true;
     auto release = [&](int acc) {
@@ -953,7 +996,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const float scale = mine >= 0 && g.p.scale ? g.p.scale[L->adapter[mine]] : 1.0f;
         uint16_t* rowH = g.lk.H + ((int64_t)(L - g.lk.lists) * g.lk.q_max * kGroup + me) * cw;
         const int rp = g.lk.rc * cw;
-        float* part = g.lk.part + ((int64_t)(mb * CTAS + (int)rank) * 128 + q * 32 + lane) * g.lk.ksplit * rp;
+        float4* part = g.lk.part + ((int64_t)(mb * CTAS + (int)rank) * 4 + q) * g.lk.ksplit * (rp / 4) * 32 + lane;
         auto store_h = [&](int sl, int c, int e0, const float (&v)[8]) {
           for (int pt = 0; pt < g.lk.parts; ++pt) {
             uint32_t w[4] = {0, 0, 0, 0};
@@ -996,9 +1039,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
               if (g.lk.ksplit == 1) {
                 store_h(sl, c, e0, v);
               } else if (sl == mine) {
-                float4* dst = reinterpret_cast<float4*>(part + sp * rp + c * cw + e0);
+                float4* dst = part + (sp * rp + c * cw + e0) / 4 * 32;
                 dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                dst[32] = make_float4(v[4], v[5], v[6], v[7]);
               }
             }
           }
@@ -1014,25 +1057,29 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           last = __shfl_sync(0xffffffffu, before, 0) == g.lk.ksplit - 1;
           __threadfence();
           if (last)
-            for (int i = 0; i < nch; ++i)
-              for (int e0 = 0; e0 < cw; e0 += 8) {
-                const int sl = i / g.lk.rc, c = i % g.lk.rc;
-                float v[8] = {};
-                if (sl == mine)
-                  for (int s = 0; s < g.lk.ksplit; ++s) {
-                    const float4* src = reinterpret_cast<const float4*>(part + s * rp + c * cw + e0);
-                    const float4 x = __ldcg(src), y = __ldcg(src + 1);
-                    v[0] += x.x;
-                    v[1] += x.y;
-                    v[2] += x.z;
-                    v[3] += x.w;
-                    v[4] += y.x;
-                    v[5] += y.y;
-                    v[6] += y.z;
-                    v[7] += y.w;
-                  }
-                store_h(sl, c, e0, v);
+            for (int x = 0; x < rp; x += 8) {
+              float4 a[8], b[8];  // this row's own eight ranks of every split, all loads in flight
+#pragma unroll
+              for (int s = 0; s < 8; ++s) {
+                const bool there = mine >= 0 && s < g.lk.ksplit;
+                const float4* src = part + ((there ? s : 0) * rp + x) / 4 * 32;
+                a[s] = there ? __ldcg(src) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                b[s] = there ? __ldcg(src + 32) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
               }
+              float v[8] = {};
+#pragma unroll
+              for (int s = 0; s < 8; ++s) {
+                v[0] += a[s].x;
+                v[1] += a[s].y;
+                v[2] += a[s].z;
+                v[3] += a[s].w;
+                v[4] += b[s].x;
+                v[5] += b[s].y;
+                v[6] += b[s].z;
+                v[7] += b[s].w;
+              }
+              for (int sl = 0; sl * g.lk.rc < nch; ++sl) store_h(sl, x / cw, x % cw, v);
+            }
         }
         if (last) {
           asm volatile("fence.proxy.async;" ::: "memory");  // for the TMA loads of other CTAs
@@ -1048,11 +1095,20 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const int acc = n & 1;
       int mb, nb;
       tile_at(it - downs, g.m_tiles, g.n_tiles, mb, nb);
-      if (!mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull)) break;
-      ++n;
-      tc_fence_after();
+      // What the tile needs beside its sums is read before they are complete.
       const int local = (mb * CTAS + (int)rank) * 128 + q * 32 + lane;
       const bool row_ok = local < g.rows, mixed = g.lk.q_max && __ldcg(&list_of(mb)->mixed);
+      if (g.p.bias) {
+        for (int c = threadIdx.x - 64; c < BN; c += 128) {
+          const int64_t col = (int64_t)nb * BN + c;
+          reinterpret_cast<float*>(sbias[acc])[c] = col < g.p.N ? __ldg(g.p.bias + col) : 0.0f;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      ok = mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
+      if (!ok) break;
+      ++n;
+      tc_fence_after();
       const int64_t row = g.row0 + local;
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
@@ -1063,64 +1119,83 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const int64_t col0 = (int64_t)nb * BN + c * 32;
         if (col0 >= g.p.N) continue;
         const int cols = (int)min((int64_t)32, g.p.N - col0);
+        if (g.y_tma) {
+          // The block that used this buffer has left it (of 2 fp32 or 4 bf16 buffers).
+          if (lane == 0) {
+            if (g.p.y_bf16)
+              tma_store_wait_read<3>();
+            else
+              tma_store_wait_read<1>();
+          }
+          __syncwarp();
+        }
         if (row_ok) {
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
           if (g.p.bias) {
-            if (g.bias_vec && cols == 32) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 b = __ldg(reinterpret_cast<const float4*>(g.p.bias + col0 + j));
-                v[j] += b.x;
-                v[j + 1] += b.y;
-                v[j + 2] += b.z;
-                v[j + 3] += b.w;
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < cols) v[j] += __ldg(g.p.bias + col0 + j);
+            for (int j = 0; j < 32; j += 4) {
+              const float4 b = sbias[acc][(c * 32 + j) / 4];
+              v[j] += b.x;
+              v[j + 1] += b.y;
+              v[j + 2] += b.z;
+              v[j + 3] += b.w;
             }
           }
-          if (g.p.y_bf16) {
-            uint16_t* y = (uint16_t*)g.p.Y + row * g.p.ldy + col0;
-            if (g.y_vec && cols == 32) {
+          if (g.y_tma) {
+            // 16-byte pieces in the swizzle of the box's row: 64 bytes of bf16 or 128 of fp32.
+            if (g.p.y_bf16) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 8)
-                *reinterpret_cast<uint4*>(y + j) = make_uint4(pack_bf16x2(v[j], v[j + 1]), pack_bf16x2(v[j + 2], v[j + 3]),
-                                                              pack_bf16x2(v[j + 4], v[j + 5]), pack_bf16x2(v[j + 6], v[j + 7]));
+              for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<uint4*>(buf + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) =
+                    make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                               pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < cols) y[j] = f32_to_bf16_rne(v[j]);
+              for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<float4*>(buf + lane * 128 + (j ^ (lane & 7)) * 16) =
+                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
+          } else if (g.p.y_bf16) {
+            uint16_t* y = (uint16_t*)g.p.Y + row * g.p.ldy + col0;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < cols) y[j] = f32_to_bf16_rne(v[j]);
           } else {
             float* y = (float*)g.p.Y + row * g.p.ldy + col0;
-            if (g.y_vec && cols == 32) {
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(y + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j < cols) y[j] = v[j];
-            }
+            for (int j = 0; j < 32; ++j)
+              if (j < cols) y[j] = v[j];
           }
         }
+        if (g.y_tma) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&tmY, buf, (int)col0, (int)(row - lane));
+          buf = stg + (buf - stg + (g.p.y_bf16 ? 2048 : 4096)) % 8192;
+        }
         if (mixed) {
-          uint32_t bad = 0;
-          if (row_ok) {
+          uint32_t bad = 0, top = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) top = max(top, r[j] & 0x7fffffffu);
+          if (row_ok && top >= 0x7f800000u) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (j < cols && (r[j] & 0x7fffffffu) >= 0x7f800000u) bad |= 1u << j;
           }
           __syncwarp();
-          if (__any_sync(0xffffffffu, bad != 0))
+          if (__any_sync(0xffffffffu, bad != 0)) {
+            if (lane == 0) tma_store_wait_all();  // what was stored above is replaced
+            __syncwarp();
             redo_chunk(g.p, g.lk, g.X, g.ldx, g.W, g.ldw, g.B, g.ldb, g.row0, local, col0, bad);
+          }
         }
       }
       release(acc);
     }
+    if (lane == 0) tma_store_wait_all();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -1157,6 +1232,14 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   } else {
     th = tb = ta = tx;  // not read
   }
+  CUtensorMap ty = tx;
+  if (g.y_tma) {
+    const uint64_t dims[2] = {(uint64_t)g.p.N, (uint64_t)g.p.T};
+    const uint64_t str[1] = {(uint64_t)g.p.ldy * (g.p.y_bf16 ? 2 : 4)};
+    const uint32_t box[2] = {32, 32};
+    encode_tmap(&ty, g.p.y_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, g.p.Y, dims, str, box,
+                g.p.y_bf16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+  }
   static int clusters[64] = {};
   auto kern = k_lora_gemm<BN, PAIR>;
   cudaLaunchConfig_t cfg{};
@@ -1188,8 +1271,9 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
     ++n;
   }
   cfg.numAttrs = n;
-  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(clusters[c.device], (int64_t)g.m_tiles * g.n_tiles) * (PAIR ? 2 : 1)));
-  check_cuda(cudaLaunchKernelEx(&cfg, kern, tx, tw, th, tb, ta, g), "linear_lora");
+  const int64_t items = (int64_t)g.m_tiles * (g.n_tiles + (overlap ? g.lk.ksplit : 0));
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(clusters[c.device], items) * (PAIR ? 2 : 1)));
+  check_cuda(cudaLaunchKernelEx(&cfg, kern, tx, tw, th, tb, ta, ty, g), "linear_lora");
   check_launch("linear_lora");
 }
 
@@ -1232,7 +1316,7 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   g.lk.done = reinterpret_cast<int*>(ws + big.lists_at);
   g.lk.lists = reinterpret_cast<GroupList*>(ws + big.lists_at + 256);
   g.lk.arrived = reinterpret_cast<int*>(ws + big.arrived_at);
-  g.lk.part = reinterpret_cast<float*>(ws + big.part_at);
+  g.lk.part = reinterpret_cast<float4*>(ws + big.part_at);
   g.lk.H = reinterpret_cast<uint16_t*>(ws + big.h_at);
   g.X = X;
   g.W = W;
@@ -1240,8 +1324,7 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   g.ldx = ldx;
   g.ldw = ldw;
   g.ldb = ldb;
-  g.y_vec = aligned16(p.Y) && p.ldy % (p.y_bf16 ? 8 : 4) == 0;
-  g.bias_vec = p.bias && aligned16(p.bias);
+  g.y_tma = aligned16(p.Y) && p.ldy % (p.y_bf16 ? 8 : 4) == 0;
   for (g.row0 = 0; g.row0 < p.T; g.row0 += big.rows) {
     g.rows = std::min(big.rows, p.T - g.row0);
     if (adapters) {
@@ -1300,29 +1383,24 @@ void launch_lora_linear(LoraLinear p, void* ws_) {
   uint8_t* ws = static_cast<uint8_t*>(ws_);
   const uint16_t *X = (const uint16_t*)p.X, *W = p.W, *A = p.A, *B = p.B;
   int64_t ldx = p.ldx, ldw = p.ldw, lda = p.lda, ldb = p.ldb;
-  auto take = [&](size_t at) { return reinterpret_cast<uint16_t*>(ws + at); };
-  if (o.pack_x) {
-    if (p.x_bf16)
-      launch_copy2d(p.X, p.ldx, take(o.x_at), o.Kp, p.T, p.K, 2);
-    else
-      launch_pack_bf16((const float*)p.X, p.ldx, take(o.x_at), o.Kp, p.T, p.K);
-    X = take(o.x_at);
-    ldx = o.Kp;
-  }
-  if (o.pack_w) {
-    launch_copy2d(W, ldw, take(o.w_at), o.Kp, p.N, p.K, 2);
-    W = take(o.w_at);
-    ldw = o.Kp;
-  }
-  if (o.pack_a) {
-    launch_copy2d(A, lda, take(o.a_at), o.Kp, p.n_adapters * p.r, p.K, 2);
-    A = take(o.a_at);
-    lda = o.Kp;
-  }
-  if (o.pack_b) {
-    launch_copy2d(B, ldb, take(o.b_at), o.rb, p.n_adapters * p.N, p.r, 2);
-    B = take(o.b_at);
-    ldb = o.rb;
+  PackAll all{};
+  auto pack = [&](bool need, const uint16_t*& x, int64_t& ld, int64_t rows, int64_t cols, int64_t pitch, size_t at, bool f32) {
+    if (!need) return;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(ws + at);
+    all.m[all.n] = PackOne{x, dst, ld, rows, (int)cols, (int)pitch, f32 ? 1 : 0};
+    all.end[all.n] = (all.n ? all.end[all.n - 1] : 0) + rows * (pitch / 8);
+    ++all.n;
+    x = dst;
+    ld = pitch;
+  };
+  pack(o.pack_x, X, ldx, p.T, p.K, o.Kp, o.x_at, !p.x_bf16);
+  pack(o.pack_w, W, ldw, p.N, p.K, o.Kp, o.w_at, false);
+  pack(o.pack_a, A, lda, p.n_adapters * p.r, p.K, o.Kp, o.a_at, false);
+  pack(o.pack_b, B, ldb, p.n_adapters * p.N, p.r, o.rb, o.b_at, false);
+  if (all.n) {
+    const int64_t grid = std::min<int64_t>((all.end[all.n - 1] + 255) / 256, (int64_t)c.num_sms * 16);
+    k_lora_pack<<<(unsigned)grid, 256, 0, c.stream>>>(all);
+    check_launch("lora_pack");
   }
   if (p.T > kMaxRowsSmall) return launch_big(p, X, ldx, W, ldw, A, lda, B, ldb, ws, lay_out_big(p, o.h_at));
   size_t h;
