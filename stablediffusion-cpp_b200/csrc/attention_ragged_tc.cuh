@@ -524,20 +524,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
-      if (lane == 0 && nkv > 0) {
+      if (nkv > 0) {  // the whole warp: an elected lane issues
         const int nq = two ? 2 : 1;
-        mbar_arrive_expect_tx(q_full, nq * C_::ATOMS * p.G * p.tpt * 128);
+        const uint32_t qbar = smem_u32(q_full), ring = smem_u32(sR), full0 = smem_u32(r_full);
+        mbar_expect_tx_elect(qbar, nq * C_::ATOMS * p.G * p.tpt * 128);
         for (int t = 0; t < nq; ++t)
           for (int a = 0; a < C_::ATOMS; ++a)
-            tma_load_3d(sQ + t * C_::Q_BYTES + a * C_::ATOM, &tmQ, q_full, a * 64, kvh * p.G, q.q0 + tok0 + t * p.tpt);
+            tma_load_3d_elect(smem_u32(sQ) + t * C_::Q_BYTES + a * C_::ATOM, &tmQ, qbar, a * 64, kvh * p.G,
+                              q.q0 + tok0 + t * p.tpt);
         int issued = -1;
-        for (int i = 0; i < 2 * nkv; ++i) {
-          const int sl = i % SLOTS, u = i / SLOTS;
-          if (!mbar_wait(&r_empty[sl], (u & 1) ^ 1u, abort_flag, err, kErrAttnWait)) break;
-          mbar_arrive_expect_tx(&r_full[sl], C_::KV_BYTES);
+        RingPos at;
+        for (int i = 0; i < 2 * nkv; ++i, at.next(SLOTS)) {
+          if (!mbar_wait(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait)) break;
+          const uint32_t bar = full0 + (uint32_t)(at.slot * 8), dst = ring + (uint32_t)(at.slot * C_::KV_BYTES);
+          mbar_expect_tx_elect(bar, C_::KV_BYTES);
           const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
           for (int a = 0; a < C_::ATOMS; ++a)
-            tma_load_3d(sR + sl * C_::KV_BYTES + a * C_::ATOM, tm, &r_full[sl], a * 64, kvh, q.k0 + (i >> 1) * kBK);
+            tma_load_3d_elect(dst + a * C_::ATOM, tm, bar, a * 64, kvh, q.k0 + (i >> 1) * kBK);
           issued = i;
         }
         if (issued < 2 * nkv - 1) {
@@ -557,76 +560,59 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (nt > 0 || (t == 0 && two)) {
         bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrAttnWait);
         tc_fence_after();
-        const uint32_t q_addr = smem_u32(sQ + t * C_::Q_BYTES);
+        const uint64_t qd = sdesc_k_sw128(smem_u32(sQ + t * C_::Q_BYTES)), kd0 = sdesc_k_sw128(smem_u32(sR));
+        const uint64_t vd0 = sdesc_mn_sw128(smem_u32(sR), C_::ATOM, 1024);
         const uint32_t d_s = tmem + (uint32_t)(t * kBK);
         const uint32_t d_o = tmem + kOCol + (uint32_t)(t * DP);
-        uint64_t qd[8] = {};
-        uint32_t pa[8];
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          if (ks < DP / 16) qd[ks] = sdesc_k_sw128(q_addr + (uint32_t)((ks >> 2) * C_::ATOM + (ks & 3) * 32));
-          pa[ks] = d_s + (uint32_t)(ks * 8);
-        }
+        RingPos k, v;  // K_j is load 2j of the ring, V_j load 2j + 1
+        v.next(SLOTS);
         for (int j = 0; ok && j <= nkv; ++j) {
-          const int vi = 2 * j - 1, ki = 2 * j;
-          const int vsl = (vi + SLOTS) % SLOTS, ksl = ki % SLOTS;
-          uint8_t* vp = sR + vsl * C_::KV_BYTES;
-          const uint32_t v_addr = smem_u32(vp), k_addr = smem_u32(sR + ksl * C_::KV_BYTES);
-          uint64_t vd[8], kd[8] = {};
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            vd[ks] = sdesc_mn_sw128(v_addr + (uint32_t)(ks * 16 * 128), C_::ATOM, 1024);
-            if (ks < DP / 16) kd[ks] = sdesc_k_sw128(k_addr + (uint32_t)((ks >> 2) * C_::ATOM + (ks & 3) * 32));
-          }
-          if (j > 0 && !mbar_wait(&r_full[vsl], (vi / SLOTS) & 1, abort_flag, err, kErrAttnWait)) break;
-          if (j < nkv && !mbar_wait(&r_full[ksl], (ki / SLOTS) & 1, abort_flag, err, kErrAttnWait)) break;
+          // K_j and V_(j-1) normally landed long ago; waiting for them before P_t(j-1) lets the
+          // PV and the QK^T go out back to back once P is there.
+          if (j > 0 && !mbar_wait(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait)) break;
+          if (j < nkv && !mbar_wait(&r_full[k.slot], k.phase, abort_flag, err, kErrAttnWait)) break;
           if (j > 0) {
             if (j <= nt) {
-              if (j * kBK > q.kl) zero_v_tail<DP>(vp, q.kl - (j - 1) * kBK);
+              if (j * kBK > q.kl) zero_v_tail<DP>(sR + v.slot * C_::KV_BYTES, q.kl - (j - 1) * kBK);
+              const uint64_t vd = vd0 + (uint64_t)(v.slot * (C_::KV_BYTES >> 4));
               if (!mbar_wait(&p_half[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
               tc_fence_after();
-              if (lane == 0) {
-                const uint32_t a4[4] = {pa[0], pa[1], pa[2], pa[3]};
-                const uint64_t b4[4] = {vd[0], vd[1], vd[2], vd[3]};
-                umma4_f16_ts(d_o, a4, b4, IDESC_O, j > 1 ? 1u : 0u);
-              }
+              umma4_f16_ts_elect(d_o, d_s, vd, IDESC_O, j > 1 ? 1u : 0u);
               if (!mbar_wait(&p_full[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
               tc_fence_after();
-              if (lane == 0) {
-                const uint32_t a4[4] = {pa[4], pa[5], pa[6], pa[7]};
-                const uint64_t b4[4] = {vd[4], vd[5], vd[6], vd[7]};
-                umma4_f16_ts(d_o, a4, b4, IDESC_O, 1u);
-                umma_commit(&r_empty[vsl]);
-                if (j == nt) umma_commit(&o_final[t]);
-              }
+              umma4_f16_ts_elect(d_o, d_s + 32, vd + 512, IDESC_O, 1u);
+              umma_commit_elect(&r_empty[v.slot]);
+              if (j == nt) umma_commit_elect(&o_final[t]);
             } else if (lane == 0) {
-              mbar_arrive(&r_empty[vsl]);  // the other tile's keys
+              mbar_arrive(&r_empty[v.slot]);  // the other tile's keys
             }
+            v.next(SLOTS);
+            v.next(SLOTS);
           }
-          if (j < nkv && lane == 0) {
+          if (j < nkv) {
             if (j < nt) {
+              const uint64_t kd = kd0 + (uint64_t)(k.slot * (C_::KV_BYTES >> 4));
               tc_fence_after();
               if constexpr (DP == 128)
-                umma8_f16_ss(d_s, qd, kd, IDESC_S, 0u);
-              else {
-                const uint64_t a4[4] = {qd[0], qd[1], qd[2], qd[3]};
-                const uint64_t b4[4] = {kd[0], kd[1], kd[2], kd[3]};
-                umma4_f16_ss(d_s, a4, b4, IDESC_S, 0u);
-              }
-              umma_commit(&s_full[t]);
-              umma_commit(&r_empty[ksl]);
-            } else {
-              mbar_arrive(&r_empty[ksl]);
+                umma8_f16_ss_elect(d_s, qd, kd, IDESC_S);
+              else
+                umma4_f16_ss_elect(d_s, qd, kd, IDESC_S);
+              umma_commit_elect(&s_full[t]);
+              umma_commit_elect(&r_empty[k.slot]);
+            } else if (lane == 0) {
+              mbar_arrive(&r_empty[k.slot]);
             }
+            k.next(SLOTS);
+            k.next(SLOTS);
           }
           __syncwarp();
         }
-        if (lane == 0) {
-          umma_commit(&drain[t]);
+        umma_commit_elect(&drain[t]);
+        {
           const uint64_t t0 = globaltimer_ns();
           while (!mbar_try_wait(&drain[t], 0))
             if (globaltimer_ns() - t0 > kWaitLimitNs) {
-              atomicOr(err, kErrWaitDrain);
+              if (lane == 0) atomicOr(err, kErrWaitDrain);
               break;
             }
         }
@@ -841,29 +827,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     if (warp == 0 || warp == 3) {
       // ------------------------------ TMA producer ------------------------------
-      if (lane == 0) {
-        int ld = 0, nq = 0;  // loads and Q tiles so far: slot ld % SL, its use ld / SL
+      {  // the whole warp: an elected lane issues
+        const uint32_t qbar = smem_u32(q_full), ring = smem_u32(sR), full0 = smem_u32(r_full);
+        int ld = 0, nq = 0;  // loads and Q tiles so far
+        RingPos at;
         bool ok = true;
         while (ok && it.next()) {
           const int nt = it.tiles();
           if (nt == 0) continue;
           const Seq& q = steps.seq[it.s];
-          for (int i = 0; i < 2 * nt && ok; ++i) {
-            if (i == 0) {
-              ok = mbar_wait(q_empty, (nq & 1) ^ 1u, abort_flag, err, kErrAttnWait);
-              if (!ok) break;
-              mbar_arrive_expect_tx(q_full, ATOMS * p.G * p.tpt * 128);
-              for (int a = 0; a < ATOMS; ++a)
-                tma_load_3d(sQ + a * p.q_atom, &tmQ, q_full, a * 64, it.kvh * p.G, q.q0);
-              ++nq;
-            }
-            const int sl = ld % SL;
-            ok = mbar_wait(&r_empty[sl], ((ld / SL) & 1) ^ 1u, abort_flag, err, kErrAttnWait);
+          ok = mbar_wait(q_empty, (nq & 1) ^ 1u, abort_flag, err, kErrAttnWait);
+          if (!ok) break;
+          mbar_expect_tx_elect(qbar, ATOMS * p.G * p.tpt * 128);
+          for (int a = 0; a < ATOMS; ++a)
+            tma_load_3d_elect(smem_u32(sQ) + a * p.q_atom, &tmQ, qbar, a * 64, it.kvh * p.G, q.q0);
+          ++nq;
+          for (int i = 0; i < 2 * nt && ok; ++i, at.next(SL)) {
+            ok = mbar_wait(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait);
             if (!ok) break;
-            mbar_arrive_expect_tx(&r_full[sl], KV_BYTES);
+            const uint32_t bar = full0 + (uint32_t)(at.slot * 8), dst = ring + (uint32_t)(at.slot * KV_BYTES);
+            mbar_expect_tx_elect(bar, KV_BYTES);
             const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
             for (int a = 0; a < ATOMS; ++a)
-              tma_load_3d(sR + sl * KV_BYTES + a * ATOM, tm, &r_full[sl], a * 64, it.kvh, q.k0 + (it.kt0 + (i >> 1)) * kBK);
+              tma_load_3d_elect(dst + a * ATOM, tm, bar, a * 64, it.kvh, q.k0 + (it.kt0 + (i >> 1)) * kBK);
             ++ld;
           }
         }
@@ -880,16 +866,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       // ------------------------------ MMA issuer --------------------------------
-      const uint32_t q_addr = smem_u32(sQ);
+      const uint64_t qd = sdesc_k_sw128(smem_u32(sQ)), kd0 = sdesc_k_sw128(smem_u32(sR));
+      const uint64_t vd0 = sdesc_mn_sw128(smem_u32(sR), ATOM, 1024);
+      const uint64_t q_jump = (uint64_t)(p.q_atom >> 4);  // a Q atom may be shorter than 128 rows
       const uint32_t d_s = tmem + (uint32_t)(t * kBK), d_o = tmem + kOCol + (uint32_t)(t * DP);
-      uint64_t qd[8] = {};
-      uint32_t pa[8];
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        if (ks < DP / 16) qd[ks] = sdesc_k_sw128(q_addr + (uint32_t)((ks >> 2) * p.q_atom + (ks & 3) * 32));
-        pa[ks] = d_s + (uint32_t)(ks * 8);
-      }
-      int ld = 0, nq = 0, step = 0;
+      int nq = 0, step = 0;
+      RingPos at;  // loads in order: K_0, V_0, K_1, V_1, ... of every piece
       bool ok = true;
       while (ok && it.next()) {
         const int nt = it.tiles();
@@ -898,73 +880,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(q_full, nq & 1, abort_flag, err, kErrAttnWait);
         ++nq;
         tc_fence_after();
-        // Loads ld + 2j (K_j) and ld + 2j + 1 (V_j) of this piece.
+        RingPos v = at;
+        v.next(SL);
         for (int j = 0; ok && j <= nt; ++j) {
-          const int vi = ld + 2 * j - 1, ki = ld + 2 * j;
           if (j > 0) {
-            const int sl = vi % SL;
-            uint8_t* vp = sR + sl * KV_BYTES;
-            const uint32_t v_addr = smem_u32(vp);
-            ok = mbar_wait(&r_full[sl], (vi / SL) & 1, abort_flag, err, kErrAttnWait);
+            uint8_t* vp = sR + v.slot * KV_BYTES;
+            ok = mbar_wait(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             const int left = kl - (it.kt0 + j - 1) * kBK;
             if (left < kBK) zero_v_tail<DP>(vp, left);
-            uint64_t vd[8];
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) vd[ks] = sdesc_mn_sw128(v_addr + (uint32_t)(ks * 16 * 128), ATOM, 1024);
+            const uint64_t vd = vd0 + (uint64_t)(v.slot * (KV_BYTES >> 4));
             ok = mbar_wait(p_half, (step - 1) & 1, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t a4[4] = {pa[0], pa[1], pa[2], pa[3]};
-              const uint64_t b4[4] = {vd[0], vd[1], vd[2], vd[3]};
-              umma4_f16_ts(d_o, a4, b4, IDESC_O, j > 1 ? 1u : 0u);
-            }
+            umma4_f16_ts_elect(d_o, d_s, vd, IDESC_O, j > 1 ? 1u : 0u);
             ok = mbar_wait(p_full, (step - 1) & 1, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t a4[4] = {pa[4], pa[5], pa[6], pa[7]};
-              const uint64_t b4[4] = {vd[4], vd[5], vd[6], vd[7]};
-              umma4_f16_ts(d_o, a4, b4, IDESC_O, 1u);
-              umma_commit(&r_empty[sl]);
-              if (j == nt) umma_commit(o_full);
-            }
+            umma4_f16_ts_elect(d_o, d_s + 32, vd + 512, IDESC_O, 1u);
+            umma_commit_elect(&r_empty[v.slot]);
+            if (j == nt) umma_commit_elect(o_full);
+            v.next(SL);
+            v.next(SL);
           }
           if (j < nt) {
-            const int sl = ki % SL;
-            const uint32_t k_addr = smem_u32(sR + sl * KV_BYTES);
-            ok = mbar_wait(&r_full[sl], (ki / SL) & 1, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait(&r_full[at.slot], at.phase, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
-            if (lane == 0) {
-              uint64_t kd[8] = {};
-#pragma unroll
-              for (int ks = 0; ks < DP / 16; ++ks)
-                kd[ks] = sdesc_k_sw128(k_addr + (uint32_t)((ks >> 2) * ATOM + (ks & 3) * 32));
-              if constexpr (DP == 128)
-                umma8_f16_ss(d_s, qd, kd, IDESC_S, 0u);
-              else {
-                const uint64_t a4[4] = {qd[0], qd[1], qd[2], qd[3]};
-                const uint64_t b4[4] = {kd[0], kd[1], kd[2], kd[3]};
-                umma4_f16_ss(d_s, a4, b4, IDESC_S, 0u);
-              }
-              umma_commit(s_full);
-              umma_commit(&r_empty[sl]);
-              if (j == nt - 1) umma_commit(q_empty);
-            }
+            const uint64_t kd = kd0 + (uint64_t)(at.slot * (KV_BYTES >> 4));
+            umma4_f16_ss_elect(d_s, qd, kd, IDESC_S);
+            if constexpr (DP == 128) umma4_f16_ss_elect(d_s, qd + q_jump, kd + (ATOM >> 4), IDESC_S, 1u);
+            umma_commit_elect(s_full);
+            umma_commit_elect(&r_empty[at.slot]);
+            if (j == nt - 1) umma_commit_elect(q_empty);
+            at.next(SL);
+            at.next(SL);
             ++step;
           }
           __syncwarp();
         }
-        ld += 2 * nt;
       }
-      if (lane == 0) {
-        umma_commit(drain);
+      umma_commit_elect(drain);
+      {
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(drain, 0))
           if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            atomicOr(err, kErrWaitDrain);
+            if (lane == 0) atomicOr(err, kErrWaitDrain);
             break;
           }
       }

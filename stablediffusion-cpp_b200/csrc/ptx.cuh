@@ -519,6 +519,65 @@ __device__ __forceinline__ void tma_load_3d_pair_elect(uint32_t dst, const CUten
       : "memory");
 }
 
+// Attention's products by the elected lane. S = Q K^T over 128 (umma8) or 64 (umma4) channels:
+// both operands K-major in a 128-byte swizzle, 64-channel atoms of 128 rows (1024 descriptor
+// units) behind one another. O += P V over 64 keys (umma4 ts): P in tensor memory (8 columns per
+// 16 keys), V MN-major (16 rows of 128 bytes = 128 units per step).
+__device__ __forceinline__ void umma8_f16_ss_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %3, %3;\n\tsetp.eq.b32 t, %3, %3;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 1024;\n\tadd.s64 y, %2, 1024;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 1026;\n\tadd.s64 y, %2, 1026;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 1028;\n\tadd.s64 y, %2, 1028;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 1030;\n\tadd.s64 y, %2, 1030;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
+__device__ __forceinline__ void umma4_f16_ss_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                                   uint32_t acc_first = 0) {
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 x, y;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %3, %3;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, t;\n\t"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc_first)
+      : "memory");
+}
+__device__ __forceinline__ void umma4_f16_ts_elect(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc_first) {
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 y;\n\t.reg .b32 z;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "add.s32 z, %1, 8;\n\tadd.s64 y, %2, 128;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [z], y, %3, t;\n\t"
+      "add.s32 z, %1, 16;\n\tadd.s64 y, %2, 256;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [z], y, %3, t;\n\t"
+      "add.s32 z, %1, 24;\n\tadd.s64 y, %2, 384;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [z], y, %3, t;\n\t"
+      "}\n" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc_first)
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
