@@ -112,6 +112,10 @@ void launch_tensor_core(const RaggedAttention& a, void* ws) {
   if (a.cap > 0.0f) {
     p.cap_in = 2.0f * kLog2e * a.scale / a.cap;
     p.cap_log2 = a.cap * kLog2e;
+    p.cap_x = a.scale / a.cap;
+    p.cap_small = a.cap / a.scale;
+    const float c[6] = {0.9999968409538269f, -0.3332400321960449f, 0.13253524899482727f, -0.05097286403179169f, 0.016114182770252228f, -0.002839465858414769f};
+    for (int i = 0; i < 6; ++i) p.tanh_c[i] = c[i] * p.cap_log2;
   }
   p.out_vec = aligned16(a.out) && a.ldo % 8 == 0;
   const bool streams = one_tile(a);

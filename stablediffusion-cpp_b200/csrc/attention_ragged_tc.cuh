@@ -51,6 +51,9 @@ struct TcParams {
   float scale_log2;    // scale log2(e)
   float cap_in;        // 2 log2(e) scale / cap
   float cap_log2;      // cap log2(e)
+  float cap_x;         // scale / cap
+  float cap_small;     // |q.k| up to which tanh is a polynomial: cap / scale
+  float tanh_c[6];     // its coefficients, times cap log2(e)
   int out_vec;         // 16-byte stores allowed
   // k_ragged_streams
   int slots, q_atom;   // K / V slots per worker, bytes of one 64-channel Q atom
@@ -142,25 +145,52 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
   for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x32(s_addr + (uint32_t)(g * 32), u[g]);
   tmem_wait_ld();
   if constexpr (MOD != 0) {
-    // To log2 units. tanh(x) = 1 - 2 / (1 + e^2x): exact to 2^-23 of 1 where tanh.approx is to
-    // 2^-11, which times a cap of 50 would be 2% of a probability. e^2x = inf gives 1.
+    // To log2 units. tanh(x) is x p(x^2) for |x| <= 1, p of degree 5 fitted to tanh(sqrt(y)) /
+    // sqrt(y) on [0, 1] for the least maximal error (3.2e-7 in fp32): eight packed
+    // multiply-adds a pair. A warp with a larger score takes 1 - 2 / (1 + e^2x), as exact
+    // (e^2x = inf gives 1), but two more MUFU operations a score beside the exponential: that
+    // bounded the kernel (286 instead of 230 us on six documents of 333 to 2500 tokens,
+    // 32 heads). tanh.approx is exact to 2^-11 only, which times a cap of 50 would be 2% of a probability.
+    bool small = true;
+    if constexpr (MOD & 1) {
+      float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < kBK; c += 2) {
-      float2 z = make_float2(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1]));
-      if constexpr (MOD & 1) {
-        z = fmul2(z, make_float2(p.cap_in, p.cap_in));
-        const float2 e = fadd2(make_float2(ex2_approx(z.x), ex2_approx(z.y)), make_float2(1.0f, 1.0f));
-        z = ffma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), make_float2(-2.0f * p.cap_log2, -2.0f * p.cap_log2),
-                  make_float2(p.cap_log2, p.cap_log2));
-      } else {
-        z = fmul2(z, make_float2(p.scale_log2, p.scale_log2));
+      for (int c = 0; c < kBK; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top[i] = fmax3(top[i], fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i])),
+                         fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1])));
+      small = !__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
+    }
+    auto modify = [&](auto curve) {
+#pragma unroll
+      for (int c = 0; c < kBK; c += 2) {
+        float2 z = curve(make_float2(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1])));
+        if constexpr (MOD & 2) {
+          z.x = fmaf(nslope, fabsf(dist0 - (float)c), z.x);
+          z.y = fmaf(nslope, fabsf(dist0 - (float)(c + 1)), z.y);
+        }
+        u[c >> 5][c & 31] = __float_as_uint(z.x);
+        u[c >> 5][(c & 31) + 1] = __float_as_uint(z.y);
       }
-      if constexpr (MOD & 2) {
-        z.x = fmaf(nslope, fabsf(dist0 - (float)c), z.x);
-        z.y = fmaf(nslope, fabsf(dist0 - (float)(c + 1)), z.y);
-      }
-      u[c >> 5][c & 31] = __float_as_uint(z.x);
-      u[c >> 5][(c & 31) + 1] = __float_as_uint(z.y);
+    };
+    auto both = [](float x) { return make_float2(x, x); };
+    if constexpr (!(MOD & 1)) {
+      modify([&](float2 z) { return fmul2(z, both(p.scale_log2)); });
+    } else if (small) {
+      modify([&](float2 z) {
+        const float2 x = fmul2(z, both(p.cap_x)), y = fmul2(x, x);
+        float2 r = ffma2(y, both(p.tanh_c[5]), both(p.tanh_c[4]));
+#pragma unroll
+        for (int i = 3; i >= 0; --i) r = ffma2(y, r, both(p.tanh_c[i]));
+        return fmul2(x, r);
+      });
+    } else {
+      modify([&](float2 z) {
+        z = fmul2(z, both(p.cap_in));
+        const float2 e = fadd2(make_float2(ex2_approx(z.x), ex2_approx(z.y)), both(1.0f));
+        return ffma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), both(-2.0f * p.cap_log2), both(p.cap_log2));
+      });
     }
   }
   if (masked) {
