@@ -44,6 +44,7 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays <= 256
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSeqs = 512;  // sequences of one k_ragged_streams launch
 constexpr int kMaxSmem = 232448;
+constexpr int kFewRows = 16, kFewPad = 32 * 128;
 
 struct TcParams {
   RaggedAttention a;
@@ -59,7 +60,7 @@ struct TcParams {
   int slots, q_atom;   // K / V slots per worker, bytes of one 64-channel Q atom
   float* part;         // [2 workers' pieces][rows][d + 2]: O, m, l
   int part_rows;       // rows of a piece: G * max_q
-  int seq0;            // first sequence of this launch
+  int seq0, seqs;      // first sequence of this launch, most sequences of one
 };
 
 template <class T>
@@ -132,6 +133,32 @@ __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, 
   return w;
 }
 
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Two scores q.k to log2 units, MOD bit 0: capped. tanh(x) is x p(x^2) for |x| <= 1, p of
+// degree 5 fitted to tanh(sqrt(y)) / sqrt(y) on [0, 1] for the least maximal error (3.2e-7 in
+// fp32): eight packed multiply-adds a pair. A warp with a larger score (small = false) takes
+// 1 - 2 / (1 + e^2x), as exact (e^2x = inf gives 1), but two more MUFU operations a score
+// beside the exponential: that bounded the kernel (286 instead of 230 us on six documents of
+// 333 to 2500 tokens, 32 heads). tanh.approx is exact to 2^-11 only, which times a cap of 50
+// would be 2% of a probability.
+template <int MOD>
+__device__ __forceinline__ float2 to_log2(const TcParams& p, float2 z, bool small) {
+  if constexpr (!(MOD & 1)) {
+    return fmul2(z, both(p.scale_log2));
+  } else if (small) {
+    const float2 x = fmul2(z, both(p.cap_x)), y = fmul2(x, x);
+    float2 r = ffma2(y, both(p.tanh_c[5]), both(p.tanh_c[4]));
+#pragma unroll
+    for (int i = 3; i >= 0; --i) r = ffma2(y, r, both(p.tanh_c[i]));
+    return fmul2(x, r);
+  } else {
+    z = fmul2(z, both(p.cap_in));
+    const float2 e = fadd2(make_float2(ex2_approx(z.x), ex2_approx(z.y)), both(1.0f));
+    return ffma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), both(-2.0f * p.cap_log2), both(p.cap_log2));
+  }
+}
+
 // One softmax step of a warp's 32 rows: S (128 keys, TMEM) -> P over its first 64 columns.
 // `turn` runs before the exp pass and returns false to abandon; `half` runs when keys 0..63
 // of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys.
@@ -145,12 +172,6 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
   for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x32(s_addr + (uint32_t)(g * 32), u[g]);
   tmem_wait_ld();
   if constexpr (MOD != 0) {
-    // To log2 units. tanh(x) is x p(x^2) for |x| <= 1, p of degree 5 fitted to tanh(sqrt(y)) /
-    // sqrt(y) on [0, 1] for the least maximal error (3.2e-7 in fp32): eight packed
-    // multiply-adds a pair. A warp with a larger score takes 1 - 2 / (1 + e^2x), as exact
-    // (e^2x = inf gives 1), but two more MUFU operations a score beside the exponential: that
-    // bounded the kernel (286 instead of 230 us on six documents of 333 to 2500 tokens,
-    // 32 heads). tanh.approx is exact to 2^-11 only, which times a cap of 50 would be 2% of a probability.
     bool small = true;
     if constexpr (MOD & 1) {
       float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -162,10 +183,10 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
                          fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1])));
       small = !__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
     }
-    auto modify = [&](auto curve) {
+    auto modify = [&](bool sm) {
 #pragma unroll
       for (int c = 0; c < kBK; c += 2) {
-        float2 z = curve(make_float2(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1])));
+        float2 z = to_log2<MOD>(p, make_float2(__uint_as_float(u[c >> 5][c & 31]), __uint_as_float(u[c >> 5][(c & 31) + 1])), sm);
         if constexpr (MOD & 2) {
           z.x = fmaf(nslope, fabsf(dist0 - (float)c), z.x);
           z.y = fmaf(nslope, fabsf(dist0 - (float)(c + 1)), z.y);
@@ -174,24 +195,10 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
         u[c >> 5][(c & 31) + 1] = __float_as_uint(z.y);
       }
     };
-    auto both = [](float x) { return make_float2(x, x); };
-    if constexpr (!(MOD & 1)) {
-      modify([&](float2 z) { return fmul2(z, both(p.scale_log2)); });
-    } else if (small) {
-      modify([&](float2 z) {
-        const float2 x = fmul2(z, both(p.cap_x)), y = fmul2(x, x);
-        float2 r = ffma2(y, both(p.tanh_c[5]), both(p.tanh_c[4]));
-#pragma unroll
-        for (int i = 3; i >= 0; --i) r = ffma2(y, r, both(p.tanh_c[i]));
-        return fmul2(x, r);
-      });
-    } else {
-      modify([&](float2 z) {
-        z = fmul2(z, both(p.cap_in));
-        const float2 e = fadd2(make_float2(ex2_approx(z.x), ex2_approx(z.y)), both(1.0f));
-        return ffma2(make_float2(rcp_approx(e.x), rcp_approx(e.y)), both(-2.0f * p.cap_log2), both(p.cap_log2));
-      });
-    }
+    if (small)
+      modify(true);
+    else
+      modify(false);
   }
   if (masked) {
 #pragma unroll
@@ -258,6 +265,107 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
   tc_fence_before();
   __syncwarp();
   return true;
+}
+
+// The state of one row of softmax_step_few: the four lanes of a quad hold it alike, but for
+// l, of which each has its own keys' part.
+struct FewRow {
+  float m = -INFINITY, l = 0.0f;
+  int lim = 0;
+  float pos = 0.0f, nslope = 0.0f;
+};
+
+// softmax_step for a tile of at most 16 rows, TMEM lanes 0 to 15 of the warp: a quad of lanes
+// shares a row (and, two = true, the one eight further), 32 scores a lane and row instead of
+// 128 on as many lanes as there are rows. A step of one token of four heads takes a third of the time;
+// for heads of 64 channels it is longer than the loads of its keys otherwise.
+template <int DP, class T, int MOD>
+__device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_addr, uint32_t o_addr, bool have_o, bool two,
+                                                 int kbase, FewRow (&row)[2]) {
+  const int lane = threadIdx.x & 31, j2 = 2 * (lane & 3);
+  uint32_t u[64], w[32];
+  __syncwarp();
+  tmem_ld_16x256b_x16(s_addr, u);
+  tmem_wait_ld();
+  float f[2] = {1.0f, 1.0f};
+  bool need_any = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (h && !two) break;
+    FewRow& r = row[h];
+    auto at = [&](int i, int e) -> uint32_t& { return u[4 * i + 2 * h + e]; };
+    bool small = true;
+    if constexpr (MOD & 1) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmax3(top, fabsf(__uint_as_float(at(i, 0))), fabsf(__uint_as_float(at(i, 1))));
+      small = !__any_sync(0xffffffffu, top > p.cap_small);
+    }
+    const int n_ok = r.lim - kbase - j2;
+    const float dist0 = r.pos - (float)(kbase + j2);
+    float top = -INFINITY;
+    auto modify = [&](bool sm) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float2 z = to_log2<MOD>(p, make_float2(__uint_as_float(at(i, 0)), __uint_as_float(at(i, 1))), sm);
+        if constexpr (MOD & 2) {
+          z.x = fmaf(r.nslope, fabsf(dist0 - (float)(8 * i)), z.x);
+          z.y = fmaf(r.nslope, fabsf(dist0 - (float)(8 * i + 1)), z.y);
+        }
+        z.x = 8 * i < n_ok ? z.x : -INFINITY;
+        z.y = 8 * i + 1 < n_ok ? z.y : -INFINITY;
+        top = fmax3(top, z.x, z.y);
+        at(i, 0) = __float_as_uint(z.x);
+        at(i, 1) = __float_as_uint(z.y);
+      }
+    };
+    if (small)
+      modify(true);
+    else
+      modify(false);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(r.m, top);
+    if (m_new > r.m + kRescaleThreshold) {
+      f[h] = ex2_approx(r.m - m_new);
+      r.l *= f[h];
+      r.m = m_new;
+      need_any = true;
+    }
+    const float neg_m = r.m == -INFINITY ? 0.0f : -r.m;
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e0 = ex2_approx(__uint_as_float(at(i, 0)) + neg_m), e1 = ex2_approx(__uint_as_float(at(i, 1)) + neg_m);
+      sum = fadd2(sum, make_float2(e0, e1));
+      w[2 * i + h] = Op<T>::pack(e0, e1);
+    }
+    r.l += sum.x + sum.y;
+  }
+  if (!two) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[2 * i + 1] = 0;  // rows 8 to 15 are nobody's
+  }
+  if (__any_sync(0xffffffffu, need_any) && have_o) {
+    // TMEM lane = row here: the factor of row `lane` is with quad lane % 8.
+    const float f0 = __shfl_sync(0xffffffffu, f[0], 4 * (lane & 7)), f1 = __shfl_sync(0xffffffffu, f[1], 4 * (lane & 7));
+    const float mine = lane < 8 ? f0 : lane < 16 ? f1 : 1.0f;
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 32) {
+      uint32_t o[32];
+      __syncwarp();
+      tmem_ld_32x32b_x32(o_addr + (uint32_t)c, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mine);
+      tmem_st_32x32b_x32(o_addr + (uint32_t)c, o);
+    }
+  }
+  __syncwarp();
+  tmem_st_16x128b_x16(s_addr, w);
+  tmem_wait_st();
+  tc_fence_before();
+  __syncwarp();
 }
 
 // Stores n <= 32 fp32 values times inv as bf16 / fp16.
@@ -706,16 +814,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 // the sequences before s over all key heads, first[n] the total. A sequence with queries has at
 // least one step per key head, so that rows without a key are written.
 struct StepList {
-  long long first[kMaxSeqs + 1];
+  int first[kMaxSeqs + 1];
+  int per, extra;  // steps of a worker, one more for the first `extra`
   Seq seq[kMaxSeqs];
-  int warp_sum[2][32];
+  int warp_sum[32];
+
+  __device__ __forceinline__ int begin(int worker) const { return worker * per + min(worker, extra); }
+  __device__ __forceinline__ int worker_of(int step) const {
+    const int longer = extra * (per + 1);
+    return step < longer ? step / (per + 1) : extra + (step - longer) / per;
+  }
 };
 __device__ __forceinline__ int steps_of(const Seq& q) { return max(1, (q.kl + kBK - 1) / kBK); }
 
-// All threads of the block (a multiple of 32, at most 1024); ends with a barrier.
-__device__ __forceinline__ void build_steps(const TcParams& p, StepList& L, int n) {
+// All threads of the block (a multiple of 32, at most 1024); ends with a barrier. The launcher
+// keeps the total below 2^31.
+__device__ __forceinline__ void build_steps(const TcParams& p, StepList& L, int n, int workers) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  long long base = 0;
+  int base = 0;
   for (int s0 = 0; s0 < n; s0 += blockDim.x) {
     const int s = s0 + threadIdx.x;
     Seq q = {0, 0, 0, 0};
@@ -723,23 +839,19 @@ __device__ __forceinline__ void build_steps(const TcParams& p, StepList& L, int 
       atomicOr(p.a.err, kErrBadIndex);
       q = {0, 0, 0, 0};
     }
-    long long x = q.ql > 0 ? (long long)steps_of(q) * p.a.kv_heads : 0;
-    const long long own = x;
+    int x = q.ql > 0 ? steps_of(q) * p.a.kv_heads : 0;
+    const int own = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    if (lane == 31) {
-      L.warp_sum[0][warp] = (int)(x & 0xffffffff);
-      L.warp_sum[1][warp] = (int)(x >> 32);
-    }
+    if (lane == 31) L.warp_sum[warp] = x;
     __syncthreads();
-    long long all = base;
+    int all = base;
     for (int i = 0; i < nw; ++i) {
-      const long long v = ((long long)L.warp_sum[1][i] << 32) | (unsigned)L.warp_sum[0][i];
-      if (i < warp) x += v;
-      all += v;
+      if (i < warp) x += L.warp_sum[i];
+      all += L.warp_sum[i];
     }
     if (s < n) {
       L.first[s] = base + x - own;
@@ -748,11 +860,15 @@ __device__ __forceinline__ void build_steps(const TcParams& p, StepList& L, int 
     base = all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) L.first[n] = base;
+  if (threadIdx.x == 0) {
+    L.first[n] = base;
+    L.per = base / workers;
+    L.extra = base % workers;
+  }
   __syncthreads();
 }
 // The sequence that step belongs to: the last one with first[s] <= step.
-__device__ __forceinline__ int find_step(const StepList& L, int n, long long step) {
+__device__ __forceinline__ int find_step(const StepList& L, int n, int step) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -763,25 +879,21 @@ __device__ __forceinline__ int find_step(const StepList& L, int n, long long ste
   }
   return lo;
 }
-__device__ __forceinline__ long long part_begin(long long total, int workers, int w) { return total * w / workers; }
 
 // A worker's pieces in order: key tiles [kt0, kt1) of key head kvh of sequence s.
 struct Pieces {
   const StepList& L;
-  int n;
-  long long at, end;
+  int n, at, end;
   int s, kvh, kt0, kt1;
   bool whole;
-  __device__ Pieces(const StepList& L_, int n_, int w, int workers)
-      : L(L_), n(n_), at(part_begin(L_.first[n_], workers, w)), end(part_begin(L_.first[n_], workers, w + 1)) {}
+  __device__ Pieces(const StepList& L_, int n_, int w) : L(L_), n(n_), at(L_.begin(w)), end(L_.begin(w + 1)) {}
   __device__ bool next() {
     if (at >= end) return false;
     s = find_step(L, n, at);
-    const int e = steps_of(L.seq[s]);
-    const long long rem = at - L.first[s];
-    kvh = (int)(rem / e);
-    kt0 = (int)(rem - (long long)kvh * e);
-    kt1 = (int)min((long long)e, kt0 + (end - at));
+    const int e = steps_of(L.seq[s]), rem = at - L.first[s];
+    kvh = rem / e;
+    kt0 = rem - kvh * e;
+    kt1 = min(e, kt0 + (end - at));
     whole = kt0 == 0 && kt1 == e;
     at += kt1 - kt0;
     return true;
@@ -789,7 +901,7 @@ struct Pieces {
   __device__ int tiles() const { return L.seq[s].kl > 0 ? kt1 - kt0 : 0; }  // to load
 };
 
-template <int DP, class T, int MOD>
+template <int DP, class T, int MOD, bool FEW>
 __global__ void __launch_bounds__(kThreads, 1)
     k_ragged_streams(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcParams p) {
@@ -812,13 +924,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Worker of this warp: producers are warps 0 and 3, issuers 1 and 2, softmax 4-7 and 8-11.
   const int t = warp < 4 ? (warp >= 2 ? 1 : 0) : (warp - 4) >> 2;
+  // With few rows worker 1 has them in TMEM lanes 32 on (its MMA reads 32 rows of what lies
+  // before them), so that the two workers' softmax warps run on different schedulers.
+  const int lane0 = FEW ? 32 * t : 0;
+  smem += FEW ? kFewPad : 0;
   uint8_t* sQ = smem + t * ATOMS * p.q_atom;
   uint8_t* sR = smem + 2 * ATOMS * p.q_atom + t * SL * KV_BYTES;
   uint64_t* b = bars[t];
   uint64_t *q_full = b, *q_empty = b + 1, *s_full = b + 2, *p_half = b + 3, *p_full = b + 4, *o_full = b + 5,
            *drain = b + 6, *r_full = b + 8, *r_empty = b + 8 + kMaxSlots;
   const int worker = t * gridDim.x + blockIdx.x, workers = 2 * gridDim.x;
-  const int n = min(p.a.n_seq - p.seq0, kMaxSeqs);
+  const int n = min(p.a.n_seq - p.seq0, p.seqs);
 
   if (threadIdx.x < 2) {
     uint64_t* z = bars[threadIdx.x];
@@ -846,11 +962,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmV);
   }
   tc_fence_before();
-  build_steps(p, steps, n);
+  build_steps(p, steps, n, workers);
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   int* err = p.a.err;
-  Pieces it(steps, n, worker, workers);
+  Pieces it(steps, n, worker);
   // The next launch (k_ragged_join) may be set up now; it waits for this grid's end.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp < 4) {
@@ -896,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else {
       // ------------------------------ MMA issuer --------------------------------
-      const uint64_t qd = sdesc_k_sw128(smem_u32(sQ)), kd0 = sdesc_k_sw128(smem_u32(sR));
+      const uint64_t qd = sdesc_k_sw128(smem_u32(sQ) - (uint32_t)(lane0 * 128)), kd0 = sdesc_k_sw128(smem_u32(sR));
       const uint64_t vd0 = sdesc_mn_sw128(smem_u32(sR), ATOM, 1024);
       const uint64_t q_jump = (uint64_t)(p.q_atom >> 4);  // a Q atom may be shorter than 128 rows
       const uint32_t d_s = tmem + (uint32_t)(t * kBK), d_o = tmem + kOCol + (uint32_t)(t * DP);
@@ -964,7 +1080,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------ softmax / epilogue ------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    const int qq = warp & 3, r = qq * 32 + lane;
+    const int qq = warp & 3, r = qq * 32 + lane - lane0;
     const uint32_t lane_base = tmem + ((uint32_t)(qq * 32) << 16);
     const uint32_t s_addr = lane_base + (uint32_t)(t * kBK);
     const uint32_t o_addr = lane_base + kOCol + (uint32_t)(t * DP);
@@ -972,11 +1088,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && it.next()) {
       const Seq q = steps.seq[it.s];
-      const int nt = it.tiles();
-      const Row w = make_row(p, q, p.seq0 + it.s, it.kvh, 0, r);
-      const bool busy = qq * 32 < p.G * q.ql;  // the warp has rows (uniform)
+      const int nt = it.tiles(), rows = p.G * q.ql;
+      const bool busy = qq * 32 >= lane0 && qq * 32 - lane0 < rows;  // the warp has rows (uniform)
+      const Row w = make_row(p, q, p.seq0 + it.s, it.kvh, 0, max(r, 0));
       const int lim0 = p.a.causal ? min(q.kl, max(q.kl - q.ql + 1, p.a.prefix ? p.a.prefix[p.seq0 + it.s] : 0)) : q.kl;
       float m = -INFINITY, l = 0.0f;
+      FewRow few[2];
+      if (FEW && busy) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Row x = make_row(p, q, p.seq0 + it.s, it.kvh, 0, (lane >> 2) + 8 * h);
+          few[h].lim = x.lim;
+          few[h].pos = x.pos;
+          few[h].nslope = x.nslope;
+        }
+      }
       for (int j = 0; j < nt; ++j, ++step) {
         if (!mbar_wait(s_full, step & 1, abort_flag, err, kErrAttnWait)) {
           ok = false;
@@ -984,7 +1110,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const int kbase = (it.kt0 + j) * kBK;
-        if (busy) {
+        if (!busy) {
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_half);
+            mbar_arrive(p_full);
+          }
+        } else if constexpr (FEW) {
+          softmax_step_few<DP, T, MOD>(p, s_addr, o_addr, j > 0, rows > 8, kbase, few);
+          if (lane == 0) {
+            mbar_arrive(p_half);
+            mbar_arrive(p_full);
+          }
+        } else {
           softmax_step<DP, T, MOD>(
               p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.pos - (float)kbase, w.nslope, m, l,
               []() { return true; },
@@ -992,11 +1130,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(p_half);
               });
           if (lane == 0) mbar_arrive(p_full);
-        } else {
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(p_half);
-            mbar_arrive(p_full);
+        }
+      }
+      if (FEW) {
+        // To one row per lane.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          few[h].l += __shfl_xor_sync(0xffffffffu, few[h].l, 1);
+          few[h].l += __shfl_xor_sync(0xffffffffu, few[h].l, 2);
+          const float mh = __shfl_sync(0xffffffffu, few[h].m, 4 * (lane & 7));
+          const float lh = __shfl_sync(0xffffffffu, few[h].l, 4 * (lane & 7));
+          if (lane >> 3 == h) {
+            m = mh;
+            l = lh;
           }
         }
       }
@@ -1029,48 +1175,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <class T>
 __global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcParams p, int workers) {
   __shared__ StepList steps;
-  const int lane = threadIdx.x & 31, n = min(p.a.n_seq - p.seq0, kMaxSeqs);
-  build_steps(p, steps, n);
+  const int lane = threadIdx.x & 31, n = min(p.a.n_seq - p.seq0, p.seqs);
+  build_steps(p, steps, n, workers);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long total = steps.first[n];
   const long long rows = (long long)n * p.a.max_q * p.a.heads;
   const int pitch = p.a.d + 2;
   for (long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); x < rows; x += (long long)gridDim.x * 8) {
     const int h = (int)(x % p.a.heads);
-    const long long y = x / p.a.heads;
+    const int y = (int)(x / p.a.heads);
     const int tok = (int)(y % p.a.max_q), s = (int)(y / p.a.max_q);
     const Seq q = steps.seq[s];
     if (tok >= q.ql) continue;
     const int kvh = h / p.G, r = tok * p.G + (h - kvh * p.G), e = steps_of(q);
-    const long long a = steps.first[s] + (long long)kvh * e;
-    int w = (int)(a * workers / total);  // the worker that holds step a
-    while (w > 0 && part_begin(total, workers, w) > a) --w;
-    while (part_begin(total, workers, w + 1) <= a) ++w;
-    if (part_begin(total, workers, w + 1) >= a + e) continue;  // whole
-    const int w0 = w;
+    const int a = steps.first[s] + kvh * e, w0 = steps.worker_of(a), w1 = steps.worker_of(a + e - 1);
+    if (w0 == w1) continue;  // whole
+    // The first worker's piece is its last one (slot 1), the others' their first (slot 0).
+    auto piece = [&](int w) { return p.part + ((int64_t)(2 * w + (w == w0 ? 1 : 0)) * p.part_rows + r) * pitch; };
     float top = -INFINITY;
-    for (; w < workers && part_begin(total, workers, w) < a + e; ++w) {
-      if (part_begin(total, workers, w + 1) == part_begin(total, workers, w)) continue;  // no steps
-      const float* piece = p.part + ((int64_t)(2 * w + (w == w0 ? 1 : 0)) * p.part_rows + r) * pitch;
-      top = fmaxf(top, piece[p.a.d]);
-    }
+    for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, piece(w)[p.a.d]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == -INFINITY) top = 0.0f;
     float l = 0.0f;
     float2 o[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    const int w1 = w;
-    for (w = w0; w < w1; ++w) {
-      if (part_begin(total, workers, w + 1) == part_begin(total, workers, w)) continue;
-      const float* piece = p.part + ((int64_t)(2 * w + (w == w0 ? 1 : 0)) * p.part_rows + r) * pitch;
-      const float2 ml = *reinterpret_cast<const float2*>(piece + p.a.d);
-      const float f = ex2_approx(ml.x - top);
-      l = fmaf(f, ml.y, l);
+    for (int b = w0; b <= w1; b += 32) {
+      float f = 0.0f;
+      if (b + lane <= w1) {
+        const float2 ml = *reinterpret_cast<const float2*>(piece(b + lane) + p.a.d);
+        f = ex2_approx(ml.x - top);
+        l = fmaf(f, ml.y, l);
+      }
+      const int cnt = min(32, w1 - b + 1);
+#pragma unroll 4
+      for (int i = 0; i < cnt; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        const float* src = piece(b + i) + 2 * lane;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (2 * lane + 64 * c < p.a.d) {
-          const float2 v = *reinterpret_cast<const float2*>(piece + 2 * lane + 64 * c);
-          o[c] = ffma2(make_float2(f, f), v, o[c]);
-        }
+        for (int c = 0; c < 2; ++c)
+          if (2 * lane + 64 * c < p.a.d) o[c] = ffma2(both(fi), *reinterpret_cast<const float2*>(src + 64 * c), o[c]);
+      }
     }
+    l = warp_add(l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = reinterpret_cast<T*>(p.a.out) + ((int64_t)q.q0 + tok) * p.a.ldo + (int64_t)h * p.a.d;
 #pragma unroll
@@ -1098,32 +1243,24 @@ void prepare_kernel(K kern, int smem, bool (&done)[64]) {
   done[dev] = true;
 }
 
-template <int DP, class T, int MOD>
-void launch_mod(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool streams) {
+template <int DP, class T, int MOD, bool FEW>
+void launch_streams(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv) {
   DeviceContext& c = ctx();
-  if (!streams) {
-    static bool done[64] = {};
-    prepare_kernel(k_ragged_tiles<DP, T, MOD>, TilesCfg<DP>::SMEM, done);
-    // Pairs of tiles: at most one per sequence more than the rows make.
-    const int64_t pairs = std::min<int64_t>((int64_t)p.a.n_seq * ((p.a.max_q + 2 * p.tpt - 1) / (2 * p.tpt)),
-                                            p.a.Tq / (2 * p.tpt) + p.a.n_seq);
-    const int64_t grid = pairs * p.a.kv_heads;
-    if (grid >= ((int64_t)1 << 31)) fail(kErrInvalidArg, "attention_ragged: too many query tiles");
-    k_ragged_tiles<DP, T, MOD><<<(unsigned)grid, kThreads, TilesCfg<DP>::SMEM, c.stream>>>(tq, tk, tv, p);
-    check_launch("attention_ragged_tiles");
-    return;
-  }
   constexpr int kKv = DP / 64 * kBK * 128;
-  const int room = kMaxSmem - (int)sizeof(StepList) - 1024 - 1024 - 2 * (DP / 64) * p.q_atom;
-  p.slots = std::min(8, room / (2 * kKv));
-  const int smem = 1024 + 2 * (DP / 64) * p.q_atom + 2 * p.slots * kKv;
+  const int fixed = 1024 + (FEW ? kFewPad : 0) + 2 * (DP / 64) * p.q_atom;
+  p.slots = std::min(8, (kMaxSmem - (int)sizeof(StepList) - 1024 - fixed) / (2 * kKv));
+  const int smem = fixed + 2 * p.slots * kKv;
   static bool done[64] = {};
-  prepare_kernel(k_ragged_streams<DP, T, MOD>, kMaxSmem - (int)sizeof(StepList) - 1024, done);
-  for (p.seq0 = 0; p.seq0 < p.a.n_seq; p.seq0 += kMaxSeqs) {
-    k_ragged_streams<DP, T, MOD><<<(unsigned)c.num_sms, kThreads, smem, c.stream>>>(tq, tk, tv, p);
+  prepare_kernel(k_ragged_streams<DP, T, MOD, FEW>, kMaxSmem - (int)sizeof(StepList) - 1024, done);
+  // Sequences of one launch: as many as its step list holds, below 2^31 steps.
+  const int64_t most = ((p.a.max_kv + kBK - 1) / kBK) * p.a.kv_heads + p.a.kv_heads;
+  if (most >= ((int64_t)1 << 31)) fail(kErrInvalidArg, "attention_ragged: too many keys");
+  p.seqs = (int)std::min<int64_t>(kMaxSeqs, (((int64_t)1 << 31) - 1) / most);
+  for (p.seq0 = 0; p.seq0 < p.a.n_seq; p.seq0 += p.seqs) {
+    k_ragged_streams<DP, T, MOD, FEW><<<(unsigned)c.num_sms, kThreads, smem, c.stream>>>(tq, tk, tv, p);
     check_launch("attention_ragged_streams");
     if (p.a.max_kv <= kBK) continue;  // every piece is a whole row
-    const int64_t rows = (int64_t)std::min(p.a.n_seq - p.seq0, kMaxSeqs) * p.a.max_q * p.a.heads;
+    const int64_t rows = (int64_t)std::min(p.a.n_seq - p.seq0, p.seqs) * p.a.max_q * p.a.heads;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)c.num_sms * 4));
     cfg.blockDim = dim3(256);
@@ -1140,6 +1277,25 @@ void launch_mod(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const
       check_cuda(cudaLaunchKernelEx(&cfg, k_ragged_join<__half>, (const TcParams)p, workers), "attention_ragged_join");
     check_launch("attention_ragged_join");
   }
+}
+
+template <int DP, class T, int MOD>
+void launch_mod(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, bool streams) {
+  DeviceContext& c = ctx();
+  if (!streams) {
+    static bool done[64] = {};
+    prepare_kernel(k_ragged_tiles<DP, T, MOD>, TilesCfg<DP>::SMEM, done);
+    // Pairs of tiles: at most one per sequence more than the rows make.
+    const int64_t pairs = std::min<int64_t>((int64_t)p.a.n_seq * ((p.a.max_q + 2 * p.tpt - 1) / (2 * p.tpt)),
+                                            p.a.Tq / (2 * p.tpt) + p.a.n_seq);
+    const int64_t grid = pairs * p.a.kv_heads;
+    if (grid >= ((int64_t)1 << 31)) fail(kErrInvalidArg, "attention_ragged: too many query tiles");
+    k_ragged_tiles<DP, T, MOD><<<(unsigned)grid, kThreads, TilesCfg<DP>::SMEM, c.stream>>>(tq, tk, tv, p);
+    check_launch("attention_ragged_tiles");
+    return;
+  }
+  if (p.G * p.tpt <= kFewRows) return launch_streams<DP, T, MOD, true>(p, tq, tk, tv);
+  launch_streams<DP, T, MOD, false>(p, tq, tk, tv);
 }
 
 template <int DP, class T>
