@@ -252,9 +252,14 @@ def _refuse_args(op, like, **tensors):
             raise ValueError(f"{op}: {name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _fits(t, dtype, dev, shape):
-    """A None tensor, or one of that type, device and contiguous shape."""
-    return t is None or (t.dtype is dtype and t.get_device() == dev and t.shape == shape and t.is_contiguous())
+_lora_bytes, _attention_bytes = {}, {}  # workspace sizes by argument sizes
+
+
+def _remember(sizes, key, need):
+    if need >= 0:  # -1: the operator itself says what is wrong
+        if len(sizes) >= 4096:
+            sizes.clear()
+        sizes[key] = need
 
 
 def _head_pitch(op, name, t):
@@ -300,8 +305,12 @@ def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleav
     table = cos.shape
     if len(table) != 2:
         raise ValueError(f"{op}: cos must be [n_pos, rot]")
-    if not (0 <= dev == _current() and _fits(cos, _F32, dev, table) and _fits(sin, _F32, dev, table)
-            and _fits(gq, _F32, dev, (d,)) and _fits(gk, _F32, dev, (d,)) and _fits(pos, _I32, dev, (T,))
+    if not (0 <= dev == _current() and cos.dtype is _F32 and cos.get_device() == dev and cos.is_contiguous()
+            and sin.dtype is _F32 and sin.get_device() == dev and sin.shape == table and sin.is_contiguous()
+            and (gq is None or (gq.dtype is _F32 and gq.get_device() == dev and gq.shape == (d,) and gq.is_contiguous()))
+            and (gk is None or (gk.dtype is _F32 and gk.get_device() == dev and gk.shape == (d,) and gk.is_contiguous()))
+            and (pos is None or (pos.dtype is _I32 and pos.get_device() == dev and pos.shape == (T,)
+                                 and pos.is_contiguous()))
             and (k is None or (k.dtype is dtype and k.get_device() == dev))
             and (q_out is None or (q_out.dtype is out_dtype and q_out.get_device() == dev))
             and (k_out is None or (k_out.dtype is out_dtype and k_out.get_device() == dev))):
@@ -330,10 +339,13 @@ def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleav
             ldko = _head_pitch(op, "k_out", k_out)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     L = lib()
-    check(L.sdb200_set_stream(_raw_stream(dev)))
-    check(L.sdb200_qk_norm_rope(T, q.data_ptr(), _head_pitch(op, "q", q), heads, kp, ldk, kv, _TYPES[dtype], d, table[1],
-                                _p(gq), _p(gk), eps, cos.data_ptr(), sin.data_ptr(), table[0], _p(pos),
-                                1 if interleaved else 0, q_out.data_ptr(), ldqo, kop, ldko, _TYPES[out_dtype]))
+    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_qk_norm_rope(
+        T, q.data_ptr(), _head_pitch(op, "q", q), heads, kp, ldk, kv, _TYPES[dtype], d, table[1],
+        None if gq is None else gq.data_ptr(), None if gk is None else gk.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(),
+        table[0], None if pos is None else pos.data_ptr(), 1 if interleaved else 0, q_out.data_ptr(), ldqo, kop, ldko,
+        _TYPES[out_dtype])
+    if rc:
+        check(rc)
     return q_out, k_out
 
 
@@ -354,8 +366,12 @@ def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32
     if out_dtype not in (_F32, _BF16):
         raise TypeError(f"{op}: output type {out_dtype}")
     if not (0 <= dev == _current() and W.dtype is _BF16 and A.dtype is _BF16 and B.dtype is _BF16 and W.get_device() == dev
-            and A.get_device() == dev and B.get_device() == dev and _fits(rows, _I32, dev, (T,))
-            and _fits(scale, _F32, dev, (n,)) and _fits(bias, _F32, dev, (N,))
+            and A.get_device() == dev and B.get_device() == dev and rows.dtype is _I32 and rows.get_device() == dev
+            and rows.shape == (T,) and rows.is_contiguous()
+            and (scale is None or (scale.dtype is _F32 and scale.get_device() == dev and scale.shape == (n,)
+                                   and scale.is_contiguous()))
+            and (bias is None or (bias.dtype is _F32 and bias.get_device() == dev and bias.shape == (N,)
+                                  and bias.is_contiguous()))
             and (out is None or out.get_device() == dev)):
         _refuse_args(op, x, W=(W, _BF16, None), A=(A, _BF16, None), B=(B, _BF16, None), rows=(rows, _I32, (T,)),
                      scale=(scale, _F32, (n,)), bias=(bias, _F32, (N,)), out=(out, out_dtype, None))
@@ -365,15 +381,23 @@ def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32
         if out.shape != (T, N):
             raise ValueError(f"{op}: out must be [{T}, {N}]")
         ldy = _row_pitch(op, "out", out)
-    operands = (T, N, K, x.data_ptr(), _row_pitch(op, "x", x), 1 if dtype is _BF16 else 0, W.data_ptr(),
-                _row_pitch(op, "W", W))
-    adapters = (n, r, A.data_ptr(), _stack_pitch(op, "A", A), B.data_ptr(), _stack_pitch(op, "B", B))
+    px, pw, pa, pb = x.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
+    ldx, ldw, lda, ldb = _row_pitch(op, "x", x), _row_pitch(op, "W", W), _stack_pitch(op, "A", A), _stack_pitch(op, "B", B)
+    bf = 1 if dtype is _BF16 else 0
     L = lib()
-    need = L.sdb200_linear_lora_workspace(*operands, *adapters)
+    # The workspace follows from sizes, pitches and alignment alone.
+    key = (T, N, K, n, r, ldx, ldw, lda, ldb, bf, px & 15, pw & 15, pa & 15, pb & 15, dev)
+    need = _lora_bytes.get(key)
+    if need is None:
+        need = L.sdb200_linear_lora_workspace(T, N, K, px, ldx, bf, pw, ldw, n, r, pa, lda, pb, ldb)
+        _remember(_lora_bytes, key, need)
     ws = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    check(L.sdb200_set_stream(_raw_stream(dev)))
-    check(L.sdb200_linear_lora(*operands, _p(bias), rows.data_ptr(), *adapters, _p(scale), out.data_ptr(), ldy,
-                               1 if out_dtype is _BF16 else 0, _p(ws), need))
+    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_linear_lora(
+        T, N, K, px, ldx, bf, pw, ldw, None if bias is None else bias.data_ptr(), rows.data_ptr(), n, r, pa, lda, pb, ldb,
+        None if scale is None else scale.data_ptr(), out.data_ptr(), ldy, 1 if out_dtype is _BF16 else 0,
+        None if ws is None else ws.data_ptr(), need)
+    if rc:
+        check(rc)
     return out
 
 
@@ -399,9 +423,16 @@ def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, s
     n = q_begin.numel()
     one = (n,)
     if not (0 <= dev == _current() and k.dtype is dtype and v.dtype is dtype and k.get_device() == dev
-            and v.get_device() == dev and _fits(q_begin, _I32, dev, one) and _fits(q_len, _I32, dev, one)
-            and _fits(kv_begin, _I32, dev, one) and _fits(kv_len, _I32, dev, one) and _fits(prefix, _I32, dev, one)
-            and _fits(slopes, _F32, dev, (heads,)) and (out is None or out.get_device() == dev)):
+            and v.get_device() == dev
+            and q_begin.dtype is _I32 and q_begin.get_device() == dev and q_begin.shape == one and q_begin.is_contiguous()
+            and q_len.dtype is _I32 and q_len.get_device() == dev and q_len.shape == one and q_len.is_contiguous()
+            and kv_begin.dtype is _I32 and kv_begin.get_device() == dev and kv_begin.shape == one
+            and kv_begin.is_contiguous()
+            and kv_len.dtype is _I32 and kv_len.get_device() == dev and kv_len.shape == one and kv_len.is_contiguous()
+            and (prefix is None or (prefix.dtype is _I32 and prefix.get_device() == dev and prefix.shape == one
+                                    and prefix.is_contiguous()))
+            and (slopes is None or (slopes.dtype is _F32 and slopes.get_device() == dev and slopes.shape == (heads,)
+                                    and slopes.is_contiguous())) and (out is None or out.get_device() == dev)):
         _refuse_args(op, q, k=(k, dtype, None), v=(v, dtype, None), q_begin=(q_begin, _I32, one), q_len=(q_len, _I32, one),
                      kv_begin=(kv_begin, _I32, one), kv_len=(kv_len, _I32, one), prefix=(prefix, _I32, one),
                      slopes=(slopes, _F32, (heads,)), out=(out, out_dtype, None))
@@ -413,15 +444,20 @@ def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, s
         ldo = _head_pitch(op, "out", out)
     L = lib()
     max_q, max_kv = min(max_q, Tq), min(max_kv, Tkv)
-    need = L.sdb200_attention_ragged_workspace(n, max_q, max_kv, heads, kv_heads, d)
+    key = (n, max_q, max_kv, heads, kv_heads, d, dev)
+    need = _attention_bytes.get(key)
+    if need is None:
+        need = L.sdb200_attention_ragged_workspace(n, max_q, max_kv, heads, kv_heads, d)
+        _remember(_attention_bytes, key, need)
     ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    check(L.sdb200_set_stream(_raw_stream(dev)))
-    check(L.sdb200_attention_ragged(q.data_ptr(), _head_pitch(op, "q", q), k.data_ptr(), _head_pitch(op, "k", k),
-                                    v.data_ptr(), _head_pitch(op, "v", v), _TYPES[dtype], out.data_ptr(), ldo,
-                                    _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(), q_len.data_ptr(),
-                                    kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads, kv_heads, d,
-                                    d ** -0.5 if scale is None else scale, cap, _p(slopes), 1 if causal else 0,
-                                    _p(prefix), _p(ws), need))
+    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_attention_ragged(
+        q.data_ptr(), _head_pitch(op, "q", q), k.data_ptr(), _head_pitch(op, "k", k), v.data_ptr(),
+        _head_pitch(op, "v", v), _TYPES[dtype], out.data_ptr(), ldo, _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(),
+        q_len.data_ptr(), kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads, kv_heads, d,
+        d ** -0.5 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(), 1 if causal else 0,
+        None if prefix is None else prefix.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    if rc:
+        check(rc)
     return out
 
 

@@ -421,6 +421,37 @@ def test_attention_ragged_peaked_scores(sdb, lens):
     run_attn(sdb, *lens, 4, 2, 64, BF16, causal=True, spread=60.0, cap=40.0)
 
 
+@pytest.mark.parametrize("lens", [[300, 40, 129, 1], [260, 257, 3], [1, 130, 77]])
+@pytest.mark.parametrize("H,Hk,d", [(4, 1, 128), (6, 6, 64)])
+def test_attention_ragged_of_a_padded_batch(sdb, lens, H, Hk, d):
+    """[N, S] rows with lengths of their own: the padding is not read and not written."""
+    g = gen(sum(lens))
+    N, S = len(lens), max(lens)
+    q, k, v = (randn(g, N * S, h, d, dtype=BF16) for h in (H, Hk, Hk))
+    for i, n in enumerate(lens):
+        for x in (q, k, v):
+            x[i * S + n:(i + 1) * S] = float("nan")
+    b = torch.arange(N, device="cuda", dtype=torch.int32) * S
+    n = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 5.0)
+    sdb.backend.attention_ragged(q, k, v, b, n, b, n, S, S, causal=True, out=out)
+    sdb.backend.synchronize()
+    want, slack, live = attn_want(q, k, v, [(i * S, m, i * S, m) for i, m in enumerate(lens)], d ** -0.5, True, None, 0.0,
+                                  None, BF16)
+    close(out[live], want[live], slack[live])
+    assert (out[~live] == 5.0).all()
+
+
+@pytest.mark.parametrize("n", [700, 1030])
+def test_attention_ragged_of_many_sequences(sdb, n):
+    """More sequences than one step list holds, some of several tiles, some of none."""
+    g = gen(n)
+    ql = [(i * 7) % 5 + (200 if i % 300 == 3 else 0) for i in range(n)]
+    kl = [q + (i * 13) % 140 for i, q in enumerate(ql)]
+    run_attn(sdb, ql, kl, 4, 2, 64, F16, causal=True, seed=n)
+    run_attn(sdb, [1] * n, [1 + (i * 31) % 300 for i in range(n)], 4, 1, 128, BF16, causal=True, seed=n)
+
+
 def test_attention_ragged_loose_maxima(sdb):
     run_attn(sdb, [5, 60], [90, 60], 4, 2, 128, F16, causal=True, max_q=4000, max_kv=100000)
     run_attn(sdb, [1, 1], [90, 600], 4, 2, 128, BF16, causal=True, max_q=1, max_kv=1 << 40)
