@@ -116,6 +116,14 @@ def test_qk_norm_rope(sdb, case):
         close(got, want, (d + 16) * 2.0 ** -24 * mag)
 
 
+@pytest.mark.parametrize("ti,to", [(F32, F32), (BF16, BF16), (F16, BF16), (F32, F16)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rot", [(40, 20), (4, 4), (124, 60), (100, 0)])
+def test_qk_norm_rope_of_pairs_of_channels(sdb, ti, to, inter, d, rot):
+    """Heads and rotated parts that only chunks of two channels divide."""
+    test_qk_norm_rope(sdb, (61, 5, 3, d, rot, ti, to, inter, False, True, True))
+
+
 def test_qk_norm_rope_in_place_of_a_fused_buffer(sdb):
     g = gen(5)
     y = randn(g, 41, 10 * 128, dtype=BF16)
