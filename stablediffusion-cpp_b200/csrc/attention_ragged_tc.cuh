@@ -1169,18 +1169,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The pieces of the rows that k_ragged_streams cut, joined: one warp per row (sequence,
-// token, head). Which workers hold them follows from the step list alone; rows that one
-// worker finished are already in out.
-template <class T>
+// The pieces of the rows that k_ragged_streams cut, joined: W warps per row (sequence, token,
+// head), each for every W-th piece. Which workers hold them follows from the step list alone;
+// rows that one worker finished are already in out. A warp waits about 0.25 us for a piece (four
+// loads in flight), so one row of 100 pieces takes 26 us with one warp; with eight to a row, a
+// launch of many rows would leave most of them idle.
+template <class T, int W>
 __global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcParams p, int workers) {
   __shared__ StepList steps;
-  const int lane = threadIdx.x & 31, n = min(p.a.n_seq - p.seq0, p.seqs);
+  __shared__ float4 sum[W > 1 ? W : 1][32];
+  __shared__ float sum_l[W];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = min(p.a.n_seq - p.seq0, p.seqs);
   build_steps(p, steps, n, workers);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long rows = (long long)n * p.a.max_q * p.a.heads;
-  const int pitch = p.a.d + 2;
-  for (long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); x < rows; x += (long long)gridDim.x * 8) {
+  const int pitch = p.a.d + 2, part = warp % W;
+  for (long long x = (long long)blockIdx.x * (8 / W) + warp / W; x < rows; x += (long long)gridDim.x * (8 / W)) {
     const int h = (int)(x % p.a.heads);
     const int y = (int)(x / p.a.heads);
     const int tok = (int)(y % p.a.max_q), s = (int)(y / p.a.max_q);
@@ -1198,24 +1202,43 @@ __global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcP
     if (top == -INFINITY) top = 0.0f;
     float l = 0.0f;
     float2 o[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-    for (int b = w0; b <= w1; b += 32) {
+    for (int b = w0 + part; b <= w1; b += 32 * W) {
       float f = 0.0f;
-      if (b + lane <= w1) {
-        const float2 ml = *reinterpret_cast<const float2*>(piece(b + lane) + p.a.d);
+      if (b + W * lane <= w1) {
+        const float2 ml = *reinterpret_cast<const float2*>(piece(b + W * lane) + p.a.d);
         f = ex2_approx(ml.x - top);
         l = fmaf(f, ml.y, l);
       }
-      const int cnt = min(32, w1 - b + 1);
+      const int cnt = min(32, (w1 - b) / W + 1);
 #pragma unroll 4
       for (int i = 0; i < cnt; ++i) {
         const float fi = __shfl_sync(0xffffffffu, f, i);
-        const float* src = piece(b + i) + 2 * lane;
+        const float* src = piece(b + W * i) + 2 * lane;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
           if (2 * lane + 64 * c < p.a.d) o[c] = ffma2(both(fi), *reinterpret_cast<const float2*>(src + 64 * c), o[c]);
       }
     }
     l = warp_add(l);
+    if constexpr (W > 1) {  // x is the same for the whole block then
+      static_assert(W == 8, "a block is one row or eight");
+      sum[part][lane] = make_float4(o[0].x, o[0].y, o[1].x, o[1].y);
+      if (lane == 0) sum_l[part] = l;
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int i = 1; i < W; ++i) {
+          const float4 v = sum[i][lane];
+          o[0].x += v.x;
+          o[0].y += v.y;
+          o[1].x += v.z;
+          o[1].y += v.w;
+          l += sum_l[i];
+        }
+      }
+      __syncthreads();
+      if (warp > 0) continue;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     T* out = reinterpret_cast<T*>(p.a.out) + ((int64_t)q.q0 + tok) * p.a.ldo + (int64_t)h * p.a.d;
 #pragma unroll
@@ -1225,6 +1248,26 @@ __global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcP
         out[2 * lane + 64 * c + 1] = from_f32<T>(o[c].y * inv);
       }
   }
+}
+
+template <class T>
+void launch_join(const TcParams& p) {
+  DeviceContext& c = ctx();
+  const int64_t rows = (int64_t)std::min(p.a.n_seq - p.seq0, p.seqs) * p.a.max_q * p.a.heads;
+  const int64_t most = (int64_t)c.num_sms * 4;
+  const bool wide = rows <= most;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>(wide ? rows : (rows + 7) / 8, most));
+  cfg.blockDim = dim3(256);
+  cfg.stream = c.stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, wide ? k_ragged_join<T, 8> : k_ragged_join<T, 1>, p, 2 * c.num_sms),
+             "attention_ragged_join");
+  check_launch("attention_ragged_join");
 }
 
 template <class K>
@@ -1260,22 +1303,7 @@ void launch_streams(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, c
     k_ragged_streams<DP, T, MOD, FEW><<<(unsigned)c.num_sms, kThreads, smem, c.stream>>>(tq, tk, tv, p);
     check_launch("attention_ragged_streams");
     if (p.a.max_kv <= kBK) continue;  // every piece is a whole row
-    const int64_t rows = (int64_t)std::min(p.a.n_seq - p.seq0, p.seqs) * p.a.max_q * p.a.heads;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>((rows + 7) / 8, (int64_t)c.num_sms * 4));
-    cfg.blockDim = dim3(256);
-    cfg.stream = c.stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const int workers = 2 * c.num_sms;
-    if (p.a.out_type == kBF16)
-      check_cuda(cudaLaunchKernelEx(&cfg, k_ragged_join<__nv_bfloat16>, (const TcParams)p, workers), "attention_ragged_join");
-    else
-      check_cuda(cudaLaunchKernelEx(&cfg, k_ragged_join<__half>, (const TcParams)p, workers), "attention_ragged_join");
-    check_launch("attention_ragged_join");
+    p.a.out_type == kBF16 ? launch_join<__nv_bfloat16>(p) : launch_join<__half>(p);
   }
 }
 
