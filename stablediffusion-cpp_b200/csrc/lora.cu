@@ -2,8 +2,8 @@
 //   y[t, n] = sum_k x[t, k] W[n, k] + bias[n] + sum_j h[t, j] B_a[n, j],
 //   h[t, j] = s_a sum_k x[t, k] A_a[j, k],   a = row_adapter[t] (no second term for a < 0).
 //
-// Up to 128 rows the work is reading W and the adapters once (k_lora_down_rows, k_lora_rows);
-// above, it is a GEMM (k_lora_lists, k_lora_gemm).
+// With few rows the work is reading W and the adapters once (k_lora_down_rows, k_lora_rows);
+// with many it is a GEMM (k_lora_lists, k_lora_gemm).
 #include <algorithm>
 #include <cmath>
 
@@ -19,7 +19,7 @@ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int kMaxRowsSmall = 128;
+constexpr int kMaxRowsSmall = 128;  // rows of a block of k_lora_rows
 
 // The adapter term rides on the same tensor-core product as W: next to the K blocks of X and
 // W, an accumulator runs through the chunks of H and B, where H holds h in the columns of the
@@ -56,7 +56,8 @@ inline CUtensorMapSwizzle swizzle_of(int cw) {
 // ------------------------------------------------------------------------------------
 // Few rows
 // ------------------------------------------------------------------------------------
-// H: [f][part][rc][TN][cw] bf16 for every row f that is the first of its adapter.
+// Rows go in blocks of 128. H: [f][part][rc][TN][cw] bf16 for every row f that is the first
+// of its adapter in its block.
 struct RowsK {
   uint16_t* H;
   int cw, rc, parts;
@@ -79,10 +80,11 @@ __global__ void __launch_bounds__(256) k_lora_down_rows(const LoraLinear p, cons
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int ids[kMaxRowsSmall];
   __shared__ float sh[8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x, T = (int)p.T;
-  const int j = blockIdx.y * 8 + warp;
+  const int64_t row0 = blockIdx.x / kMaxRowsSmall * kMaxRowsSmall;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = blockIdx.x % kMaxRowsSmall;
+  const int T = (int)min(p.T - row0, (int64_t)kMaxRowsSmall), j = blockIdx.y * 8 + warp;
   if (threadIdx.x < T) {
-    const int a = p.row_adapter[threadIdx.x];
+    const int a = p.row_adapter[row0 + threadIdx.x];
     if (a >= p.n_adapters && threadIdx.x == t && blockIdx.y == 0) atomicOr(p.err, kErrBadIndex);
     ids[threadIdx.x] = a < p.n_adapters ? a : -1;
   }
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(256) k_lora_down_rows(const LoraLinear p, cons
   float s = 0.0f;
   if (a >= 0 && j < p.r) {
     const float scale = p.scale ? p.scale[a] : 1.0f;
-    const uint16_t* x = X + (int64_t)t * ldx;
+    const uint16_t* x = X + (row0 + t) * ldx;
     const uint16_t* w = A + ((int64_t)a * p.r + j) * lda;
     float2 s2 = make_float2(0.0f, 0.0f);
     const int whole = (int)(p.K / 8);
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(256) k_lora_down_rows(const LoraLinear p, cons
       if (own)
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(sh[e], part) << (16 * (e & 1));
-      uint16_t* dst = rk.H + ((((int64_t)threadIdx.x * rk.parts + part) * rk.rc + c) * TN + t) * rk.cw + j0 % rk.cw;
+      uint16_t* dst = rk.H + ((((row0 + threadIdx.x) * rk.parts + part) * rk.rc + c) * TN + t) * rk.cw + j0 % rk.cw;
       *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -138,8 +140,8 @@ __device__ __noinline__ int spoilt_feature(const LoraRows& g, const int* ids, co
   }
   return 0;
 }
-__device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int t, int64_t n, int TN) {
-  const uint16_t *x = g.X + t * g.ldx, *w = g.W + n * g.ldw;
+__device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int64_t row0, int t, int64_t n, int TN) {
+  const uint16_t *x = g.X + (row0 + t) * g.ldx, *w = g.W + n * g.ldw;
   float s = g.p.bias ? g.p.bias[n] : 0.0f;
   for (int64_t k = 0; k < g.p.K; ++k) s = fmaf(bf16_to_f32(x[k]), bf16_to_f32(w[k]), s);
   const int a = ids[t];
@@ -150,7 +152,7 @@ __device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int 
   for (int c = 0; c < g.p.r; ++c)
     for (int part = 0; part < g.rk.parts; ++part) {
       const uint16_t hv =
-          g.rk.H[((((int64_t)f * g.rk.parts + part) * g.rk.rc + c / g.rk.cw) * TN + t) * g.rk.cw + c % g.rk.cw];
+          g.rk.H[((((row0 + f) * g.rk.parts + part) * g.rk.rc + c / g.rk.cw) * TN + t) * g.rk.cw + c % g.rk.cw];
       s = fmaf(bf16_to_f32(hv), bf16_to_f32(b[c]), s);
     }
   return s;
@@ -198,8 +200,10 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
   volatile int* abort_flag = &abort_word;
   const LoraLinear& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = g.splits;
-  const int rank = blockIdx.x % splits, tile = blockIdx.x / splits;
-  const int T = (int)p.T, per_stage = 64 / g.rk.cw, cwb = 2 * g.rk.cw;
+  const int rank = blockIdx.x % splits, blocks = (int)((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
+  const int tile = blockIdx.x / splits / blocks;  // the blocks of rows side by side: W comes from L2 for all but one
+  const int row0 = (int)(blockIdx.x / splits % blocks) * kMaxRowsSmall;
+  const int T = min((int)p.T - row0, kMaxRowsSmall), per_stage = 64 / g.rk.cw, cwb = 2 * g.rk.cw;
   const int64_t n0 = (int64_t)tile * 128;
   const int kblocks = (int)((p.K + 63) / 64);
   const int kb0 = (int)((int64_t)kblocks * rank / splits), kb1 = (int)((int64_t)kblocks * (rank + 1) / splits);
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
         const uint32_t st = stage(C_::STAGE);
         if (!ok) break;
         tma_load_2d_elect(st, &tmW, full0 + (uint32_t)(at.slot * 8), kb * 64, (int)n0);
-        tma_load_2d_elect(st + C_::W_BYTES, &tmX, full0 + (uint32_t)(at.slot * 8), kb * 64, 0);
+        tma_load_2d_elect(st + C_::W_BYTES, &tmX, full0 + (uint32_t)(at.slot * 8), kb * 64, row0);
       }
       if (ok && g.rk.rc > 0) {
         ok = mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull);
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
           for (int i = 0; i < n; ++i) {
             const int q = (q0 + i) * splits + rank, f = list[q / g.rk.per()], sub = q % g.rk.per();
             tma_load_3d_elect(st + i * 128 * cwb, &tmB, bar, sub % g.rk.rc * g.rk.cw, (int)n0, ids[f]);
-            tma_load_2d_elect(st + C_::W_BYTES + i * TN * cwb, &tmH, bar, 0, (f * g.rk.per() + sub) * TN);
+            tma_load_2d_elect(st + C_::W_BYTES + i * TN * cwb, &tmH, bar, 0, ((row0 + f) * g.rk.per() + sub) * TN);
           }
         }
       }
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
     if (g.rk.rc > 0) {
       // The adapters among the rows, in the order of their first rows.
       if (tid < T) {
-        const int a = p.row_adapter[tid];
+        const int a = p.row_adapter[row0 + tid];
         ids[tid] = a < p.n_adapters ? a : -1;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -385,12 +389,12 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
             // Zero times what is not finite in another row's adapter is NaN: such a value is
             // computed again without the tensor core.
             if (spoilt < 0) spoilt = spoilt_feature(g, ids, list, in_warp[0], n);
-            if (spoilt) y[u] = redo_value(g, ids, t, n, TN);
+            if (spoilt) y[u] = redo_value(g, ids, row0, t, n, TN);
           }
           if (p.y_bf16)
-            ((uint16_t*)p.Y)[t * p.ldy + n] = f32_to_bf16_rne(y[u]);
+            ((uint16_t*)p.Y)[(row0 + t) * p.ldy + n] = f32_to_bf16_rne(y[u]);
           else
-            ((float*)p.Y)[t * p.ldy + n] = y[u];
+            ((float*)p.Y)[(row0 + t) * p.ldy + n] = y[u];
         }
       }
     }
@@ -468,6 +472,13 @@ __global__ void __launch_bounds__(256) k_lora_pack(const __grid_constant__ PackA
   }
 }
 
+// K splits of k_lora_rows, until two CTAs a processor have a part, of two K blocks at least.
+int row_splits(const LoraLinear& p) {
+  const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall), kblocks = (p.K + 63) / 64;
+  int splits = 1;
+  while (splits < 8 && kblocks >= 4 * splits && tiles * splits * 2 <= (int64_t)ctx().num_sms * 2) splits *= 2;
+  return splits;
+}
 int rows_tile(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128; }
 RowsK lay_out_rows(const LoraLinear& p, uint8_t* at, size_t* bytes) {
   RowsK k{};
@@ -513,11 +524,8 @@ void launch_rows(LoraRows g) {
   } else {
     tb = th = tx;  // no chunk is read
   }
-  const int64_t tiles = (p.N + 127) / 128;
-  const int kblocks = (int)((p.K + 63) / 64);
-  // K splits until two CTAs a processor have a part, of two K blocks at least.
-  g.splits = 1;
-  while (g.splits < 8 && kblocks >= 4 * g.splits && tiles * g.splits * 2 <= (int64_t)c.num_sms * 2) g.splits *= 2;
+  const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
+  g.splits = row_splits(p);
   static bool done[64] = {};
   if (!done[c.device]) {
     check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM),
@@ -1277,6 +1285,52 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   check_launch("linear_lora");
 }
 
+// Tile shape by waves, as gemm_tc.cu prices them: a tile costs its width and 48 columns of
+// fixed cost, a pair tile (256 rows over two processors) 8% less. Several pair widths, because
+// a few rows of tiles leave the last wave nearly empty: 2397 x 4096 outputs are 2.2 waves of
+// 256 columns (3 x 280) but 3.0 waves of 192 (3 x 221).
+struct Tile {
+  int bm, bn;
+  double cost;
+};
+Tile choose_tile(int64_t rows, int64_t N, bool adapters) {
+  const int sms = ctx().num_sms;
+  Tile best{128, 64, 1e30};
+  for (int bn : {256, 224, 192, 160, 128, 64})
+    for (int bm : {256, 128}) {
+      if (bm == 256 ? bn == 64 || rows <= 128 : bn != 256 && bn != 128 && bn != 64) continue;
+      const int64_t m = (rows + bm - 1) / bm;
+      const double down = adapters ? 0.3 * (double)m : 0.0;  // the items that make H
+      const double x = std::ceil(((double)(m * ((N + bn - 1) / bn)) + down) / (bm == 256 ? sms / 2 : sms)) * (bn + 48) *
+                       (bm == 256 ? 0.92 : 1.0);
+      if (x < best.cost - 1e-9) best = Tile{bm, bn, x};
+    }
+  return best;
+}
+
+// Whether k_lora_rows, in blocks of 128 rows, takes fewer microseconds than the GEMM. The
+// GEMM's groups of 256 rows multiply every row with all adapters of the group, so requests of few
+// rows each cost it dearly: 129 rows, 3840 x 3840, rank 128, take 40 us with 2 requests, 144
+// with 16 and 506 with 64; k_lora_rows takes 38, 40 and 52, but 153 to 170 (42, 56 and 112)
+// for 1024 rows, because it reads an adapter anew for every row. How many adapters the rows
+// use is known on the device only; a mixture of 16 is assumed, or all there are. The constants
+// are fitted to N, K from 224 to 10240, ranks 16 and 128, T from 129 to 1024.
+bool few_rows(const LoraLinear& p) {
+  if (p.T <= kMaxRowsSmall) return true;
+  if (p.T > 1024 || p.n_adapters <= 0 || p.r <= 0) return false;
+  const int sms = ctx().num_sms, splits = row_splits(p);
+  const double kb = (double)((p.K + 63) / 64), t = (double)p.T;
+  const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
+  const double rows = 12.0 + std::ceil((double)(tiles * splits) / (2 * sms)) * (kb / splits) * 0.6 +
+                      t * (double)p.r * (2.7e-4 + 1.5e-7 * (double)p.K);
+  const Tile tile = choose_tile(p.T, p.N, true);
+  const int64_t m = (p.T + tile.bm - 1) / tile.bm;
+  const double ksplit = std::max(1.0, std::min({8.0, (double)sms / (tile.bm / 128) / (double)m, kb / 2}));
+  const double chunks = (double)std::min<int64_t>(p.n_adapters, 16) / (double)((p.T + kGroup - 1) / kGroup) *
+                        (double)round_up(p.r, chunk_width(p.r)) / 64.0;
+  return rows < 12.0 + tile.cost * kb * 1.1e-3 + chunks * (1.8 + 0.25 * kb / ksplit);
+}
+
 // What the large path keeps in the workspace: one block of rows' lists and H.
 struct Big {
   LoraK lk;
@@ -1327,31 +1381,12 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
   g.y_tma = aligned16(p.Y) && p.ldy % (p.y_bf16 ? 8 : 4) == 0;
   for (g.row0 = 0; g.row0 < p.T; g.row0 += big.rows) {
     g.rows = std::min(big.rows, p.T - g.row0);
+    const Tile tile = choose_tile(g.rows, p.N, adapters);
     if (adapters) {
       k_lora_lists<<<(unsigned)((g.rows + kGroup - 1) / kGroup), kGroup, 0, c.stream>>>(p, g.lk, g.row0, g.rows);
       check_launch("lora_lists");
     }
-    // Tile shape by waves, as gemm_tc.cu prices them: a tile costs its width and 48 columns
-    // of fixed cost, a pair tile (256 rows over two processors) 8% less. Several pair widths,
-    // because a few rows of tiles leave the last wave nearly empty: 2397 x 4096 outputs are
-    // 2.2 waves of 256 columns (3 x 280) but 3.0 waves of 192 (3 x 221).
-    auto cost = [&](int bm, int bn, int64_t units) {
-      const int64_t rows = (g.rows + bm - 1) / bm, t = rows * ((p.N + bn - 1) / bn);
-      const double down = adapters ? 0.3 * (double)rows : 0.0;  // the items that make H
-      return std::ceil(((double)t + down) / (double)units) * (bn + 48) * (bm == 256 ? 0.92 : 1.0);
-    };
-    double best = 1e30;
-    int bm = 128, bn = 64;
-    for (int cand : {256, 224, 192, 160, 128, 64})
-      for (int rows : {256, 128}) {
-        if (rows == 256 ? cand == 64 || g.rows <= 128 : cand != 256 && cand != 128 && cand != 64) continue;
-        const double x = cost(rows, cand, rows == 256 ? c.num_sms / 2 : c.num_sms);
-        if (x < best - 1e-9) {
-          best = x;
-          bm = rows;
-          bn = cand;
-        }
-      }
+    const int bm = tile.bm, bn = tile.bn;
     if (bm == 256) {
       if (bn == 256) launch_lora_gemm<256, true>(g, A, lda, adapters);
       if (bn == 224) launch_lora_gemm<224, true>(g, A, lda, adapters);
@@ -1370,7 +1405,7 @@ void launch_big(const LoraLinear& p, const uint16_t* X, int64_t ldx, const uint1
 
 size_t lora_linear_workspace(const LoraLinear& p) {
   const Operands o = lay_out(p);
-  if (p.T > kMaxRowsSmall) return lay_out_big(p, o.h_at).bytes;
+  if (!few_rows(p)) return lay_out_big(p, o.h_at).bytes;
   size_t h;
   lay_out_rows(p, nullptr, &h);
   return o.h_at + h;
@@ -1402,7 +1437,7 @@ void launch_lora_linear(LoraLinear p, void* ws_) {
     k_lora_pack<<<(unsigned)grid, 256, 0, c.stream>>>(all);
     check_launch("lora_pack");
   }
-  if (p.T > kMaxRowsSmall) return launch_big(p, X, ldx, W, ldw, A, lda, B, ldb, ws, lay_out_big(p, o.h_at));
+  if (!few_rows(p)) return launch_big(p, X, ldx, W, ldw, A, lda, B, ldb, ws, lay_out_big(p, o.h_at));
   size_t h;
   LoraRows g{p, lay_out_rows(p, ws + o.h_at, &h), X, W, B, ldx, ldw, ldb, 1};
   const int tn = rows_tile(p.T);
