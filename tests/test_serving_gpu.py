@@ -245,6 +245,26 @@ def test_linear_lora(sdb, case):
     lora_close(got, x, W, A, B, rows, scale, bias)
 
 
+@pytest.mark.parametrize("case", [
+    (1025, 8, 24, 2, 3, "random", BF16, BF16, True, True),
+    (1030, 96, 64, 256, 3, "runs", BF16, F32, True, True),
+    (1100, 777, 331, 20, 6, "random", BF16, BF16, True, True),
+    (1153, 300, 72, 33, 200, "each", BF16, F32, True, False),
+    (1281, 512, 512, 16, 4, "none", BF16, F32, True, True),
+    (1536, 130, 1000, 64, 1, "one", F32, BF16, False, True),
+    (1023, 72, 136, 16, 300, "each", BF16, F32, True, True),           # eight blocks of 128 rows
+], ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_linear_lora_of_many_rows(sdb, case):
+    test_linear_lora(sdb, case)
+
+
+@pytest.mark.parametrize("T", [1100, 1500])
+@pytest.mark.parametrize("to", [BF16, F32])
+def test_linear_lora_of_many_rows_keeps_requests_apart(sdb, T, to):
+    test_linear_lora_strided_operands(sdb, T)
+    test_linear_lora_keeps_requests_apart(sdb, T, 320, to)
+
+
 @pytest.mark.parametrize("T", [5, 40, 200, 600])
 def test_linear_lora_strided_operands(sdb, T):
     """Row pitches and bases that TMA cannot read, outputs with gaps left as they were."""
