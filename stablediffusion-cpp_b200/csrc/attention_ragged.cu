@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention_ragged_any(const Ragg
 
 template <class TI, class TO>
 void launch_any(const RaggedAttention& p) {
-  const dim3 grid((unsigned)((p.max_q + kWarps - 1) / kWarps), (unsigned)p.heads, (unsigned)p.n_seq);
+  const dim3 grid((unsigned)((std::min(p.max_q, p.Tq) + kWarps - 1) / kWarps), (unsigned)p.heads, (unsigned)p.n_seq);
   k_attention_ragged_any<TI, TO><<<grid, kWarps * 32, 0, ctx().stream>>>(p);
   check_launch("attention_ragged");
 }
@@ -96,7 +96,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // TMA reads rows and heads that start on 16-byte boundaries; wider heads than two swizzle
 // atoms do not fit the tensor-core kernels' shared memory.
 bool tensor_core_shape(const RaggedAttention& p) {
-  return p.d <= 128 && p.d % 8 == 0 && p.ldq % 8 == 0 && p.ldk % 8 == 0 && p.ldv % 8 == 0 && p.max_kv > 0 &&
+  return p.d <= 128 && p.d % 8 == 0 && p.ldq % 8 == 0 && p.ldk % 8 == 0 && p.ldv % 8 == 0 && p.max_kv > 0 && p.Tkv > 0 &&
          aligned16(p.q) && aligned16(p.k) && aligned16(p.v);
 }
 

@@ -571,8 +571,10 @@ __device__ __forceinline__ int find_pair(const TcParams& p, int want, int* sh, i
     }
     __syncthreads();
     base = all;
-    if (sh[13] >= 0) break;
+    if (sh[13] >= 0 && blockIdx.x < gridDim.x - 1) break;
   }
+  // The launch has room for the pairs of sequences that share no query row.
+  if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1 && base > (int)(gridDim.x / p.a.kv_heads)) atomicOr(p.a.err, kErrBadIndex);
   pair = sh[14];
   return sh[13];
 }
@@ -1296,7 +1298,7 @@ void launch_streams(TcParams& p, const CUtensorMap& tq, const CUtensorMap& tk, c
   static bool done[64] = {};
   prepare_kernel(k_ragged_streams<DP, T, MOD, FEW>, kMaxSmem - (int)sizeof(StepList) - 1024, done);
   // Sequences of one launch: as many as its step list holds, below 2^31 steps.
-  const int64_t most = ((p.a.max_kv + kBK - 1) / kBK) * p.a.kv_heads + p.a.kv_heads;
+  const int64_t most = ((std::min(p.a.max_kv, p.a.Tkv) + kBK - 1) / kBK) * p.a.kv_heads + p.a.kv_heads;
   if (most >= ((int64_t)1 << 31)) fail(kErrInvalidArg, "attention_ragged: too many keys");
   p.seqs = (int)std::min<int64_t>(kMaxSeqs, (((int64_t)1 << 31) - 1) / most);
   for (p.seq0 = 0; p.seq0 < p.a.n_seq; p.seq0 += p.seqs) {

@@ -66,7 +66,8 @@ void check_attention(const RaggedAttention& p) {
   require(p.out_type == kBF16 || p.out_type == kF16, op, "output must be bf16 or fp16");
   require(p.n_seq >= 0 && p.n_seq <= 65535, op, "n_seq must be 0..65535");
   require(p.Tq >= 0 && p.Tkv >= 0 && p.max_q >= 0 && p.max_kv >= 0, op, "bad shape");
-  require(p.Tq < kMaxRows && p.Tkv < kMaxRows, op, "row count >= 2^31");
+  // A tile may end up to 256 rows past the last one; that is still an int.
+  require(p.Tq < kMaxRows - 256 && p.Tkv < kMaxRows - 256, op, "row count >= 2^31 - 256");
   require(p.heads > 0 && p.kv_heads > 0 && p.heads % p.kv_heads == 0, op, "heads must be a multiple of kv_heads");
   require(p.heads <= 65535 && p.heads / p.kv_heads <= 128, op, "too many heads");
   require(p.d > 0 && p.d <= 256, op, "head width must be 1..256");
@@ -174,8 +175,8 @@ static RaggedAttention attention_args(const void* q, int64_t ldq, const void* k,
                                       int heads, int kv_heads, int64_t d, float scale, float cap, const float* slopes,
                                       int causal, const int32_t* prefix) {
   return RaggedAttention{q, k, v, out, ldq, ldk, ldv, ldo, in_type, out_type, Tq, Tkv, n_seq, q_begin, q_len, kv_begin,
-                         kv_len, max_q, max_kv, heads, kv_heads, (int)std::min<int64_t>(d, 1 << 30), scale, cap, slopes,
-                         causal != 0, prefix, nullptr};
+                         kv_len, std::min(max_q, kMaxRows), std::min(max_kv, kMaxRows), heads, kv_heads,
+                         (int)std::min<int64_t>(d, 1 << 30), scale, cap, slopes, causal != 0, prefix, nullptr};
 }
 
 int64_t sdb200_attention_ragged_workspace(int n_seq, int64_t max_q, int64_t max_kv, int heads, int kv_heads,
@@ -205,9 +206,7 @@ int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t l
                                        q_len, kv_begin, kv_len, max_q, max_kv, heads, kv_heads, d, scale, cap, slopes,
                                        causal, prefix);
     check_attention(p);
-    p.max_q = std::min(p.max_q, Tq);
-    p.max_kv = std::min(p.max_kv, Tkv);
-    if (n_seq == 0 || p.max_q == 0) return kOk;
+    if (n_seq == 0 || max_q == 0 || Tq == 0) return kOk;
     require_ptr(q_begin, 4, op, "q_begin");
     require_ptr(q_len, 4, op, "q_len");
     require_ptr(kv_begin, 4, op, "kv_begin");
@@ -215,7 +214,7 @@ int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t l
     require(ldq >= heads * d && ldo >= heads * d, op, "row pitch smaller than heads * d");
     require_ptr(q, 2, op, "q");
     require_ptr(out, 2, op, "out");
-    if (p.max_kv > 0) {
+    if (p.max_kv > 0 && Tkv > 0) {
       require(ldk >= kv_heads * d && ldv >= kv_heads * d, op, "row pitch smaller than kv_heads * d");
       require_ptr(k, 2, op, "k");
       require_ptr(v, 2, op, "v");
@@ -227,7 +226,7 @@ int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t l
       require(rows <= 0 || o1 <= x0 || x0 + ((rows - 1) * ld + cols) * 2 <= o0, op, std::string("out overlaps ") + name);
     };
     apart(q, Tq, ldq, heads * d, "q");
-    if (p.max_kv > 0) {
+    if (p.max_kv > 0 && Tkv > 0) {
       apart(k, Tkv, ldk, kv_heads * d, "k");
       apart(v, Tkv, ldv, kv_heads * d, "v");
     }

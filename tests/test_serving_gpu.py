@@ -485,6 +485,27 @@ def test_attention_ragged_loose_maxima(sdb):
     run_attn(sdb, [1, 1], [90, 600], 4, 2, 128, BF16, causal=True, max_q=1, max_kv=1 << 40)
 
 
+@pytest.mark.parametrize("max_q,max_kv", [(50, 700), (4000, 700), (1 << 40, 1 << 40), (50, 1 << 40)])
+def test_attention_ragged_c_call_with_loose_maxima(sdb, max_q, max_kv):
+    """The workspace that the C function names is enough for the same maxima, however loose."""
+    g, d = gen(17), 64
+    q, k, v = randn(g, 50, 2, d, dtype=F16), randn(g, 700, 1, d, dtype=F16), randn(g, 700, 1, d, dtype=F16)
+    out = torch.empty_like(q)
+    cols = [torch.tensor([x], device="cuda", dtype=torch.int32) for x in (0, 50, 0, 700)]
+    L = sdb.lib()
+    need = L.sdb200_attention_ragged_workspace(1, max_q, max_kv, 2, 1, d)
+    assert need >= 0
+    ws = torch.empty(max(need, 256), device="cuda", dtype=torch.uint8)
+    torch.cuda.synchronize()
+    rc = L.sdb200_set_stream(torch.cuda.current_stream().cuda_stream) or L.sdb200_attention_ragged(
+        q.data_ptr(), 2 * d, k.data_ptr(), d, v.data_ptr(), d, 2, out.data_ptr(), 2 * d, 2, 50, 700, 1,
+        *[c.data_ptr() for c in cols], max_q, max_kv, 2, 1, d, d ** -0.5, 0.0, None, 0, None, ws.data_ptr(), need)
+    assert rc == 0
+    sdb.backend.synchronize()
+    want, slack, _ = attn_want(q, k, v, [(0, 50, 0, 700)], d ** -0.5, False, None, 0.0, None, F16)
+    close(out, want, slack)
+
+
 def test_attention_ragged_strided_rows_and_shared_keys(sdb):
     """q, k, v as views of one fused projection; two sequences that read the same keys."""
     g = gen(9)
@@ -528,6 +549,40 @@ def test_attention_ragged_masked_values_do_not_count(sdb, lens):
     keep = torch.ones(d, dtype=torch.bool, device="cuda")
     keep[3] = False
     close(got[:, :2][:, :, keep], want[:, :2][:, :, keep], slack[:, :2][:, :, keep])
+
+
+LONG = [  # sequences of several tiles of queries and many of keys
+    ([700, 1, 300], [1500, 1, 900], 6, 2, 64, F16, dict(causal=True)),
+    ([1030], [1030], 2, 1, 128, BF16, {}),
+    ([130, 900], [2600, 900], 3, 3, 128, F16, dict(causal=True, prefix=[2000, 5], cap=30.0, bias=True)),
+    ([257, 0, 40, 600], [640, 5, 2000, 0], 4, 4, 40, BF16, {}),
+    ([300], [5000], 16, 2, 80, BF16, dict(bias=True)),
+    ([50] * 20 + [1200], [50] * 20 + [1333], 8, 8, 64, F16, dict(causal=True, cap=20.0)),
+    ([900], [700], 4, 1, 128, F16, dict(causal=True)),
+    ([400], [513], 64, 1, 8, BF16, {}),
+]
+
+
+@pytest.mark.parametrize("gap", [0, 7])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[2]}-{c[3]}-{c[4]}")
+def test_attention_ragged_of_long_sequences(sdb, case, gap):
+    test_attention_ragged(sdb, case, gap)
+
+
+def test_attention_ragged_of_long_sequences_isolates_and_reports(sdb):
+    test_attention_ragged_masked_values_do_not_count(sdb, ([900, 700], [900, 1800]))
+    test_attention_ragged_skips_bad_sequences(sdb, ([900, 60, 700], [900, 160, 1300]))
+
+
+@pytest.mark.parametrize("n", [300, 700])
+def test_attention_ragged_reports_shared_query_rows(sdb, n):
+    """Eight sequences of the same query rows: more tiles than rows of their own could make."""
+    g = gen(n)
+    q, k, v = (randn(g, n, 1, 64, dtype=F16) for _ in range(3))
+    cols = [torch.full((8,), x, device="cuda", dtype=torch.int32) for x in (0, n, 0, n)]
+    sdb.backend.attention_ragged(q, k, v, *cols, n, n)
+    with pytest.raises(sdb.SdbError, match="out of range"):
+        sdb.backend.synchronize()
 
 
 @pytest.mark.parametrize("lens", [([1, 1, 1], [200, 300, 9]), ([300, 60, 9], [300, 160, 9])])
