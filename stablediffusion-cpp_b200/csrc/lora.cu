@@ -437,9 +437,8 @@ Operands lay_out(const LoraLinear& p) {
 }
 
 // Up to four matrices in one launch: rows of `cols` values, bf16 or fp32 (rounded to bf16),
-// to rows of `pitch` bf16, zero past cols. Eight values a thread: 16-byte stores, loads that a
-// warp's lines cover. Bound by memory; the copies of packed operands would otherwise cost more
-// than the product of a few rows (46 us for a 455 x 8276 W with one value a thread).
+// to rows of `pitch` bf16, zero past cols. Eight values a thread: a 16-byte store of what lies
+// in two aligned 16-byte words (bf16), or eight loads where those would leave the matrix.
 struct PackOne {
   const void* src;
   uint16_t* dst;
@@ -461,6 +460,26 @@ __global__ void __launch_bounds__(256) k_lora_pack(const __grid_constant__ PackA
     const int64_t r = x / per;
     const int c = (int)(x - r * per) * 8;
     uint32_t w[4] = {0, 0, 0, 0};
+    const uintptr_t from = reinterpret_cast<uintptr_t>(m.src) + (uintptr_t)(r * m.ld + c) * 2, word = from & ~uintptr_t(15);
+    if (!m.f32 && c + 8 <= m.cols && word >= reinterpret_cast<uintptr_t>(m.src) &&
+        word + 32 <= reinterpret_cast<uintptr_t>(m.src) + (uintptr_t)((m.rows - 1) * m.ld + m.cols) * 2) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(word)), b = __ldg(reinterpret_cast<const uint4*>(word) + 1);
+      const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      const int skip = (int)(from & 15) >> 2, half = (int)(from & 2) * 8;  // whole words, and 16 bits of one
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t lo = v[i], hi = v[i + 1];
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+          if (skip == k) {
+            lo = v[i + k];
+            hi = i + k + 1 < 8 ? v[i + k + 1] : 0u;
+          }
+        w[i] = __funnelshift_r(lo, hi, half);
+      }
+      *reinterpret_cast<uint4*>(m.dst + r * m.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      continue;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e < m.cols) {
