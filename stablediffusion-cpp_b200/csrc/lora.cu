@@ -36,16 +36,23 @@ __device__ __forceinline__ uint64_t sdesc_k(uint32_t saddr, int pitch) {
   d |= (uint64_t)(pitch == 128 ? 2u : pitch == 64 ? 4u : 6u) << 61;
   return d;
 }
+// Conversions by the processor's own instructions: eight integer ones and a branch per value
+// (f32_to_bf16_rne) were two thirds of the time of products of short rows.
+__device__ __forceinline__ uint16_t bf16_bits(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 // Two bf16 of a word, the low half first.
 __device__ __forceinline__ float2 bf16x2_to_f32(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 // h in bf16 (part 0), and what that lost (part 1): together h to 2^-16.
 __device__ __forceinline__ uint32_t h_part(float h, int part) {
-  const uint32_t hi = f32_to_bf16_rne(h);
+  const uint32_t hi = bf16_bits(h);
   if (!part) return hi;
   const float v = bf16_to_f32((uint16_t)hi);
-  return f32_to_bf16_rne(fabsf(v) < INFINITY ? h - v : 0.0f);
+  return bf16_bits(fabsf(v) < INFINITY ? h - v : 0.0f);
 }
 inline int chunk_width(int64_t r) { return r <= 16 ? 16 : r <= 32 ? 32 : 64; }
 inline CUtensorMapSwizzle swizzle_of(int cw) {
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
             if (spoilt) y[u] = redo_value(g, ids, row0, t, n, TN);
           }
           if (p.y_bf16)
-            ((uint16_t*)p.Y)[(row0 + t) * p.ldy + n] = f32_to_bf16_rne(y[u]);
+            ((uint16_t*)p.Y)[(row0 + t) * p.ldy + n] = bf16_bits(y[u]);
           else
             ((float*)p.Y)[(row0 + t) * p.ldy + n] = y[u];
         }
@@ -484,7 +491,7 @@ __global__ void __launch_bounds__(256) k_lora_pack(const __grid_constant__ PackA
     for (int e = 0; e < 8; ++e)
       if (c + e < m.cols) {
         const int64_t at = r * m.ld + c + e;
-        const uint32_t v = m.f32 ? f32_to_bf16_rne(((const float*)m.src)[at]) : ((const uint16_t*)m.src)[at];
+        const uint32_t v = m.f32 ? bf16_bits(((const float*)m.src)[at]) : ((const uint16_t*)m.src)[at];
         w[e >> 1] |= v << (16 * (e & 1));
       }
     *reinterpret_cast<uint4*>(m.dst + r * m.pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -709,7 +716,7 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
       s = warp_add(s) + (p.bias ? p.bias[n] : 0.0f);
       if (lane == 0) {
         if (p.y_bf16)
-          ((uint16_t*)p.Y)[(row0 + t) * p.ldy + n] = f32_to_bf16_rne(s);
+          ((uint16_t*)p.Y)[(row0 + t) * p.ldy + n] = bf16_bits(s);
         else
           ((float*)p.Y)[(row0 + t) * p.ldy + n] = s;
       }
@@ -1176,8 +1183,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<uint4*>(buf + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) =
-                    make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                               pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+                    make_uint4(bf16_pair(v[8 * j], v[8 * j + 1]), bf16_pair(v[8 * j + 2], v[8 * j + 3]),
+                               bf16_pair(v[8 * j + 4], v[8 * j + 5]), bf16_pair(v[8 * j + 6], v[8 * j + 7]));
             } else {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
@@ -1198,7 +1205,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             for (int i = 0; i < (int)min((int64_t)32, g.row0 + g.rows - first); ++i) {
               const float x = reinterpret_cast<const float*>(buf)[i * 32 + (lane ^ i)];
               if (g.p.y_bf16)
-                ((uint16_t*)g.p.Y)[(first + i) * g.p.ldy + col0 + lane] = f32_to_bf16_rne(x);
+                ((uint16_t*)g.p.Y)[(first + i) * g.p.ldy + col0 + lane] = bf16_bits(x);
               else
                 ((float*)g.p.Y)[(first + i) * g.p.ldy + col0 + lane] = x;
             }
