@@ -244,7 +244,7 @@ int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const 
  *   Y[t, n] = X[t, :] W[n, :] (+ bias[n]) + scale[a] * sum_j (X[t, :] A_a[j, :]) B_a[n, j]
  * and no second term where a < 0. X [T, ldx] bf16 (x_bf16 != 0) or fp32 (rounded to bf16 as
  * gemm_nt_bf16 rounds it); W [N, ldw], A [n_adapters, r, lda], B [n_adapters, N, ldb] bf16;
- * scale fp32 [n_adapters] or null for 1; Y fp32 or bf16 (y_bf16). r <= 256; adapters of
+ * scale fp32 [n_adapters] or null for 1; Y fp32 or bf16 (y_bf16), apart from the operands. r <= 256; adapters of
  * smaller rank are padded with zeros. Accumulation is fp32. ws: at least
  * sdb200_linear_lora_workspace() bytes for the same arguments. */
 int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void* X, int64_t ldx, int x_bf16,

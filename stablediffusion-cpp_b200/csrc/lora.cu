@@ -736,7 +736,8 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
 // epilogue keeps each row's own, scaled, and counts up `done`. The other items are
 // the tiles of Y: the K blocks of X and W first, then, once `done` says that H is complete,
 // the chunks of H and B, 64 / cw of them a stage. Every unit runs its items of the first kind
-// before those of the second, and only the second kind waits, so the wait ends. In a kernel of its
+// before those of the second, only the second kind waits, and a cooperative launch has all units
+// resident, so the wait ends. In a kernel of its
 // own the adapter product cost a pass over X that nothing overlapped: 827 instead of
 // us at 33792 x 3840 x 3840 with one adapter of rank 16 (640 without).
 template <int BN, bool PAIR>
@@ -1284,7 +1285,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   static int clusters[64] = {};
   auto kern = k_lora_gemm<BN, PAIR>;
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[2] = {};
+  cudaLaunchAttribute attr[3] = {};
   int n = 0;
   if (PAIR) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
@@ -1309,6 +1310,11 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   if (overlap) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+    // Units wait for H that others make, so all must be resident: two such launches at once,
+    // each with a part of the processors, would wait for each other's.
+    attr[n].id = cudaLaunchAttributeCooperative;
+    attr[n].val.cooperative = 1;
     ++n;
   }
   cfg.numAttrs = n;

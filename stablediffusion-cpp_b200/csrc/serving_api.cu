@@ -33,10 +33,21 @@ void require_apart(const char* op, const char* what, const void* x, int64_t ldx,
   require(y1 <= x0 || x1 <= y0, op, std::string(what) + " overlaps its input without being the same buffer");
 }
 
+// Whether rows of x and of y share bytes; rows of one pitch may lie side by side.
+bool share(const void* x, int64_t x_rows, int64_t x_pitch, int64_t x_bytes, const void* y, int64_t y_rows, int64_t y_pitch,
+           int64_t y_bytes) {
+  const char *x0 = (const char*)x, *y0 = (const char*)y;
+  if (y0 + (y_rows - 1) * y_pitch + y_bytes <= x0 || x0 + (x_rows - 1) * x_pitch + x_bytes <= y0) return false;
+  if (x_pitch != y_pitch) return true;
+  const int64_t off = (((y0 - x0) % x_pitch) + x_pitch) % x_pitch;
+  return off < x_bytes || off + y_bytes > x_pitch;
+}
+
 void check_lora(const LoraLinear& p) {
   const char* op = "linear_lora";
   require(p.T >= 0 && p.N >= 0 && p.K > 0 && p.n_adapters >= 0 && p.r >= 0, op, "bad shape");
-  require(p.T < kMaxRows && p.N < kMaxRows && p.K < kMaxRows && p.n_adapters < kMaxRows, op, "dimension >= 2^31");
+  // A tile may end up to 512 rows or columns past the last one; that is still an int.
+  require(std::max({p.T, p.N, p.K, p.n_adapters}) < kMaxRows - 512, op, "dimension >= 2^31 - 512");
   require(p.r <= 256, op, "rank > 256");
   if (p.T == 0 || p.N == 0) return;
   require(p.ldx >= p.K && p.ldw >= p.K && p.ldy >= p.N, op, "leading dimension too small");
@@ -161,6 +172,17 @@ int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t l
     check_lora(p);
     if (T == 0 || N == 0) return kOk;
     require_ptr(Y, p.y_bf16 ? 2 : 4, op, "Y");
+    const int64_t ey = p.y_bf16 ? 2 : 4;
+    const int64_t ex = p.x_bf16 ? 2 : 4;
+    auto apart = [&](const void* x, int64_t rows, int64_t ld, int64_t cols, int64_t e, const char* name) {
+      require(!share(x, rows, ld * e, cols * e, Y, T, ldy * ey, N * ey), op, std::string("Y overlaps ") + name);
+    };
+    apart(X, T, ldx, K, ex, "X");
+    apart(W, N, ldw, K, 2, "W");
+    if (n_adapters > 0 && r > 0) {
+      apart(A, n_adapters * r, lda, K, 2, "A");
+      apart(B, n_adapters * N, ldb, r, 2, "B");
+    }
     const int64_t need = (int64_t)lora_linear_workspace(p);
     require(ws_bytes >= need, op, "workspace of " + std::to_string(need) + " bytes needed");
     if (need) require_ptr(ws, 256, op, "ws");

@@ -67,6 +67,21 @@ def test_linear_lora_refusals(kw, text):
     refused(lora(**kw), text)
 
 
+@pytest.mark.parametrize("kw,text", [
+    (dict(Y=P), "Y overlaps X"), (dict(Y=P + 128, X=P2 + (1 << 20), ldw=64), "Y overlaps W"),
+    (dict(X=P2 + (1 << 20), W=P2 + (1 << 20), Y=P), "Y overlaps A"), (dict(T=(1 << 31) - 512), "2^31"),
+    (dict(Y=P2, X=P2 + 100, ldx=64), "Y overlaps X"),
+])
+def test_linear_lora_refuses_shared_buffers_and_huge_ones(kw, text):
+    refused(lora(**kw), text)
+
+
+def test_linear_lora_takes_columns_side_by_side():
+    """X and Y may be columns of the same rows: only the missing workspace is refused here."""
+    refused(lora(X=P2, ldx=96, Y=P2 + 64, ldy=96), "workspace of")
+    refused(lora(X=P2 + 128, ldx=96, Y=P2, ldy=96), "workspace of")
+
+
 def attn(**kw):
     a = dict(q=P, ldq=128, k=P, ldk=64, v=P, ldv=64, in_type=BF16, out=P2, ldo=128, out_type=BF16, Tq=4, Tkv=9, n_seq=2,
              q_begin=P, q_len=P, kv_begin=P, kv_len=P, max_q=4, max_kv=9, heads=4, kv_heads=2, d=32, scale=0.1, cap=0.0,
@@ -89,6 +104,11 @@ def attn(**kw):
 ])
 def test_attention_ragged_refusals(kw, text):
     refused(attn(**kw), text)
+
+
+@pytest.mark.parametrize("kw", [dict(Tq=(1 << 31) - 256), dict(Tkv=(1 << 31) - 256)])
+def test_attention_ragged_refuses_huge_tensors(kw):
+    refused(attn(**kw), "2^31")
 
 
 def test_wrappers_refuse_host_tensors():

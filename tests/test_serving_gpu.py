@@ -706,6 +706,39 @@ def test_the_three_on_their_own_stream_and_in_graphs(sdb):
     sdb.backend.synchronize()
 
 
+def test_linear_lora_on_two_streams_at_once(sdb):
+    """Calls whose processors wait for one another's h, on streams of different priorities."""
+    g = gen(23)
+    calls, streams = [], [torch.cuda.Stream(), torch.cuda.Stream(priority=-1)]
+    for T, N, K, r, n in ((3000, 2048, 512, 32, 5), (5000, 1024, 640, 16, 3)):
+        x, W, A, B, scale, bias = lora_inputs(g, T, N, K, r, n)
+        calls.append((x, W, A, B, lora_rows(g, "runs", T, n), scale, bias))
+    want = [sdb.backend.linear_lora(*c) for c in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(sdb.backend.linear_lora(*calls[i]))
+    torch.cuda.synchronize()
+    sdb.backend.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+@pytest.mark.parametrize("T", [7, 300, 1100])
+def test_linear_lora_beside_its_input(sdb, T):
+    """x and out are columns of one buffer."""
+    g = gen(T)
+    x, W, A, B, scale, bias = lora_inputs(g, T, 128, 64, 16, 3)
+    rows = lora_rows(g, "random", T, 3)
+    buf = torch.cat([x, torch.zeros(T, 128, device="cuda", dtype=BF16)], 1)
+    sdb.backend.linear_lora(buf[:, :64], W, A, B, rows, scale=scale, bias=bias, out=buf[:, 64:])
+    sdb.backend.synchronize()
+    assert torch.equal(buf[:, :64], x)
+    lora_close(buf[:, 64:], x, W, A, B, rows, scale, bias)
+
+
 def test_the_three_repeat_exactly(sdb):
     s = layer_inputs([333, 1, 64], 5)
     a = layer(sdb, **s)
