@@ -3,6 +3,8 @@
 // scores never leave the SM:
 //   S = Q K^T (tcgen05, fp32 in TMEM);  P = 2^(S' - m) in the operand type, back in TMEM over
 //   S;  O += P V (tcgen05);  O is rescaled when m grows by more than 2^8; out = O / l.
+// P is rounded to the operand type because the tensor core multiplies it so: 2^-8 (bf16) or
+// 2^-11 (fp16) of each probability, averaged over the keys; l, m, S and O stay fp32.
 //
 // The G = heads / kv_heads query heads of a key head share its keys, so a 128-row tile
 // holds floor(128 / G) tokens x G heads (row r is token r / G, head r % G): K and V are read
@@ -11,13 +13,18 @@
 // Two kernels:
 //   k_ragged_tiles    sequences of several tiles: a CTA owns two neighbouring tiles of one
 //                     key head, which share one ring of K / V slots and take turns at the
-//                     exp pass (as attention_tc.cu).
+//                     exp pass (as attention_tc.cu). Bound by the exponentials in the
+//                     chain of a tile step: 4 x 4200 tokens, 30 heads of 128, 1040 to
+//                     1160 us (0.92 to 1.02 PFLOP/s).
 //   k_ragged_streams  sequences of one tile (single tokens, short prompts): the CTAs are
 //                     persistent, each with two workers that own a tile and a ring of
 //                     their own. The key tiles of all sequences and heads form one list,
 //                     cut into equal parts, one per worker, whatever the lengths are;
 //                     a worker's first and last piece may be part of a row, kept as
-//                     (m, l, O) in fp32 and joined by k_ragged_join.
+//                     (m, l, O) in fp32 and joined by k_ragged_join. Bound by memory
+//                     with long caches (16 tokens over 152525 keys, 8 key heads of 128:
+//                     110 us, 86% of the copy rate), by the latency of a tile with short
+//                     prompts (64 of 5 to 77 tokens, 12 heads of 64: 17.7 us).
 // A score's modifications (MOD bit 0: cap tanh(z / cap), bit 1: minus slope x distance) are
 // applied between the TMEM load and the maximum. Masks are row limits: row r sees keys
 // j < lim = min(kv_len, max(p + 1, prefix)).
@@ -1173,9 +1180,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // The pieces of the rows that k_ragged_streams cut, joined: W warps per row (sequence, token,
 // head), each for every W-th piece. Which workers hold them follows from the step list alone;
-// rows that one worker finished are already in out. A warp waits about 0.25 us for a piece (four
-// loads in flight), so one row of 100 pieces takes 26 us with one warp; with eight to a row, a
-// launch of many rows would leave most of them idle.
+// rows that one worker finished are already in out. With one warp a row of many pieces is a
+// chain of loads: a query over 12828 keys (101 pieces) took 39 us in all, 15 with eight warps to
+// a row; for many rows of few pieces eight would mostly idle.
 template <class T, int W>
 __global__ void __launch_bounds__(256) k_ragged_join(const __grid_constant__ TcParams p, int workers) {
   __shared__ StepList steps;

@@ -24,8 +24,10 @@ constexpr int kMaxRowsSmall = 128;  // rows of a block of k_lora_rows
 // The adapter term rides on the same tensor-core product as W: next to the K blocks of X and
 // W, an accumulator runs through the chunks of H and B, where H holds h in the columns of the
 // row's own adapter and zeros in those of the other adapters among the rows it is multiplied with.
-// A chunk is cw = 16, 32 or 64 ranks of one adapter; for an fp32 output h is kept in two bf16
-// parts, high and low, and each chunk has one of either.
+// A chunk is cw = 16, 32 or 64 ranks of one adapter. For a bf16 output h is rounded to bf16: 2^-8
+// of each of its terms, at most what the output's own rounding may cost if the adapter's part is no
+// larger than the output. For an fp32 output h is kept in two bf16 parts, high and low, and each
+// chunk has one of either.
 // K-major operand rows of `pitch` = 32, 64 or 128 bytes in the swizzle of that width.
 __device__ __forceinline__ uint64_t sdesc_k(uint32_t saddr, int pitch) {
   uint64_t d = 0;
@@ -168,7 +170,9 @@ __device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int6
 // The rows are the N of one MMA tile: D[n, t] = sum_k W[n, k] x[t, k] (+ the chunks of B and
 // H) on tcgen05, 128 rows of W (the M of the MMA) per cluster. K blocks and chunks are split
 // over the cluster's CTAs, so that every processor streams W; the CTAs' partial sums are read
-// from their shared memory in rank order (the result does not depend on timing).
+// from their shared memory in rank order (the result does not depend on timing). Bound by the
+// reads of W and the latency of the K loops: 48 rows, 9728 x 2560, 32 adapters of rank 32, 26.7 us
+// with k_lora_down_rows (2.8 TB/s); one row, 2560 x 2560, 8.4 us.
 template <int TN>
 struct RowsCfg {
   static constexpr int W_BYTES = 128 * 128, X_BYTES = TN * 128, STAGE = W_BYTES + X_BYTES;
@@ -738,8 +742,9 @@ __device__ __noinline__ void redo_chunk(const LoraLinear& p, const LoraK& lk, co
 // the chunks of H and B, 64 / cw of them a stage. Every unit runs its items of the first kind
 // before those of the second, only the second kind waits, and a cooperative launch has all units
 // resident, so the wait ends. In a kernel of its
-// own the adapter product cost a pass over X that nothing overlapped: 827 instead of
-// us at 33792 x 3840 x 3840 with one adapter of rank 16 (640 without).
+// own the adapter product cost a pass over X that nothing overlapped: 827 us at 33792 x 3840 x
+// 3840 with one adapter of rank 16, now 692 (634 without adapters; 1440 TFLOP/s, torch.matmul 650).
+// Bound by the tensor core under the power limit there, by the epilogue where K <= 400.
 template <int BN, bool PAIR>
 struct LoraGemmCfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;

@@ -198,6 +198,9 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
   }
 }
 
+// Bound by memory: 33792 tokens of 60 heads of 128, fp32 in, fp16 out, 242 us, 98% of the copy
+// rate; 2397 tokens of 40 heads, bf16, 12.6 us, a single wave of blocks. The kernel for any shape
+// takes 1038 and 51 us.
 template <class TI, class TO, int VE, bool INTER>
 __global__ void __launch_bounds__(kThreads, 5) k_qk_norm_rope(const QkNormRope p, int lg, int parts, int part_heads) {
   const int lane = threadIdx.x & 31, in = lane & ((1 << lg) - 1);
