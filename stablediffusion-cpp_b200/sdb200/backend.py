@@ -229,16 +229,34 @@ def conv2d(x, w, bias, stride, pad):
 # ---------------------------------------------------------------------------------
 # Several requests at once: adapters, per-head norms with the rotation, ragged attention
 # ---------------------------------------------------------------------------------
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
-_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_calls = None
+
+
+def _serving():
+    """The compiled calls (binding/serving_py.cpp), bound to the library's functions."""
+    global _calls
+    if _calls is None:
+        import ctypes
+        import os
+
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_serving.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"_serving.so not built at {path}; run `make -C stablediffusion-cpp_b200`")
+        from . import _serving as module
+
+        L = lib()
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            L.sdb200_set_stream, L.sdb200_qk_norm_rope, L.sdb200_linear_lora_workspace, L.sdb200_linear_lora,
+            L.sdb200_attention_ragged_workspace, L.sdb200_attention_ragged)))
+        _calls = module
+    return _calls
 
 
 def _refuse_args(op, like, **tensors):
     """Names what is wrong with the tensors, (tensor, dtype, shape or None) by name: all on
-    like's device, which must be the current one, and contiguous where a shape is given. The
-    operators below test all of it in one expression and come here only when it fails: at one
-    token a call's GPU time is that of a few tensor checks."""
+    like's device, which must be the current one, and contiguous where a shape is given."""
     if not like.is_cuda or like.device.index != torch.cuda.current_device():
         raise ValueError(f"{op}: tensors must be on the current CUDA device, got {like.device}")
     for name, (t, dtype, shape) in tensors.items():
@@ -252,40 +270,28 @@ def _refuse_args(op, like, **tensors):
             raise ValueError(f"{op}: {name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
 
 
-_lora_bytes, _attention_bytes = {}, {}  # workspace sizes by argument sizes
+def _refuse_heads(op, **tensors):
+    for name, t in tensors.items():
+        if t is not None:
+            _, h, d = t.shape
+            _, head, one = t.stride()
+            if (one != 1 and d > 1) or (head != d and h > 1):
+                raise ValueError(f"{op}: the heads of {name} must be dense within a row")
 
 
-def _remember(sizes, key, need):
-    if need >= 0:  # -1: the operator itself says what is wrong
-        if len(sizes) >= 4096:
-            sizes.clear()
-        sizes[key] = need
+def _refuse_rows(op, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.stride(1) != 1 and t.shape[1] > 1:
+            raise ValueError(f"{op}: the rows of {name} must be dense")
 
 
-def _head_pitch(op, name, t):
-    """Row pitch (elements) of [T, heads, d] whose heads lie next to each other."""
-    T, h, d = t.shape
-    row, head, one = t.stride()
-    if (one != 1 and d > 1) or (head != d and h > 1):
-        raise ValueError(f"{op}: the heads of {name} must be dense within a row")
-    return row if T > 1 else h * d
-
-
-def _row_pitch(op, name, t):
-    rows, cols = t.shape
-    row, one = t.stride()
-    if one != 1 and cols > 1:
-        raise ValueError(f"{op}: the rows of {name} must be dense")
-    return row if rows > 1 else cols
-
-
-def _stack_pitch(op, name, t):
-    n, rows, cols = t.shape
-    s0, s1, s2 = t.stride()
-    ld = s1 if rows > 1 else s0 if n > 1 else cols
-    if (s2 != 1 and cols > 1) or (n > 1 and s0 != rows * ld):
-        raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
-    return ld
+def _refuse_stacks(op, **tensors):
+    for name, t in tensors.items():
+        n, rows, cols = t.shape
+        s0, s1, s2 = t.stride()
+        ld = s1 if rows > 1 else s0 if n > 1 else cols
+        if (s2 != 1 and cols > 1) or (n > 1 and s0 != rows * ld):
+            raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
 
 
 def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleaved=False, out_dtype=None, q_out=None,
@@ -294,68 +300,43 @@ def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleav
     be strided, as views of a fused projection); cos / sin [n_pos, rot] fp32 with rot <= d,
     row pos[t] (int32), or t % n_pos without pos. Returns (q, k) in out_dtype (default: as
     given), or in q_out / k_out, which may be q / k themselves. k may be None."""
-    op = "qk_norm_rope"
-    dtype, dev = q.dtype, q.get_device()
+    r = (_calls or _serving()).qk_norm_rope(q, k, cos, sin, gq, gk, eps, pos, interleaved, out_dtype, q_out, k_out)
+    if r.__class__ is tuple:
+        return r
+    if r is not None:
+        check(r)
+    op, dtype = "qk_norm_rope", q.dtype
     if dtype not in _TYPES or q.dim() != 3:
         raise TypeError(f"{op}: q must be [T, heads, d] fp32, bf16 or fp16, got {dtype} {tuple(q.shape)}")
-    T, heads, d = q.shape
+    T, _, d = q.shape
     out_dtype = out_dtype or (q_out.dtype if q_out is not None else dtype)
     if out_dtype not in _TYPES:
         raise TypeError(f"{op}: output type {out_dtype}")
-    table = cos.shape
-    if len(table) != 2:
+    if cos.dim() != 2:
         raise ValueError(f"{op}: cos must be [n_pos, rot]")
-    if not (0 <= dev == _current() and cos.dtype is _F32 and cos.get_device() == dev and cos.is_contiguous()
-            and sin.dtype is _F32 and sin.get_device() == dev and sin.shape == table and sin.is_contiguous()
-            and (gq is None or (gq.dtype is _F32 and gq.get_device() == dev and gq.shape == (d,) and gq.is_contiguous()))
-            and (gk is None or (gk.dtype is _F32 and gk.get_device() == dev and gk.shape == (d,) and gk.is_contiguous()))
-            and (pos is None or (pos.dtype is _I32 and pos.get_device() == dev and pos.shape == (T,)
-                                 and pos.is_contiguous()))
-            and (k is None or (k.dtype is dtype and k.get_device() == dev))
-            and (q_out is None or (q_out.dtype is out_dtype and q_out.get_device() == dev))
-            and (k_out is None or (k_out.dtype is out_dtype and k_out.get_device() == dev))):
-        _refuse_args(op, q, k=(k, dtype, None), cos=(cos, _F32, table), sin=(sin, _F32, table), gq=(gq, _F32, (d,)),
-                     gk=(gk, _F32, (d,)), pos=(pos, _I32, (T,)), q_out=(q_out, out_dtype, None),
-                     k_out=(k_out, out_dtype, None))
-    ldqo, kv, ldk, ldko, kp, kop = heads * d, 0, 0, 0, None, None
-    if q_out is None:
-        q_out = q.new_empty((T, heads, d), dtype=out_dtype)
-    else:
-        if q_out.shape != q.shape:
-            raise ValueError(f"{op}: q_out must have the shape of q")
-        ldqo = _head_pitch(op, "q_out", q_out)
-    if k is None:
-        k_out = None
-    else:
-        if k.dim() != 3 or k.shape[0] != T or k.shape[2] != d:
-            raise ValueError(f"{op}: k must be [{T}, kv_heads, {d}], got {tuple(k.shape)}")
-        kv = k.shape[1]
-        ldk, ldko = _head_pitch(op, "k", k), kv * d
-        if k_out is None:
-            k_out = q.new_empty((T, kv, d), dtype=out_dtype)
-        else:
-            if k_out.shape != k.shape:
-                raise ValueError(f"{op}: k_out must have the shape of k")
-            ldko = _head_pitch(op, "k_out", k_out)
-        kp, kop = k.data_ptr(), k_out.data_ptr()
-    L = lib()
-    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_qk_norm_rope(
-        T, q.data_ptr(), _head_pitch(op, "q", q), heads, kp, ldk, kv, _TYPES[dtype], d, table[1],
-        None if gq is None else gq.data_ptr(), None if gk is None else gk.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(),
-        table[0], None if pos is None else pos.data_ptr(), 1 if interleaved else 0, q_out.data_ptr(), ldqo, kop, ldko,
-        _TYPES[out_dtype])
-    if rc:
-        check(rc)
-    return q_out, k_out
+    _refuse_args(op, q, k=(k, dtype, None), cos=(cos, _F32, cos.shape), sin=(sin, _F32, cos.shape), gq=(gq, _F32, (d,)),
+                 gk=(gk, _F32, (d,)), pos=(pos, _I32, (T,)), q_out=(q_out, out_dtype, None), k_out=(k_out, out_dtype, None))
+    if k is not None and (k.dim() != 3 or k.shape[0] != T or k.shape[2] != d):
+        raise ValueError(f"{op}: k must be [{T}, kv_heads, {d}], got {tuple(k.shape)}")
+    if q_out is not None and q_out.shape != q.shape:
+        raise ValueError(f"{op}: q_out must have the shape of q")
+    if k is not None and k_out is not None and k_out.shape != k.shape:
+        raise ValueError(f"{op}: k_out must have the shape of k")
+    _refuse_heads(op, q=q, k=k, q_out=q_out, k_out=k_out)
+    raise TypeError(f"{op}: an argument is not of its kind")
 
 
 def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32, out=None):
     """x W^T (+ bias) + scale[a] (x A[a]^T) B[a]^T with a = rows[t] for row t (int32, < 0: no
     adapter). x [T, K] bf16 or fp32 (rounded to bf16), W [N, K], A [n, r, K], B [n, N, r] bf16,
     scale [n] and bias [N] fp32. Returns [T, N] in out_dtype (fp32 or bf16), or out."""
+    r = (_calls or _serving()).linear_lora(x, W, A, B, rows, scale, bias, out_dtype, out)
+    if r is not None and r.__class__ is not int:
+        return r
+    if r is not None:
+        check(r)
     op = "linear_lora"
-    dtype, dev = x.dtype, x.get_device()
-    if dtype not in (_F32, _BF16) or x.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
+    if x.dtype not in (_F32, _BF16) or x.dim() != 2 or W.dim() != 2 or A.dim() != 3 or B.dim() != 3:
         raise TypeError(f"{op}: x [T, K] fp32 or bf16, W [N, K], A [n, r, K], B [n, N, r]")
     T, K = x.shape
     N, (n, r, Ka) = W.shape[0], A.shape
@@ -365,40 +346,13 @@ def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32
         out_dtype = out.dtype
     if out_dtype not in (_F32, _BF16):
         raise TypeError(f"{op}: output type {out_dtype}")
-    if not (0 <= dev == _current() and W.dtype is _BF16 and A.dtype is _BF16 and B.dtype is _BF16 and W.get_device() == dev
-            and A.get_device() == dev and B.get_device() == dev and rows.dtype is _I32 and rows.get_device() == dev
-            and rows.shape == (T,) and rows.is_contiguous()
-            and (scale is None or (scale.dtype is _F32 and scale.get_device() == dev and scale.shape == (n,)
-                                   and scale.is_contiguous()))
-            and (bias is None or (bias.dtype is _F32 and bias.get_device() == dev and bias.shape == (N,)
-                                  and bias.is_contiguous()))
-            and (out is None or out.get_device() == dev)):
-        _refuse_args(op, x, W=(W, _BF16, None), A=(A, _BF16, None), B=(B, _BF16, None), rows=(rows, _I32, (T,)),
-                     scale=(scale, _F32, (n,)), bias=(bias, _F32, (N,)), out=(out, out_dtype, None))
-    if out is None:
-        out, ldy = x.new_empty((T, N), dtype=out_dtype), N
-    else:
-        if out.shape != (T, N):
-            raise ValueError(f"{op}: out must be [{T}, {N}]")
-        ldy = _row_pitch(op, "out", out)
-    px, pw, pa, pb = x.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr()
-    ldx, ldw, lda, ldb = _row_pitch(op, "x", x), _row_pitch(op, "W", W), _stack_pitch(op, "A", A), _stack_pitch(op, "B", B)
-    bf = 1 if dtype is _BF16 else 0
-    L = lib()
-    # The workspace follows from sizes, pitches and alignment alone.
-    key = (T, N, K, n, r, ldx, ldw, lda, ldb, bf, px & 15, pw & 15, pa & 15, pb & 15, dev)
-    need = _lora_bytes.get(key)
-    if need is None:
-        need = L.sdb200_linear_lora_workspace(T, N, K, px, ldx, bf, pw, ldw, n, r, pa, lda, pb, ldb)
-        _remember(_lora_bytes, key, need)
-    ws = x.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_linear_lora(
-        T, N, K, px, ldx, bf, pw, ldw, None if bias is None else bias.data_ptr(), rows.data_ptr(), n, r, pa, lda, pb, ldb,
-        None if scale is None else scale.data_ptr(), out.data_ptr(), ldy, 1 if out_dtype is _BF16 else 0,
-        None if ws is None else ws.data_ptr(), need)
-    if rc:
-        check(rc)
-    return out
+    _refuse_args(op, x, W=(W, _BF16, None), A=(A, _BF16, None), B=(B, _BF16, None), rows=(rows, _I32, (T,)),
+                 scale=(scale, _F32, (n,)), bias=(bias, _F32, (N,)), out=(out, out_dtype, None))
+    if out is not None and out.shape != (T, N):
+        raise ValueError(f"{op}: out must be [{T}, {N}]")
+    _refuse_rows(op, x=x, W=W, out=out)
+    _refuse_stacks(op, A=A, B=B)
+    raise TypeError(f"{op}: an argument is not of its kind")
 
 
 def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, scale=None, causal=False, prefix=None,
@@ -410,55 +364,28 @@ def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, s
     prefix[s]; cap > 0 turns a score z into cap tanh(z / cap); slopes [heads] subtract
     slope * distance. scale defaults to 1 / sqrt(d). Returns out [Tq, heads, d] in out_dtype
     (bf16 or fp16, default as q); rows of no sequence keep what out held (zeros without out)."""
-    op = "attention_ragged"
-    dtype, dev = q.dtype, q.get_device()
+    r = (_calls or _serving()).attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, scale, causal,
+                                                prefix, cap, slopes, out_dtype, out)
+    if r is not None and r.__class__ is not int:
+        return r
+    if r is not None:
+        check(r)
+    op, dtype = "attention_ragged", q.dtype
     if dtype not in (_BF16, torch.float16) or q.dim() != 3 or k.dim() != 3:
         raise TypeError(f"{op}: q, k, v must be [T, heads, d] bf16 or fp16, got {dtype}")
-    (Tq, heads, d), (Tkv, kv_heads, dk) = q.shape, k.shape
-    if dk != d or v.shape != k.shape:
+    if k.shape[2] != q.shape[2] or v.shape != k.shape:
         raise ValueError(f"{op}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     out_dtype = out.dtype if out is not None else (out_dtype or dtype)
     if out_dtype not in (_BF16, torch.float16):
         raise TypeError(f"{op}: output type {out_dtype}")
-    n = q_begin.numel()
-    one = (n,)
-    if not (0 <= dev == _current() and k.dtype is dtype and v.dtype is dtype and k.get_device() == dev
-            and v.get_device() == dev
-            and q_begin.dtype is _I32 and q_begin.get_device() == dev and q_begin.shape == one and q_begin.is_contiguous()
-            and q_len.dtype is _I32 and q_len.get_device() == dev and q_len.shape == one and q_len.is_contiguous()
-            and kv_begin.dtype is _I32 and kv_begin.get_device() == dev and kv_begin.shape == one
-            and kv_begin.is_contiguous()
-            and kv_len.dtype is _I32 and kv_len.get_device() == dev and kv_len.shape == one and kv_len.is_contiguous()
-            and (prefix is None or (prefix.dtype is _I32 and prefix.get_device() == dev and prefix.shape == one
-                                    and prefix.is_contiguous()))
-            and (slopes is None or (slopes.dtype is _F32 and slopes.get_device() == dev and slopes.shape == (heads,)
-                                    and slopes.is_contiguous())) and (out is None or out.get_device() == dev)):
-        _refuse_args(op, q, k=(k, dtype, None), v=(v, dtype, None), q_begin=(q_begin, _I32, one), q_len=(q_len, _I32, one),
-                     kv_begin=(kv_begin, _I32, one), kv_len=(kv_len, _I32, one), prefix=(prefix, _I32, one),
-                     slopes=(slopes, _F32, (heads,)), out=(out, out_dtype, None))
-    if out is None:
-        out, ldo = q.new_zeros((Tq, heads, d), dtype=out_dtype), heads * d
-    else:
-        if out.shape != q.shape:
-            raise ValueError(f"{op}: out must have the shape of q")
-        ldo = _head_pitch(op, "out", out)
-    L = lib()
-    max_q, max_kv = min(max_q, Tq), min(max_kv, Tkv)
-    key = (n, max_q, max_kv, heads, kv_heads, d, dev)
-    need = _attention_bytes.get(key)
-    if need is None:
-        need = L.sdb200_attention_ragged_workspace(n, max_q, max_kv, heads, kv_heads, d)
-        _remember(_attention_bytes, key, need)
-    ws = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    rc = L.sdb200_set_stream(_raw_stream(dev)) or L.sdb200_attention_ragged(
-        q.data_ptr(), _head_pitch(op, "q", q), k.data_ptr(), _head_pitch(op, "k", k), v.data_ptr(),
-        _head_pitch(op, "v", v), _TYPES[dtype], out.data_ptr(), ldo, _TYPES[out_dtype], Tq, Tkv, n, q_begin.data_ptr(),
-        q_len.data_ptr(), kv_begin.data_ptr(), kv_len.data_ptr(), max_q, max_kv, heads, kv_heads, d,
-        d ** -0.5 if scale is None else scale, cap, None if slopes is None else slopes.data_ptr(), 1 if causal else 0,
-        None if prefix is None else prefix.data_ptr(), None if ws is None else ws.data_ptr(), need)
-    if rc:
-        check(rc)
-    return out
+    one = (q_begin.numel(),)
+    _refuse_args(op, q, k=(k, dtype, None), v=(v, dtype, None), q_begin=(q_begin, _I32, one), q_len=(q_len, _I32, one),
+                 kv_begin=(kv_begin, _I32, one), kv_len=(kv_len, _I32, one), prefix=(prefix, _I32, one),
+                 slopes=(slopes, _F32, (q.shape[1],)), out=(out, out_dtype, None))
+    if out is not None and out.shape != q.shape:
+        raise ValueError(f"{op}: out must have the shape of q")
+    _refuse_heads(op, q=q, k=k, v=v, out=out)
+    raise TypeError(f"{op}: an argument is not of its kind")
 
 
 def mul_rows_(x, v):

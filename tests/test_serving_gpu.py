@@ -739,6 +739,83 @@ def test_linear_lora_beside_its_input(sdb, T):
     lora_close(buf[:, 64:], x, W, A, B, rows, scale, bias)
 
 
+def test_wrappers_name_what_does_not_fit(sdb):
+    be, g = sdb.backend, gen(31)
+    q, cos = randn(g, 4, 2, 8, dtype=BF16), randn(g, 4, 8)
+    pos = torch.zeros(4, device="cuda", dtype=torch.int32)
+
+    def refused(text, kind, f, *a, **kw):
+        with pytest.raises(kind, match=text):
+            f(*a, **kw)
+
+    for kw, text, kind in (
+            (dict(cos=cos.half()), "cos must be", TypeError), (dict(sin=cos[:3]), "sin must be", ValueError),
+            (dict(cos=cos.cpu()), "cos is on", ValueError), (dict(gq=cos[0, :7]), "gq must be", ValueError),
+            (dict(pos=pos.long()), "pos must be", TypeError), (dict(pos=pos[:3]), "pos must be", ValueError),
+            (dict(k=q.float()), "k must be", TypeError), (dict(k=q[:3]), "k must be", ValueError),
+            (dict(q=q[..., ::2]), "heads of q must be dense", ValueError), (dict(out_dtype=torch.int8), "output type", TypeError),
+            (dict(q_out=q.float()[:, :1].to(BF16)), "shape of q", ValueError), (dict(q_out=q.cpu()), "q_out is on", ValueError),
+            (dict(cos=cos[:, :7].contiguous(), sin=cos[:, :7].contiguous()), "rot must be even", sdb.SdbError),
+            (dict(eps="x"), "not of its kind", TypeError)):
+        a = dict(q=q, k=q, cos=cos, sin=cos)
+        a.update(kw)
+        if "q" in kw:
+            a.update(k=None, cos=cos[:, :4].contiguous(), sin=cos[:, :4].contiguous())
+        refused(text, kind, be.qk_norm_rope, **a)
+    x, W, A, B = randn(g, 4, 16, dtype=BF16), randn(g, 8, 16, dtype=BF16), randn(g, 2, 4, 16, dtype=BF16), randn(g, 2, 8, 4, dtype=BF16)
+    for kw, text, kind in (
+            (dict(W=W.float()), "W must be", TypeError), (dict(W=W[:, :15]), "shapes", ValueError),
+            (dict(rows=pos[:2]), "rows must be", ValueError), (dict(rows=pos.cpu()), "rows is on", ValueError),
+            (dict(bias=cos[0, :7]), "bias must be", ValueError), (dict(scale=cos[0]), "scale must be", ValueError),
+            (dict(out_dtype=F16), "output type", TypeError), (dict(out=cos[:, :7]), "out must be", ValueError),
+            (dict(x=randn(g, 16, 4, dtype=BF16).t()), "rows of x must be dense", ValueError),
+            (dict(A=randn(g, 4, 2, 16, dtype=BF16).transpose(0, 1)), "adapters of A", ValueError)):
+        a = dict(x=x, W=W, A=A, B=B, rows=pos)
+        a.update(kw)
+        refused(text, kind, be.linear_lora, **a)
+    one = torch.ones(1, device="cuda", dtype=torch.int32)
+    for kw, text, kind in (
+            (dict(k=q.half()), "k must be", TypeError), (dict(v=q[:, :1]), "shapes", ValueError),
+            (dict(q_len=one.long()), "q_len must be", TypeError), (dict(kv_len=pos), "kv_len must be", ValueError),
+            (dict(prefix=one), "prefix needs", sdb.SdbError), (dict(slopes=cos[0]), "slopes must be", ValueError),
+            (dict(out=q[:3]), "shape of q", ValueError), (dict(out_dtype=F32), "output type", TypeError),
+            (dict(out=q), "out overlaps", sdb.SdbError), (dict(max_q=-1), "bad shape", sdb.SdbError),
+            (dict(scale=0.0), "scale must be", sdb.SdbError)):
+        a = dict(q=q, k=q, v=q, q_begin=one * 0, q_len=one * 4, kv_begin=one * 0, kv_len=one * 4, max_q=4, max_kv=4)
+        a.update(kw)
+        refused(text, kind, be.attention_ragged, **a)
+    sdb.backend.synchronize()
+
+
+def test_calls_of_two_threads_go_to_their_own_streams(sdb):
+    """A thread's call runs on its current stream, also while another thread calls."""
+    import threading
+
+    inputs = [layer_inputs([200, 3, 77], 11), layer_inputs([1, 1, 400], 12)]
+    want = [layer(sdb, **s).clone() for s in inputs]
+    torch.cuda.synchronize()
+    got, wrong = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i].append(layer(sdb, **inputs[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - shown below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
+    sdb.backend.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
 def test_the_three_repeat_exactly(sdb):
     s = layer_inputs([333, 1, 64], 5)
     a = layer(sdb, **s)
