@@ -153,8 +153,13 @@ int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void
                                      int64_t lda, const uint16_t* B, int64_t ldb) {
   try {
     if (T <= 0 || N <= 0) return 0;
-    return (int64_t)lora_linear_workspace(lora_args(T, N, K, X, ldx, x_bf16, W, ldw, nullptr, nullptr, n_adapters, r,
-                                                    A, lda, B, ldb, nullptr, nullptr, N, 0));
+    // For either type of Y: an fp32 one has more chunks to a group of rows and so fewer groups at a
+    // time, a bf16 one longer lists.
+    size_t need = 0;
+    for (int y_bf16 = 0; y_bf16 < 2; ++y_bf16)
+      need = std::max(need, lora_linear_workspace(lora_args(T, N, K, X, ldx, x_bf16, W, ldw, nullptr, nullptr, n_adapters, r,
+                                                            A, lda, B, ldb, nullptr, nullptr, N, y_bf16)));
+    return (int64_t)need;
   } catch (const sdb::Error& e) {
     sdb::set_last_error(e.msg);
     return -1;

@@ -706,6 +706,13 @@ def test_the_three_on_their_own_stream_and_in_graphs(sdb):
     sdb.backend.synchronize()
 
 
+@pytest.mark.parametrize("to", [BF16, F32])
+@pytest.mark.parametrize("T,n,r", [(9000, 64, 128), (20000, 40, 256), (3000, 200, 20)])
+def test_linear_lora_of_many_adapters_and_rows(sdb, T, n, r, to):
+    """H of all rows at once would pass its share of the workspace, so that blocks of rows go one after another."""
+    test_linear_lora(sdb, (T, 40, 64, r, n, "random", BF16, to, True, True))
+
+
 def test_linear_lora_on_two_streams_at_once(sdb):
     """Calls whose processors wait for one another's h, on streams of different priorities."""
     g = gen(23)
