@@ -91,7 +91,7 @@ struct Chunk {
   }
 };
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 64;
 
 // `n` heads of one token starting at x, a group of 2^lg lanes per head. A lane holds two
 // chunks of VE channels, at c0 and c1, that form whole pairs: the two halves of a rotation
@@ -199,10 +199,10 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
 }
 
 // Bound by memory: 33792 tokens of 60 heads of 128, fp32 in, fp16 out, 242 us, 98% of the copy
-// rate; 2397 tokens of 40 heads, bf16, 12.6 us, a single wave of blocks. The kernel for any shape
+// rate; 2397 tokens of 40 heads, bf16, 11.1 us, a single wave of blocks. The kernel for any shape
 // takes 1038 and 51 us.
 template <class TI, class TO, int VE, bool INTER>
-__global__ void __launch_bounds__(kThreads, 5) k_qk_norm_rope(const QkNormRope p, int lg, int parts, int part_heads) {
+__global__ void __launch_bounds__(kThreads, 10) k_qk_norm_rope(const QkNormRope p, int lg, int parts, int part_heads) {
   const int lane = threadIdx.x & 31, in = lane & ((1 << lg) - 1);
   // Groups of one warp take consecutive tokens of the same part of the heads.
   const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
@@ -264,9 +264,11 @@ void launch_chunks(const QkNormRope& p) {
   int lg = 0;
   while ((2 << lg) * VE < p.d) ++lg;
   const int64_t warps = (p.T + (32 >> lg) - 1) / (32 >> lg);
-  // A warp runs through all heads of its tokens with one set of table values; where that
-  // leaves fewer than the 20 warps a processor that fit, through fewer.
-  const int64_t want = (int64_t)ctx().num_sms * 20;
+  // A warp runs through all heads of its tokens with one set of table values; where that leaves
+  // fewer than ten warps a processor, half of what fit, through fewer. 2397 tokens of 40 heads,
+  // bf16: 11.1 us; 12.7 if filled up to twenty, which makes every set serve half as many heads,
+  // 14.6 with seven.
+  const int64_t want = (int64_t)ctx().num_sms * 10;
   int part_heads = nh;
   while (part_heads > 1 && warps * ((nh + part_heads - 1) / part_heads) < want) part_heads = (part_heads + 1) / 2;
   const int parts = (nh + part_heads - 1) / part_heads;
