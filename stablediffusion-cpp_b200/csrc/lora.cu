@@ -19,6 +19,7 @@ inline int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 inline size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+constexpr int kMaxSmem = 232448;
 constexpr int kMaxRowsSmall = 128;  // rows of a block of k_lora_rows
 
 // The adapter term rides on the same tensor-core product as W: next to the K blocks of X and
@@ -171,8 +172,8 @@ __device__ __noinline__ float redo_value(const LoraRows& g, const int* ids, int6
 // H) on tcgen05, 128 rows of W (the M of the MMA) per cluster. K blocks and chunks are split
 // over the cluster's CTAs, so that every processor streams W; the CTAs' partial sums are read
 // from their shared memory in rank order (the result does not depend on timing). Bound by the
-// reads of W and the latency of the K loops: 48 rows, 9728 x 2560, 32 adapters of rank 32, 26.7 us
-// with k_lora_down_rows (2.8 TB/s); one row, 2560 x 2560, 8.4 us.
+// reads of W and the latency of the K loops: 48 rows, 9728 x 2560, 32 adapters of rank 32, 25.7 us
+// with k_lora_down_rows (2.9 TB/s); one row, 2560 x 2560, 8.4 us.
 template <int TN>
 struct RowsCfg {
   static constexpr int W_BYTES = 128 * 128, X_BYTES = TN * 128, STAGE = W_BYTES + X_BYTES;
@@ -502,11 +503,46 @@ __global__ void __launch_bounds__(256) k_lora_pack(const __grid_constant__ PackA
   }
 }
 
-// K splits of k_lora_rows, until two CTAs a processor have a part, of two K blocks at least.
+// CTAs of k_lora_rows that run at a time in clusters of `splits`: two a processor, but clusters of
+// four and eight leave some processors of a group out (132 and 120 of 148 have one). 296 CTAs in
+// clusters of four ran in two waves: 48 rows, 9472 x 2560, 33 us instead of 25.6.
+template <int TN>
+int64_t row_units(int splits) {
+  static int64_t units[64][9] = {};
+  DeviceContext& c = ctx();
+  if (!units[c.device][splits]) {
+    using C_ = RowsCfg<TN>;
+    constexpr int kOne = 120 * 1024;  // shared memory that one CTA a processor has, for the query
+    static_assert(C_::SMEM <= kOne && 2 * (C_::SMEM + 8192) <= kMaxSmem, "two CTAs a processor");
+    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kOne),
+               "cudaFuncSetAttribute(linear_lora)");
+    // The default carve-out would hold one CTA a processor, and the rest would run after it.
+    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                    cudaSharedmemCarveoutMaxShared),
+               "cudaFuncSetAttribute(linear_lora)");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)splits);
+    cfg.blockDim = dim3(64 + kSumThreads);
+    cfg.dynamicSmemBytes = kOne;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    check_cuda(cudaOccupancyMaxActiveClusters(&fit, k_lora_rows<TN>, &cfg), "cudaOccupancyMaxActiveClusters(linear_lora)");
+    units[c.device][splits] = std::max<int64_t>(1, 2 * (int64_t)fit * splits);
+  }
+  return units[c.device][splits];
+}
+// K splits of k_lora_rows, while all CTAs run at a time, of two K blocks at least.
+template <int TN>
 int row_splits(const LoraLinear& p) {
   const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall), kblocks = (p.K + 63) / 64;
   int splits = 1;
-  while (splits < 8 && kblocks >= 4 * splits && tiles * splits * 2 <= (int64_t)ctx().num_sms * 2) splits *= 2;
+  while (splits < 8 && kblocks >= 4 * splits && tiles * splits * 2 <= row_units<TN>(splits * 2)) splits *= 2;
+  row_units<TN>(splits);  // the kernel's attributes are set
   return splits;
 }
 int rows_tile(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128; }
@@ -555,17 +591,7 @@ void launch_rows(LoraRows g) {
     tb = th = tx;  // no chunk is read
   }
   const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
-  g.splits = row_splits(p);
-  static bool done[64] = {};
-  if (!done[c.device]) {
-    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::SMEM),
-               "cudaFuncSetAttribute(linear_lora)");
-    // The default carve-out would hold one CTA a processor, and the rest would run after it.
-    check_cuda(cudaFuncSetAttribute(k_lora_rows<TN>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                    cudaSharedmemCarveoutMaxShared),
-               "cudaFuncSetAttribute(linear_lora)");
-    done[c.device] = true;
-  }
+  g.splits = row_splits<TN>(p);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(tiles * g.splits));
   cfg.blockDim = dim3(64 + kSumThreads);
@@ -586,7 +612,6 @@ void launch_rows(LoraRows g) {
 // ------------------------------------------------------------------------------------
 // Many rows: Y = [X | H] [W | B]^T as one GEMM.
 // ------------------------------------------------------------------------------------
-constexpr int kMaxSmem = 232448;
 constexpr int kGroup = 256;  // rows that share a list of adapters and a block of H
 constexpr int kHash = 512;
 
@@ -1362,10 +1387,10 @@ Tile choose_tile(int64_t rows, int64_t N, bool adapters) {
 bool few_rows(const LoraLinear& p) {
   if (p.T <= kMaxRowsSmall) return true;
   if (p.T > 1024 || p.n_adapters <= 0 || p.r <= 0) return false;
-  const int sms = ctx().num_sms, splits = row_splits(p);
+  const int sms = ctx().num_sms, splits = row_splits<kMaxRowsSmall>(p);
   const double kb = (double)((p.K + 63) / 64), t = (double)p.T;
   const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
-  const double rows = 12.0 + std::ceil((double)(tiles * splits) / (2 * sms)) * (kb / splits) * 0.6 +
+  const double rows = 12.0 + std::ceil((double)(tiles * splits) / (double)row_units<kMaxRowsSmall>(splits)) * (kb / splits) * 0.6 +
                       t * (double)p.r * (2.7e-4 + 1.5e-7 * (double)p.K);
   const Tile tile = choose_tile(p.T, p.N, true);
   const int64_t m = (p.T + tile.bm - 1) / tile.bm;
