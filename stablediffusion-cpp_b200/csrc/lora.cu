@@ -135,6 +135,83 @@ __global__ void __launch_bounds__(256) k_lora_down_rows(const LoraLinear p, cons
   }
 }
 
+// The same for four rows a CTA: rows of requests come in runs of one adapter, whose A is then
+// read once for up to four of them. (A template of both is slower for one row: the loop below
+// takes the registers that keep eight loads of the one above in flight.)
+constexpr int kRunRows = 4;
+__global__ void __launch_bounds__(256) k_lora_down_runs(const LoraLinear p, const uint16_t* __restrict__ X, int64_t ldx,
+                                                        const uint16_t* __restrict__ A, int64_t lda, RowsK rk) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int R = kRunRows, TN = kMaxRowsSmall;
+  static_assert(kMaxRowsSmall % R == 0, "a CTA's rows are of one block");
+  __shared__ int ids[kMaxRowsSmall];
+  __shared__ float sh[R][8];
+  const int64_t row0 = (int64_t)blockIdx.x * R / kMaxRowsSmall * kMaxRowsSmall;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = (int)((int64_t)blockIdx.x * R - row0);
+  const int T = (int)min(p.T - row0, (int64_t)kMaxRowsSmall), j = blockIdx.y * 8 + warp, n = min(R, T - t0);
+  if (threadIdx.x < T) {
+    const int a = p.row_adapter[row0 + threadIdx.x];
+    if (a >= p.n_adapters && threadIdx.x >= t0 && threadIdx.x < t0 + n && blockIdx.y == 0) atomicOr(p.err, kErrBadIndex);
+    ids[threadIdx.x] = a < p.n_adapters ? a : -1;
+  }
+  __syncthreads();
+  const int whole = (int)(p.K / 8);
+  for (int i0 = 0; i0 < n;) {
+    const int a = ids[t0 + i0];
+    int m = 1;
+    while (i0 + m < n && ids[t0 + i0 + m] == a) ++m;
+    if (a < 0 || j >= p.r) {
+      if (lane < m) sh[i0 + lane][warp] = 0.0f;
+    } else {
+      float2 s2[R];
+      const uint16_t* x[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        s2[i] = make_float2(0.0f, 0.0f);
+        x[i] = X + (row0 + t0 + i0 + min(i, m - 1)) * ldx;
+      }
+      const float scale = p.scale ? p.scale[a] : 1.0f;
+      const uint16_t* w = A + ((int64_t)a * p.r + j) * lda;
+#pragma unroll 4
+      for (int c = lane; c < whole; c += 32) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(w + 8 * c));
+#pragma unroll
+        for (int i = 0; i < R; ++i) {  // rows past m are the last one again: a test here would hold up the loads
+          const uint4 u = *reinterpret_cast<const uint4*>(x[i] + 8 * c);
+          s2[i] = ffma2(bf16x2_to_f32(u.x), bf16x2_to_f32(v.x), s2[i]);
+          s2[i] = ffma2(bf16x2_to_f32(u.y), bf16x2_to_f32(v.y), s2[i]);
+          s2[i] = ffma2(bf16x2_to_f32(u.z), bf16x2_to_f32(v.z), s2[i]);
+          s2[i] = ffma2(bf16x2_to_f32(u.w), bf16x2_to_f32(v.w), s2[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i >= m) break;
+        float s = s2[i].x + s2[i].y;
+        for (int k = whole * 8 + lane; k < p.K; k += 32) s = fmaf(bf16_to_f32(x[i][k]), bf16_to_f32(w[k]), s);
+        s = warp_add(s) * scale;
+        if (lane == 0) sh[i0 + i][warp] = s;
+      }
+    }
+    i0 += m;
+  }
+  __syncthreads();
+  if (threadIdx.x < T && is_first(ids, threadIdx.x)) {
+    const int j0 = blockIdx.y * 8, c = j0 / rk.cw;
+    for (int i = 0; i < n; ++i) {
+      const bool own = ids[threadIdx.x] == ids[t0 + i];
+      for (int part = 0; part < rk.parts; ++part) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (own)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e >> 1] |= h_part(sh[i][e], part) << (16 * (e & 1));
+        uint16_t* dst = rk.H + ((((row0 + threadIdx.x) * rk.parts + part) * rk.rc + c) * TN + t0 + i) * rk.cw + j0 % rk.cw;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+}
+
 struct LoraRows {
   LoraLinear p;
   RowsK rk;
@@ -535,6 +612,12 @@ int64_t row_units(int splits) {
     units[c.device][splits] = std::max<int64_t>(1, 2 * (int64_t)fit * splits);
   }
   return units[c.device][splits];
+}
+// Four rows to a CTA of the down product where that leaves every processor six: 384 rows of rank
+// 128, 3840 x 3840, 59 us instead of 71 with two requests, 77 instead of 81 with 64. With fewer
+// CTAs a chain of four rows is slower (160 rows of rank 16: 29 instead of 26).
+bool by_runs(const LoraLinear& p) {
+  return (p.T + kRunRows - 1) / kRunRows * (round_up(p.r, chunk_width(p.r)) / 8) >= 6 * (int64_t)ctx().num_sms;
 }
 // K splits of k_lora_rows, while all CTAs run at a time, of two K blocks at least.
 template <int TN>
@@ -1380,8 +1463,9 @@ Tile choose_tile(int64_t rows, int64_t N, bool adapters) {
 // Whether k_lora_rows, in blocks of 128 rows, takes fewer microseconds than the GEMM. The
 // GEMM's groups of 256 rows multiply every row with all adapters of the group, so requests of few
 // rows each cost it dearly: 129 rows, 3840 x 3840, rank 128, take 40 us with 2 requests, 144
-// with 16 and 506 with 64; k_lora_rows takes 38, 40 and 52, but 153 to 170 (42, 56 and 112)
-// for 1024 rows, because it reads an adapter anew for every row. How many adapters the rows
+// with 16 and 506 with 64; k_lora_rows takes 38, 40 and 52. With 512 rows the GEMM takes 38, 71
+// and 202 and k_lora_rows 70, 69 and 76, with 1024 the GEMM 40, 54 and 112 and k_lora_rows over
+// 100, because it reads an adapter for every row or every four. How many adapters the rows
 // use is known on the device only; a mixture of 16 is assumed, or all there are. The constants
 // are fitted to N, K from 224 to 10240, ranks 16 and 128, T from 129 to 1024.
 bool few_rows(const LoraLinear& p) {
@@ -1391,7 +1475,7 @@ bool few_rows(const LoraLinear& p) {
   const double kb = (double)((p.K + 63) / 64), t = (double)p.T;
   const int64_t tiles = (p.N + 127) / 128 * ((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
   const double rows = 12.0 + std::ceil((double)(tiles * splits) / (double)row_units<kMaxRowsSmall>(splits)) * (kb / splits) * 0.6 +
-                      t * (double)p.r * (2.7e-4 + 1.5e-7 * (double)p.K);
+                      t * (double)p.r * ((by_runs(p) ? 0.7e-4 : 2.7e-4) + 1.5e-7 * (double)p.K);
   const Tile tile = choose_tile(p.T, p.N, true);
   const int64_t m = (p.T + tile.bm - 1) / tile.bm;
   const double ksplit = std::max(1.0, std::min({8.0, (double)sms / (tile.bm / 128) / (double)m, kb / 2}));
@@ -1511,7 +1595,11 @@ void launch_lora_linear(LoraLinear p, void* ws_) {
   LoraRows g{p, lay_out_rows(p, ws + o.h_at, &h), X, W, B, ldx, ldw, ldb, 1};
   const int tn = rows_tile(p.T);
   if (g.rk.rc > 0) {
-    k_lora_down_rows<<<dim3((unsigned)p.T, (unsigned)(g.rk.rc * g.rk.cw / 8)), 256, 0, c.stream>>>(p, X, ldx, A, lda, g.rk, tn);
+    const unsigned eights = (unsigned)(g.rk.rc * g.rk.cw / 8);
+    if (by_runs(p))
+      k_lora_down_runs<<<dim3((unsigned)((p.T + kRunRows - 1) / kRunRows), eights), 256, 0, c.stream>>>(p, X, ldx, A, lda, g.rk);
+    else
+      k_lora_down_rows<<<dim3((unsigned)p.T, eights), 256, 0, c.stream>>>(p, X, ldx, A, lda, g.rk, tn);
     check_launch("lora_down_rows");
   }
   if (tn == 16) return launch_rows<16>(g);
