@@ -718,7 +718,6 @@ struct LoraK {
 
 // The distinct adapters of a group's rows, through a hash table.
 __global__ void __launch_bounds__(kGroup) k_lora_lists(const LoraLinear p, const LoraK lk, int64_t row0, int64_t rows) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int hash_key[kHash], hash_row[kHash], first_at[kGroup], in_warp[kGroup / 32], mixed;
   const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
   const int64_t t = (int64_t)blockIdx.x * kGroup + i;
@@ -943,7 +942,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any signal crosses
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // k_lora_lists
   // The list of tile row mb's group (without adapters there is none), its adapters and the
   // passes over them that make H.
   auto list_of = [&](int mb) { return g.lk.lists + (PAIR ? mb : mb >> 1); };
@@ -1398,7 +1396,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   static int clusters[64] = {};
   auto kern = k_lora_gemm<BN, PAIR>;
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[3] = {};
+  cudaLaunchAttribute attr[2] = {};
   int n = 0;
   if (PAIR) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
@@ -1421,11 +1419,9 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
     clusters[c.device] = fit;
   }
   if (overlap) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
     // Units wait for H that others make, so all must be resident: two such launches at once,
-    // each with a part of the processors, would wait for each other's.
+    // each with a part of the processors, would wait for each other's. (Starting beside
+    // k_lora_lists as well would save under 1 us, but the profiler fails on such a launch.)
     attr[n].id = cudaLaunchAttributeCooperative;
     attr[n].val.cooperative = 1;
     ++n;
