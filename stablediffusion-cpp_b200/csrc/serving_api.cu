@@ -152,6 +152,8 @@ int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void
                                      const uint16_t* W, int64_t ldw, int64_t n_adapters, int64_t r, const uint16_t* A,
                                      int64_t lda, const uint16_t* B, int64_t ldb) {
   try {
+    require(K > 0 && n_adapters >= 0 && r >= 0 && r <= 256 && std::max({T, N, K, n_adapters}) < kMaxRows - 512, "linear_lora",
+            "bad shape");
     if (T <= 0 || N <= 0) return 0;
     // For either type of Y: an fp32 one has more chunks to a group of rows and so fewer groups at a
     // time, a bf16 one longer lists.
@@ -162,6 +164,9 @@ int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void
     return (int64_t)need;
   } catch (const sdb::Error& e) {
     sdb::set_last_error(e.msg);
+    return -1;
+  } catch (const std::exception& e) {
+    sdb::set_last_error(e.what());
     return -1;
   }
 }
@@ -217,6 +222,9 @@ int64_t sdb200_attention_ragged_workspace(int n_seq, int64_t max_q, int64_t max_
     return (int64_t)ragged_attention_workspace(p);
   } catch (const sdb::Error& e) {
     sdb::set_last_error(e.msg);
+    return -1;
+  } catch (const std::exception& e) {
+    sdb::set_last_error(e.what());
     return -1;
   }
 }

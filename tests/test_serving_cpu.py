@@ -76,6 +76,13 @@ def test_linear_lora_refuses_shared_buffers_and_huge_ones(kw, text):
     refused(lora(**kw), text)
 
 
+@pytest.mark.parametrize("kw", [dict(K=0), dict(r=300), dict(n=-1), dict(T=1 << 40), dict(N=1 << 31)])
+def test_linear_lora_workspace_of_bad_shapes(kw):
+    a = dict(T=4, N=64, K=32, X=P, ldx=32, x_bf16=1, W=P, ldw=32, n=2, r=8, A=P, lda=32, B=P, ldb=8)
+    a.update(kw)
+    assert lib().sdb200_linear_lora_workspace(*a.values()) == -1
+
+
 def test_linear_lora_takes_columns_side_by_side():
     """X and Y may be columns of the same rows: only the missing workspace is refused here."""
     refused(lora(X=P2, ldx=96, Y=P2 + 64, ldy=96), "workspace of")
