@@ -122,7 +122,7 @@ __device__ __forceinline__ bool load_seq(const RaggedAttention& p, int s, Seq& q
 struct Row {
   int tok, head;  // token of the sequence, query head
   bool valid;
-  int lim;        // keys [0, lim) are seen
+  int lim;        // keys [0, lim) are seen (none by a row that is nobody's)
   float pos;      // position among the keys
   float nslope;   // -slope log2(e)
 };
@@ -133,8 +133,7 @@ __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, 
   w.head = kvh * p.G + (r - t * p.G);
   w.valid = t < p.tpt && w.tok < q.ql;
   const int pos = w.tok + q.kl - q.ql;
-  w.lim = q.kl;
-  if (p.a.causal) w.lim = min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0));
+  w.lim = !w.valid ? 0 : p.a.causal ? min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0)) : q.kl;
   w.pos = (float)pos;
   w.nslope = p.a.slopes && w.valid ? -p.a.slopes[w.head] * kLog2e : 0.0f;
   return w;
@@ -143,12 +142,14 @@ __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Two scores q.k to log2 units, MOD bit 0: capped. tanh(x) is x p(x^2) for |x| <= 1, p of
-// degree 5 fitted to tanh(sqrt(y)) / sqrt(y) on [0, 1] for the least maximal error (3.2e-7 in
-// fp32): eight packed multiply-adds a pair. A warp with a larger score (small = false) takes
-// 1 - 2 / (1 + e^2x), as exact (e^2x = inf gives 1), but two more MUFU operations a score
-// beside the exponential: that bounded the kernel (286 instead of 230 us on six documents of
-// 333 to 2500 tokens, 32 heads). tanh.approx is exact to 2^-11 only, which times a cap of 50
-// would be 2% of a probability.
+// degree 5, fitted so that x p(x^2) has the least maximal error: within 3.2e-7 of tanh(x) in
+// fp32 (p itself is 3.2e-6 below 1 at 0). Eight packed multiply-adds a pair. A row with a larger
+// score among those it sees of the tile (small = false) takes 1 - 2 / (1 + e^2x), as exact
+// (e^2x = inf gives 1), but two more MUFU operations a score beside the exponential: that
+// bounded the kernel (286 instead of 230 us on six documents of 333 to 2500 tokens, 32 heads).
+// The two differ in the last bits, so each row chooses by what it sees alone: hidden keys and
+// other rows, which may hold anything, do not reach its result. tanh.approx is exact to 2^-11
+// only, which times a cap of 50 would be 2% of a probability.
 template <int MOD>
 __device__ __forceinline__ float2 to_log2(const TcParams& p, float2 z, bool small) {
   if constexpr (!(MOD & 1)) {
@@ -181,6 +182,11 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
   if constexpr (MOD != 0) {
     bool small = true;
     if constexpr (MOD & 1) {
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < kBK; ++c)
+          if (c >= n_ok) u[c >> 5][c & 31] = 0;
+      }
       float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < kBK; c += 8)
@@ -188,7 +194,7 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
         for (int i = 0; i < 4; ++i)
           top[i] = fmax3(top[i], fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i])),
                          fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1])));
-      small = !__any_sync(0xffffffffu, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
+      small = n_ok <= 0 || !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
     }
     auto modify = [&](bool sm) {
 #pragma unroll
@@ -206,6 +212,7 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
       modify(true);
     else
       modify(false);
+    __syncwarp();
   }
   if (masked) {
 #pragma unroll
@@ -301,14 +308,18 @@ __device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_a
     if (h && !two) break;
     FewRow& r = row[h];
     auto at = [&](int i, int e) -> uint32_t& { return u[4 * i + 2 * h + e]; };
+    const int n_ok = r.lim - kbase - j2;
     bool small = true;
     if constexpr (MOD & 1) {
       float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmax3(top, fabsf(__uint_as_float(at(i, 0))), fabsf(__uint_as_float(at(i, 1))));
-      small = !__any_sync(0xffffffffu, top > p.cap_small);
+      for (int i = 0; i < 16; ++i) {
+        if (8 * i >= n_ok) at(i, 0) = 0;
+        if (8 * i + 1 >= n_ok) at(i, 1) = 0;
+        top = fmax3(top, fabsf(__uint_as_float(at(i, 0))), fabsf(__uint_as_float(at(i, 1))));
+      }
+      small = !(top > p.cap_small);
     }
-    const int n_ok = r.lim - kbase - j2;
     const float dist0 = r.pos - (float)(kbase + j2);
     float top = -INFINITY;
     auto modify = [&](bool sm) {
@@ -330,6 +341,7 @@ __device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_a
       modify(true);
     else
       modify(false);
+    __syncwarp();
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float m_new = fmaxf(r.m, top);
