@@ -245,8 +245,10 @@ int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const 
  * and no second term where a < 0. X [T, ldx] bf16 (x_bf16 != 0) or fp32 (rounded to bf16 as
  * gemm_nt_bf16 rounds it); W [N, ldw], A [n_adapters, r, lda], B [n_adapters, N, ldb] bf16;
  * scale fp32 [n_adapters] or null for 1; Y fp32 or bf16 (y_bf16), apart from the operands. r <= 256; adapters of
- * smaller rank are padded with zeros. Accumulation is fp32. ws: at least
- * sdb200_linear_lora_workspace() bytes for the same arguments. */
+ * smaller rank are padded with zeros. Sums are fp32. Between the two adapter products
+ * h_j = scale[a] sum_k X A_a[j] is rounded: to bf16 for a bf16 Y (up to 2^-8 sum_j |h_j B_a[n, j]| in Y[t, n],
+ * besides Y's own rounding), to 2^-16 for an fp32 Y, which is the one to ask for where adapter terms cancel.
+ * ws: at least sdb200_linear_lora_workspace() bytes for the same arguments. */
 int64_t sdb200_linear_lora_workspace(int64_t T, int64_t N, int64_t K, const void* X, int64_t ldx, int x_bf16,
                                      const uint16_t* W, int64_t ldw, int64_t n_adapters, int64_t r, const uint16_t* A,
                                      int64_t lda, const uint16_t* B, int64_t ldb);

@@ -329,7 +329,8 @@ def qk_norm_rope(q, k, cos, sin, gq=None, gk=None, eps=1e-6, pos=None, interleav
 def linear_lora(x, W, A, B, rows, scale=None, bias=None, out_dtype=torch.float32, out=None):
     """x W^T (+ bias) + scale[a] (x A[a]^T) B[a]^T with a = rows[t] for row t (int32, < 0: no
     adapter). x [T, K] bf16 or fp32 (rounded to bf16), W [N, K], A [n, r, K], B [n, N, r] bf16,
-    scale [n] and bias [N] fp32. Returns [T, N] in out_dtype (fp32 or bf16), or out."""
+    scale [n] and bias [N] fp32. Returns [T, N] in out_dtype (fp32 or bf16), or out. For a bf16 result
+    scale[a] (x A[a]^T) is rounded to bf16 before it meets B; for an fp32 one to 2^-16."""
     r = (_calls or _serving()).linear_lora(x, W, A, B, rows, scale, bias, out_dtype, out)
     if r is not None and r.__class__ is not int:
         return r
