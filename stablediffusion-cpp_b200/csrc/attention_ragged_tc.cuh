@@ -122,7 +122,7 @@ __device__ __forceinline__ bool load_seq(const RaggedAttention& p, int s, Seq& q
 struct Row {
   int tok, head;  // token of the sequence, query head
   bool valid;
-  int lim;        // keys [0, lim) are seen (none by a row that is nobody's)
+  int lim;        // keys [0, lim) are seen
   float pos;      // position among the keys
   float nslope;   // -slope log2(e)
 };
@@ -133,7 +133,8 @@ __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, 
   w.head = kvh * p.G + (r - t * p.G);
   w.valid = t < p.tpt && w.tok < q.ql;
   const int pos = w.tok + q.kl - q.ql;
-  w.lim = !w.valid ? 0 : p.a.causal ? min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0)) : q.kl;
+  w.lim = q.kl;
+  if (p.a.causal) w.lim = min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0));
   w.pos = (float)pos;
   w.nslope = p.a.slopes && w.valid ? -p.a.slopes[w.head] * kLog2e : 0.0f;
   return w;
@@ -169,10 +170,11 @@ __device__ __forceinline__ float2 to_log2(const TcParams& p, float2 z, bool smal
 
 // One softmax step of a warp's 32 rows: S (128 keys, TMEM) -> P over its first 64 columns.
 // `turn` runs before the exp pass and returns false to abandon; `half` runs when keys 0..63
-// of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys.
+// of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys. valid: the
+// row is somebody's (what others hold must not cost the warp the longer tanh).
 template <int DP, class T, int MOD, class Turn, class Half>
 __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr, uint32_t o_addr, bool have_o, bool masked,
-                                             int n_ok, float dist0, float nslope, float& m_used, float& l, Turn turn,
+                                             int n_ok, bool valid, float dist0, float nslope, float& m_used, float& l, Turn turn,
                                              Half half) {
   uint32_t u[4][32];
   __syncwarp();
@@ -182,11 +184,6 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
   if constexpr (MOD != 0) {
     bool small = true;
     if constexpr (MOD & 1) {
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kBK; ++c)
-          if (c >= n_ok) u[c >> 5][c & 31] = 0;
-      }
       float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < kBK; c += 8)
@@ -194,7 +191,12 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
         for (int i = 0; i < 4; ++i)
           top[i] = fmax3(top[i], fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i])),
                          fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1])));
-      small = n_ok <= 0 || !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
+      small = !valid || !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
+      if (masked && !small) {  // rarely: again over the keys that the row sees
+        small = true;
+#pragma unroll
+        for (int c = 0; c < kBK; ++c) small &= c >= n_ok || !(fabsf(__uint_as_float(u[c >> 5][c & 31])) > p.cap_small);
+      }
     }
     auto modify = [&](bool sm) {
 #pragma unroll
@@ -313,12 +315,16 @@ __device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_a
     if constexpr (MOD & 1) {
       float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (8 * i >= n_ok) at(i, 0) = 0;
-        if (8 * i + 1 >= n_ok) at(i, 1) = 0;
-        top = fmax3(top, fabsf(__uint_as_float(at(i, 0))), fabsf(__uint_as_float(at(i, 1))));
+      for (int i = 0; i < 16; ++i) top = fmax3(top, fabsf(__uint_as_float(at(i, 0))), fabsf(__uint_as_float(at(i, 1))));
+      small = !(top > p.cap_small) || n_ok <= 0;
+      if (!small) {  // rarely: again over the keys that the row sees
+        small = true;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          small &= 8 * i >= n_ok || !(fabsf(__uint_as_float(at(i, 0))) > p.cap_small);
+          small &= 8 * i + 1 >= n_ok || !(fabsf(__uint_as_float(at(i, 1))) > p.cap_small);
+        }
       }
-      small = !(top > p.cap_small);
     }
     const float dist0 = r.pos - (float)(kbase + j2);
     float top = -INFINITY;
@@ -799,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int kbase = j * kBK;
       ok = softmax_step<DP, T, MOD>(
-          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.pos - (float)kbase, w.nslope, m, l,
+          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, w.pos - (float)kbase, w.nslope, m, l,
           [&]() {
             // The tiles take turns (A(0), B(0), A(1), ...) while both have keys.
             if (!two || (t == 0 ? j == 0 : j >= nA)) return true;
@@ -1119,7 +1125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const Row x = make_row(p, q, p.seq0 + it.s, it.kvh, 0, (lane >> 2) + 8 * h);
-          few[h].lim = x.lim;
+          few[h].lim = !(MOD & 1) || x.valid ? x.lim : 0;
           few[h].pos = x.pos;
           few[h].nslope = x.nslope;
         }
@@ -1145,7 +1151,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           softmax_step<DP, T, MOD>(
-              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.pos - (float)kbase, w.nslope, m, l,
+              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, w.pos - (float)kbase, w.nslope, m, l,
               []() { return true; },
               [&]() {
                 if (lane == 0) mbar_arrive(p_half);
