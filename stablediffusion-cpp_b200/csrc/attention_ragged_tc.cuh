@@ -2,9 +2,12 @@
 // widths up to 128. Flash attention: the running maximum m and sum l of a softmax, so
 // scores never leave the SM:
 //   S = Q K^T (tcgen05, fp32 in TMEM);  P = 2^(S' - m) in the operand type, back in TMEM over
-//   S;  O += P V (tcgen05);  O is rescaled when m grows by more than 2^8; out = O / l.
+//   S;  O += P V (tcgen05);  O is rescaled when m grows by more than 2^8 (2^4 for fp16); out = O / l.
 // P is rounded to the operand type because the tensor core multiplies it so: 2^-8 (bf16) or
-// 2^-11 (fp16) of each probability, averaged over the keys; l, m, S and O stay fp32.
+// 2^-11 (fp16) of each probability, averaged over the keys; l, m, S and O stay fp32. fp16 ends
+// at 2^-24, and a long cache has many keys of little weight each, so its P (and l and O with it)
+// is 2^11 times as large: up to 2^15, and what rounds away is 2^-36 of the largest or less. With
+// the largest at 1, 60000 keys of 2^-26 each left the sum without a trace.
 //
 // The G = heads / kv_heads query heads of a key head share its keys, so a 128-row tile
 // holds floor(128 / G) tokens x G heads (row r is token r / G, head r % G): K and V are read
@@ -47,7 +50,6 @@ constexpr int kThreads = 384;  // control warpgroup + two softmax warpgroups
 // setmaxnreg split as in attention_tc.cu: 128 x 56 + 256 x 224 = 384 x 168.
 constexpr int kRegsLaunch = 168, kRegsControl = 56, kRegsSoftmax = 224;
 static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split");
-constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays <= 256
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSeqs = 512;  // sequences of one k_ragged_streams launch
 constexpr int kMaxSmem = 232448;
@@ -72,9 +74,11 @@ struct TcParams {
 
 template <class T>
 struct Op;
+// kLift: log2 of what P is multiplied by; kSlack: how far m may stay behind, so P <= 2^(kLift + kSlack).
 template <>
 struct Op<__half> {
   static constexpr uint32_t kFmt = 0;
+  static constexpr float kLift = 11.0f, kSlack = 4.0f;
   __device__ static uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -83,6 +87,7 @@ struct Op<__half> {
 template <>
 struct Op<__nv_bfloat16> {
   static constexpr uint32_t kFmt = 1;
+  static constexpr float kLift = 0.0f, kSlack = 8.0f;
   __device__ static uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -229,7 +234,7 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
       pm[i] = fmax3(pm[i], __uint_as_float(u[c >> 5][(c & 31) + 2 * i]), __uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1]));
   const float sc = MOD ? 1.0f : p.scale_log2;  // positive, so max(s) sc = max(s sc)
   const float m_new = fmaxf(m_used, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])) * sc);
-  const bool need = m_new > m_used + kRescaleThreshold;
+  const bool need = m_new > m_used + Op<T>::kSlack;
   if (__any_sync(0xffffffffu, need)) {
     // The PV of the step before completed before S was posted, so O is at rest here.
     if (have_o) {
@@ -251,7 +256,7 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
     }
   }
   if (!turn()) return false;
-  const float neg_m = (m_used == -INFINITY) ? 0.0f : -m_used;
+  const float neg_m = (m_used == -INFINITY) ? 0.0f : Op<T>::kLift - m_used;
   const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(neg_m, neg_m);
   float2 psa = make_float2(0.0f, 0.0f), psb = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -351,13 +356,13 @@ __device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_a
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const float m_new = fmaxf(r.m, top);
-    if (m_new > r.m + kRescaleThreshold) {
+    if (m_new > r.m + Op<T>::kSlack) {
       f[h] = ex2_approx(r.m - m_new);
       r.l *= f[h];
       r.m = m_new;
       need_any = true;
     }
-    const float neg_m = r.m == -INFINITY ? 0.0f : -r.m;
+    const float neg_m = r.m == -INFINITY ? 0.0f : Op<T>::kLift - r.m;
     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -467,12 +472,13 @@ __device__ __noinline__ void redo_rows(const TcParams& p, const Seq& q, const Ro
     float o[4], m, l;
     slow_row<T>(p, (int64_t)q.q0 + tok, head, q.k0, j0, min(j1, lim), pos, ns, o, m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float lift = ex2_approx(Op<T>::kLift);  // as the other pieces of the row
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int ch = lane + 32 * c;
       if (ch >= p.a.d) continue;
       if (piece) {
-        piece[(int64_t)row * (p.a.d + 2) + ch] = o[c];
+        piece[(int64_t)row * (p.a.d + 2) + ch] = o[c] * lift;
       } else {
         const int64_t at = ((int64_t)q.q0 + tok) * p.a.ldo + (int64_t)head * p.a.d + ch;
         if (p.a.out_type == kBF16)
@@ -483,7 +489,7 @@ __device__ __noinline__ void redo_rows(const TcParams& p, const Seq& q, const Ro
     }
     if (piece && lane == 0) {
       piece[(int64_t)row * (p.a.d + 2) + p.a.d] = m;
-      piece[(int64_t)row * (p.a.d + 2) + p.a.d + 1] = l;
+      piece[(int64_t)row * (p.a.d + 2) + p.a.d + 1] = l * lift;
     }
   }
 }
