@@ -177,7 +177,8 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
       for (int o = 1 << lg >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       const float rstd = rsqrtf(fmaf(s, inv_d, p.eps));
       const float2 r2 = make_float2(rstd, rstd);
-      if (on && h < n) {
+      // Channels that are not rotated leave their partner out: 0 times an infinity there is NaN.
+      auto finish = [&](auto turn) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float f[VE];
@@ -185,7 +186,9 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
           for (int i = 0; i < VE / 2; ++i) {
             const int e = k * VE / 2 + i;
             const float2 o = INTER ? make_float2(v[e].y, v[e].x) : v[(e + VE / 2) % VE];
-            const float2 r = fmul2(r2, ffma2(o, B[e], fmul2(v[e], A[e])));
+            float2 r = fmul2(v[e], A[e]);
+            if constexpr (decltype(turn)::value) r = ffma2(o, B[e], r);
+            r = fmul2(r2, r);
             f[2 * i] = r.x;
             f[2 * i + 1] = r.y;
           }
@@ -193,6 +196,12 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
           out.set(f);
           out.store(y + (int64_t)h * p.d + (k ? c1 : c0));
         }
+      };
+      if (on && h < n) {
+        if (cos)
+          finish(std::true_type{});
+        else
+          finish(std::false_type{});
       }
     }
   }
