@@ -223,6 +223,9 @@ int sdb200_set_attention_path(int path);
  *     was (a row with a bad adapter gets no adapter); sdb200_synchronize reports it.
  *   - Workspaces are the caller's (256-byte aligned, contents arbitrary, free again when
  *     the call's work is done), so calls may be captured into graphs. No call allocates.
+ *   - What a call writes (outputs, workspace) shares no byte with what it reads or with its other
+ *     outputs, except that q and k may be written in place (below); rows of one pitch may lie side
+ *     by side, as columns of one buffer. Anything else is refused.
  *   - Element types: */
 #define SDB200_F32 0
 #define SDB200_BF16 1
@@ -234,7 +237,7 @@ int sdb200_set_attention_path(int path);
  * [n_pos, rot] (pos null: row t % n_pos); channels rot..d-1 stay u. q [T, heads * d] and
  * k [T, kv_heads * d] have row pitches ldq / ldk (views of a fused QKV projection), either
  * head count may be 0. in_type / out_type: SDB200_F32, _BF16 or _F16; computed in fp32,
- * rounded once. q_out may be q itself (same type and pitch), likewise k_out. d <= 1024. */
+ * rounded once. q_out may be q itself (same type and pitch), likewise k_out k. d <= 1024. */
 int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const void* k, int64_t ldk, int kv_heads,
                         int in_type, int64_t d, int64_t rot, const float* gq, const float* gk, float eps,
                         const float* cos, const float* sin, int64_t n_pos, const int32_t* pos, int interleaved,

@@ -24,24 +24,25 @@ void require_ptr(const void* p, int64_t align, const char* op, const char* name)
 }
 int64_t esize(int type) { return type == kF32 ? 4 : 2; }
 
-// y may be x itself (same pointer, type and pitch) and must not overlap it otherwise.
-void require_apart(const char* op, const char* what, const void* x, int64_t ldx, int64_t ex, const void* y,
-                   int64_t ldy, int64_t ey, int64_t rows, int64_t cols) {
-  if (x == y && ldx == ldy && ex == ey) return;
-  const char *x0 = (const char*)x, *y0 = (const char*)y;
-  const char *x1 = x0 + ((rows - 1) * ldx + cols) * ex, *y1 = y0 + ((rows - 1) * ldy + cols) * ey;
-  require(y1 <= x0 || x1 <= y0, op, std::string(what) + " overlaps its input without being the same buffer");
+// Memory that a call reads or writes: `rows` rows of `bytes` bytes, `pitch` bytes apart.
+struct Rows {
+  const void* p;
+  int64_t rows, pitch, bytes;
+};
+Rows vec(const void* p, int64_t bytes) { return Rows{p, 1, bytes, bytes}; }
+// Whether two share bytes; rows of one pitch may lie side by side.
+bool share(const Rows& x, const Rows& y) {
+  if (!x.p || !y.p || x.rows <= 0 || y.rows <= 0 || x.bytes <= 0 || y.bytes <= 0) return false;
+  const char *x0 = (const char*)x.p, *y0 = (const char*)y.p;
+  if (y0 + (y.rows - 1) * y.pitch + y.bytes <= x0 || x0 + (x.rows - 1) * x.pitch + x.bytes <= y0) return false;
+  if (x.pitch != y.pitch) return true;
+  const int64_t off = (((y0 - x0) % x.pitch) + x.pitch) % x.pitch;
+  return off < x.bytes || off + y.bytes > x.pitch;
 }
-
-// Whether rows of x and of y share bytes; rows of one pitch may lie side by side.
-bool share(const void* x, int64_t x_rows, int64_t x_pitch, int64_t x_bytes, const void* y, int64_t y_rows, int64_t y_pitch,
-           int64_t y_bytes) {
-  const char *x0 = (const char*)x, *y0 = (const char*)y;
-  if (y0 + (y_rows - 1) * y_pitch + y_bytes <= x0 || x0 + (x_rows - 1) * x_pitch + x_bytes <= y0) return false;
-  if (x_pitch != y_pitch) return true;
-  const int64_t off = (((y0 - x0) % x_pitch) + x_pitch) % x_pitch;
-  return off < x_bytes || off + y_bytes > x_pitch;
+void require_apart(const char* op, const char* out_name, const Rows& out, const char* name, const Rows& x) {
+  require(!share(out, x), op, std::string(out_name) + " overlaps " + name);
 }
+bool same(const Rows& x, const Rows& y) { return x.p == y.p && x.pitch == y.pitch && x.bytes == y.bytes; }
 
 void check_lora(const LoraLinear& p) {
   const char* op = "linear_lora";
@@ -120,18 +121,22 @@ int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const 
     if (T == 0) return kOk;
     const int64_t ei = esize(in_type);
     const int64_t eo = esize(out_type);
+    const Rows rq{heads ? q : nullptr, T, ldq * ei, heads * d * ei};
+    const Rows rk{kv_heads ? k : nullptr, T, ldk * ei, kv_heads * d * ei};
+    const Rows rqo{heads ? q_out : nullptr, T, ldqo * eo, heads * d * eo};
+    const Rows rko{kv_heads ? k_out : nullptr, T, ldko * eo, kv_heads * d * eo};
     if (heads) {
       require(ldq >= heads * d && ldqo >= heads * d, op, "row pitch of q smaller than heads * d");
       require_ptr(q, ei, op, "q");
       require_ptr(q_out, eo, op, "q_out");
-      require_apart(op, "q_out", q, ldq, ei, q_out, ldqo, eo, T, heads * d);
+      if (!same(rq, rqo)) require_apart(op, "q_out", rqo, "q (and is not q itself)", rq);
       require(q != q_out || in_type == out_type, op, "in place needs one type");
     }
     if (kv_heads) {
       require(ldk >= kv_heads * d && ldko >= kv_heads * d, op, "row pitch of k smaller than kv_heads * d");
       require_ptr(k, ei, op, "k");
       require_ptr(k_out, eo, op, "k_out");
-      require_apart(op, "k_out", k, ldk, ei, k_out, ldko, eo, T, kv_heads * d);
+      if (!same(rk, rko)) require_apart(op, "k_out", rko, "k (and is not k itself)", rk);
       require(k != k_out || in_type == out_type, op, "in place needs one type");
     }
     if (gq) require_ptr(gq, 4, op, "gq");
@@ -142,6 +147,20 @@ int sdb200_qk_norm_rope(int64_t T, const void* q, int64_t ldq, int heads, const 
       require(n_pos > 0 && n_pos < kMaxRows, op, "n_pos must be positive");
     }
     if (pos) require_ptr(pos, 4, op, "pos");
+    // Warps write q_out and k_out while others still read the rest.
+    require_apart(op, "q_out", rqo, "k", rk);
+    require_apart(op, "k_out", rko, "q", rq);
+    require_apart(op, "k_out", rko, "q_out", rqo);
+    const int64_t table = rot ? n_pos * rot * 4 : 0;
+    auto apart = [&](const char* name, const void* x, int64_t bytes) {
+      require_apart(op, "q_out", rqo, name, vec(x, bytes));
+      require_apart(op, "k_out", rko, name, vec(x, bytes));
+    };
+    apart("cos", cos, table);
+    apart("sin", sin, table);
+    apart("gq", gq, d * 4);
+    apart("gk", gk, d * 4);
+    apart("pos", pos, T * 4);
     QkNormRope p{T, q, k, ldq, ldk, heads, kv_heads, (int)d, (int)rot, gq, gk, eps, cos, sin, rot ? n_pos : T,
                  rot ? pos : nullptr, interleaved != 0, q_out, k_out, ldqo, ldko, nullptr};
     launch_qk_norm_rope(p, in_type, out_type);
@@ -184,18 +203,26 @@ int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t l
     require_ptr(Y, p.y_bf16 ? 2 : 4, op, "Y");
     const int64_t ey = p.y_bf16 ? 2 : 4;
     const int64_t ex = p.x_bf16 ? 2 : 4;
-    auto apart = [&](const void* x, int64_t rows, int64_t ld, int64_t cols, int64_t e, const char* name) {
-      require(!share(x, rows, ld * e, cols * e, Y, T, ldy * ey, N * ey), op, std::string("Y overlaps ") + name);
-    };
-    apart(X, T, ldx, K, ex, "X");
-    apart(W, N, ldw, K, 2, "W");
-    if (n_adapters > 0 && r > 0) {
-      apart(A, n_adapters * r, lda, K, 2, "A");
-      apart(B, n_adapters * N, ldb, r, 2, "B");
-    }
+    const bool adapters = n_adapters > 0 && r > 0;
+    const Rows y{Y, T, ldy * ey, N * ey};
+    const struct {
+      const char* name;
+      Rows at;
+    } inputs[] = {{"X", {X, T, ldx * ex, K * ex}},
+                  {"W", {W, N, ldw * 2, K * 2}},
+                  {"A", {adapters ? A : nullptr, n_adapters * r, lda * 2, K * 2}},
+                  {"B", {adapters ? B : nullptr, n_adapters * N, ldb * 2, r * 2}},
+                  {"bias", vec(bias, N * 4)},
+                  {"row_adapter", vec(adapters ? row_adapter : nullptr, T * 4)},
+                  {"scale", vec(adapters ? scale : nullptr, n_adapters * 4)}};
+    for (const auto& x : inputs) require_apart(op, "Y", y, x.name, x.at);
     const int64_t need = (int64_t)lora_linear_workspace(p);
     require(ws_bytes >= need, op, "workspace of " + std::to_string(need) + " bytes needed");
-    if (need) require_ptr(ws, 256, op, "ws");
+    if (need) {
+      require_ptr(ws, 256, op, "ws");
+      require_apart(op, "Y", y, "ws", vec(ws, need));
+      for (const auto& x : inputs) require_apart(op, "ws", vec(ws, need), x.name, x.at);
+    }
     launch_lora_linear(p, ws);
   })
 }
@@ -254,22 +281,31 @@ int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t l
       require_ptr(k, 2, op, "k");
       require_ptr(v, 2, op, "v");
     }
-    const char* o0 = (const char*)out;
-    const char* o1 = o0 + ((Tq - 1) * ldo + heads * d) * 2;
-    auto apart = [&](const void* x, int64_t rows, int64_t ld, int64_t cols, const char* name) {
-      const char* x0 = (const char*)x;
-      require(rows <= 0 || o1 <= x0 || x0 + ((rows - 1) * ld + cols) * 2 <= o0, op, std::string("out overlaps ") + name);
-    };
-    apart(q, Tq, ldq, heads * d, "q");
-    if (p.max_kv > 0 && Tkv > 0) {
-      apart(k, Tkv, ldk, kv_heads * d, "k");
-      apart(v, Tkv, ldv, kv_heads * d, "v");
-    }
+    const Rows o{out, Tq, ldo * 2, heads * d * 2};
+    const bool keys = p.max_kv > 0 && Tkv > 0;
+    const int64_t per_seq = (int64_t)n_seq * 4;
+    const struct {
+      const char* name;
+      Rows at;
+    } inputs[] = {{"q", {q, Tq, ldq * 2, heads * d * 2}},
+                  {"k", {keys ? k : nullptr, Tkv, ldk * 2, kv_heads * d * 2}},
+                  {"v", {keys ? v : nullptr, Tkv, ldv * 2, kv_heads * d * 2}},
+                  {"q_begin", vec(q_begin, per_seq)},
+                  {"q_len", vec(q_len, per_seq)},
+                  {"kv_begin", vec(kv_begin, per_seq)},
+                  {"kv_len", vec(kv_len, per_seq)},
+                  {"slopes", vec(slopes, (int64_t)heads * 4)},
+                  {"prefix", vec(prefix, per_seq)}};
     if (slopes) require_ptr(slopes, 4, op, "slopes");
     if (prefix) require_ptr(prefix, 4, op, "prefix");
+    for (const auto& x : inputs) require_apart(op, "out", o, x.name, x.at);
     const int64_t need = (int64_t)ragged_attention_workspace(p);
     require(ws_bytes >= need, op, "workspace of " + std::to_string(need) + " bytes needed");
-    if (need) require_ptr(ws, 256, op, "ws");
+    if (need) {
+      require_ptr(ws, 256, op, "ws");
+      require_apart(op, "out", o, "ws", vec(ws, need));
+      for (const auto& x : inputs) require_apart(op, "ws", vec(ws, need), x.name, x.at);
+    }
     launch_ragged_attention(p, ws);
   })
 }
