@@ -128,7 +128,7 @@ struct Row {
   int tok, head;  // token of the sequence, query head
   bool valid;
   int lim;        // keys [0, lim) are seen
-  float pos;      // position among the keys
+  int pos;        // position among the keys (beyond 2^24 not every one is an fp32 number; distances are taken first)
   float nslope;   // -slope log2(e)
 };
 __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, int kvh, int tok0, int r) {
@@ -140,7 +140,7 @@ __device__ __forceinline__ Row make_row(const TcParams& p, const Seq& q, int s, 
   const int pos = w.tok + q.kl - q.ql;
   w.lim = q.kl;
   if (p.a.causal) w.lim = min(q.kl, max(pos + 1, p.a.prefix ? p.a.prefix[s] : 0));
-  w.pos = (float)pos;
+  w.pos = pos;
   w.nslope = p.a.slopes && w.valid ? -p.a.slopes[w.head] * kLog2e : 0.0f;
   return w;
 }
@@ -292,8 +292,8 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
 // l, of which each has its own keys' part.
 struct FewRow {
   float m = -INFINITY, l = 0.0f;
-  int lim = 0;
-  float pos = 0.0f, nslope = 0.0f;
+  int lim = 0, pos = 0;
+  float nslope = 0.0f;
 };
 
 // softmax_step for a tile of at most 16 rows, TMEM lanes 0 to 15 of the warp: a quad of lanes
@@ -331,7 +331,7 @@ __device__ __forceinline__ void softmax_step_few(const TcParams& p, uint32_t s_a
         }
       }
     }
-    const float dist0 = r.pos - (float)(kbase + j2);
+    const float dist0 = (float)(r.pos - (kbase + j2));
     float top = -INFINITY;
     auto modify = [&](bool sm) {
 #pragma unroll
@@ -425,7 +425,7 @@ __device__ __forceinline__ void store_out(const TcParams& p, int64_t at, const u
 // infinity or NaN. A masked key's probability is 0, but 0 times a value that is not finite
 // is NaN in a matrix product; here such keys are left out.
 template <class T>
-__device__ __noinline__ void slow_row(const TcParams& p, int64_t qrow, int head, int k0, int j0, int j1, float pos, float nslope,
+__device__ __noinline__ void slow_row(const TcParams& p, int64_t qrow, int head, int k0, int j0, int j1, int pos, float nslope,
                                       float (&o)[4], float& m, float& l) {
   const RaggedAttention& a = p.a;
   const int lane = threadIdx.x & 31, kvh = head / p.G;
@@ -447,7 +447,7 @@ __device__ __noinline__ void slow_row(const TcParams& p, int64_t qrow, int head,
       if (lane + 32 * c < a.d) z = fmaf(qv[c], to_f32(k[lane + 32 * c]), z);
     z = warp_add(z);
     z = a.cap > 0.0f ? p.cap_log2 - 2.0f * p.cap_log2 * rcp_approx(1.0f + ex2_approx(z * p.cap_in)) : z * p.scale_log2;
-    z = fmaf(nslope, fabsf(pos - (float)j), z);
+    z = fmaf(nslope, fabsf((float)(pos - j)), z);
     if (z == -INFINITY) continue;
     const float mn = fmaxf(m, z), f = ex2_approx(m - mn), w = ex2_approx(z - mn);
     m = mn;
@@ -468,7 +468,8 @@ __device__ __noinline__ void redo_rows(const TcParams& p, const Seq& q, const Ro
     const int src = __ffs(todo) - 1;
     const int tok = __shfl_sync(0xffffffffu, w.tok, src), head = __shfl_sync(0xffffffffu, w.head, src);
     const int lim = __shfl_sync(0xffffffffu, w.lim, src), row = __shfl_sync(0xffffffffu, r, src);
-    const float pos = __shfl_sync(0xffffffffu, w.pos, src), ns = __shfl_sync(0xffffffffu, w.nslope, src);
+    const int pos = __shfl_sync(0xffffffffu, w.pos, src);
+    const float ns = __shfl_sync(0xffffffffu, w.nslope, src);
     float o[4], m, l;
     slow_row<T>(p, (int64_t)q.q0 + tok, head, q.k0, j0, min(j1, lim), pos, ns, o, m, l);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -811,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int kbase = j * kBK;
       ok = softmax_step<DP, T, MOD>(
-          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, w.pos - (float)kbase, w.nslope, m, l,
+          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, (float)(w.pos - kbase), w.nslope, m, l,
           [&]() {
             // The tiles take turns (A(0), B(0), A(1), ...) while both have keys.
             if (!two || (t == 0 ? j == 0 : j >= nA)) return true;
@@ -1157,7 +1158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           softmax_step<DP, T, MOD>(
-              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, w.pos - (float)kbase, w.nslope, m, l,
+              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, (float)(w.pos - kbase), w.nslope, m, l,
               []() { return true; },
               [&]() {
                 if (lane == 0) mbar_arrive(p_half);
