@@ -15,8 +15,12 @@ namespace {
 
 constexpr int64_t kMaxRows = (int64_t)1 << 31;
 
-void require(bool ok, const char* op, const std::string& what) {
+// Messages are put together where a check fails only: a call makes dozens.
+void require(bool ok, const char* op, const char* what) {
   if (!ok) fail(kErrInvalidArg, std::string(op) + ": " + what);
+}
+void require_workspace(int64_t got, int64_t need, const char* op) {
+  if (got < need) fail(kErrInvalidArg, std::string(op) + ": workspace of " + std::to_string(need) + " bytes needed");
 }
 void require_ptr(const void* p, int64_t align, const char* op, const char* name) {
   if (!p) fail(kErrInvalidArg, std::string(op) + ": null pointer " + name);
@@ -40,7 +44,7 @@ bool share(const Rows& x, const Rows& y) {
   return off < x.bytes || off + y.bytes > x.pitch;
 }
 void require_apart(const char* op, const char* out_name, const Rows& out, const char* name, const Rows& x) {
-  require(!share(out, x), op, std::string(out_name) + " overlaps " + name);
+  if (share(out, x)) fail(kErrInvalidArg, std::string(op) + ": " + out_name + " overlaps " + name);
 }
 bool same(const Rows& x, const Rows& y) { return x.p == y.p && x.pitch == y.pitch && x.bytes == y.bytes; }
 
@@ -217,7 +221,7 @@ int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t l
                   {"scale", vec(adapters ? scale : nullptr, n_adapters * 4)}};
     for (const auto& x : inputs) require_apart(op, "Y", y, x.name, x.at);
     const int64_t need = (int64_t)lora_linear_workspace(p);
-    require(ws_bytes >= need, op, "workspace of " + std::to_string(need) + " bytes needed");
+    require_workspace(ws_bytes, need, op);
     if (need) {
       require_ptr(ws, 256, op, "ws");
       require_apart(op, "Y", y, "ws", vec(ws, need));
@@ -300,7 +304,7 @@ int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t l
     if (prefix) require_ptr(prefix, 4, op, "prefix");
     for (const auto& x : inputs) require_apart(op, "out", o, x.name, x.at);
     const int64_t need = (int64_t)ragged_attention_workspace(p);
-    require(ws_bytes >= need, op, "workspace of " + std::to_string(need) + " bytes needed");
+    require_workspace(ws_bytes, need, op);
     if (need) {
       require_ptr(ws, 256, op, "ws");
       require_apart(op, "out", o, "ws", vec(ws, need));
