@@ -269,7 +269,8 @@ int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t l
  *   out = softmax(z) v, 0 where no key is left
  * q [Tq, ldq], k / v [Tkv, ldk / ldv] bf16 or fp16 (in_type), out [Tq, ldo] bf16 or fp16
  * (out_type), heads d <= 256 wide, out apart from the inputs. max_q / max_kv bound the lengths;
- * sequences may share key rows, not query rows.
+ * sequences may share key rows, not query rows. scale, cap, scale / cap and cap / scale are normal
+ * fp32 numbers, with a factor of 1000 to spare.
  * What a mask hides does not reach the result, whatever it holds; rows of no sequence are
  * left as they were. ws: at least sdb200_attention_ragged_workspace() bytes. */
 int64_t sdb200_attention_ragged_workspace(int n_seq, int64_t max_q, int64_t max_kv, int heads, int kv_heads,

@@ -89,6 +89,13 @@ void check_attention(const RaggedAttention& p) {
   require(p.d > 0 && p.d <= 256, op, "head width must be 1..256");
   require(std::isfinite(p.scale) && p.scale > 0.0f, op, "scale must be positive and finite");
   require(std::isfinite(p.cap) && p.cap >= 0.0f, op, "cap must be 0 (off) or positive and finite");
+  // The kernels multiply scores with these; an infinite one makes NaN of 0, a subnormal one has lost its digits.
+  const float log2e = 1.4426950f;
+  bool usable = std::isnormal(p.scale) && std::isnormal(p.scale * log2e);
+  if (p.cap > 0.0f)
+    for (const float x : {p.scale / p.cap, p.cap / p.scale, 2.0f * log2e * p.scale / p.cap, p.cap * log2e, p.cap * 1e-3f})
+      usable = usable && std::isnormal(x);
+  require(usable, op, "scale and cap leave fp32's range");
   require(!p.prefix || p.causal, op, "a prefix needs the causal mask");
 }
 
