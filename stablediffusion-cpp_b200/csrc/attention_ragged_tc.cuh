@@ -175,11 +175,10 @@ __device__ __forceinline__ float2 to_log2(const TcParams& p, float2 z, bool smal
 
 // One softmax step of a warp's 32 rows: S (128 keys, TMEM) -> P over its first 64 columns.
 // `turn` runs before the exp pass and returns false to abandon; `half` runs when keys 0..63
-// of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys. valid: the
-// row is somebody's (what others hold must not cost the warp the longer tanh).
+// of P are stored. masked: some row of the tile sees only the first n_ok < 128 keys.
 template <int DP, class T, int MOD, class Turn, class Half>
 __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr, uint32_t o_addr, bool have_o, bool masked,
-                                             int n_ok, bool valid, float dist0, float nslope, float& m_used, float& l, Turn turn,
+                                             int n_ok, float dist0, float nslope, float& m_used, float& l, Turn turn,
                                              Half half) {
   uint32_t u[4][32];
   __syncwarp();
@@ -196,7 +195,7 @@ __device__ __forceinline__ bool softmax_step(const TcParams& p, uint32_t s_addr,
         for (int i = 0; i < 4; ++i)
           top[i] = fmax3(top[i], fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i])),
                          fabsf(__uint_as_float(u[c >> 5][(c & 31) + 2 * i + 1])));
-      small = !valid || !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
+      small = n_ok <= 0 || !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > p.cap_small);
       if (masked && !small) {  // rarely: again over the keys that the row sees
         small = true;
 #pragma unroll
@@ -563,7 +562,8 @@ struct TilesCfg {
   static constexpr int Q_BYTES = ATOMS * ATOM;
   static constexpr int KV_BYTES = ATOMS * ATOM;
   static constexpr int SLOTS = DP == 128 ? 5 : 10;
-  static constexpr int SMEM = 2 * Q_BYTES + SLOTS * KV_BYTES + 1024 + 512;
+  static constexpr int SMEM = 2 * Q_BYTES + SLOTS * KV_BYTES + 1024 + 512;  // 512: barriers, TMEM address, abort words, scan
+  static_assert((13 + 2 * SLOTS) * 8 + 4 + kAbortWords(kThreads / 32) * 4 + 64 <= 512, "room behind the slots");
 };
 constexpr uint32_t kOCol = 256;  // TMEM: S_A | S_B | O_A | O_B
 
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* r_empty = r_full + SLOTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + SLOTS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* scan = reinterpret_cast<int*>(tmem_slot + 2);  // [16]
+  int* scan = reinterpret_cast<int*>(tmem_slot + 1 + kAbortWords(kThreads / 32));  // [16]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x % p.a.kv_heads;
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&o_final[i], 1);
       mbar_init(&drain[i], 1);
     }
-    *abort_flag = 0;
+    for (int i = 0; i < kAbortWords(kThreads / 32); ++i) abort_flag[i] = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int issued = -1;
         RingPos at;
         for (int i = 0; i < 2 * nkv; ++i, at.next(SLOTS)) {
-          if (!mbar_wait(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait)) break;
+          if (!mbar_wait_warp(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait)) break;
           const uint32_t bar = full0 + (uint32_t)(at.slot * 8), dst = ring + (uint32_t)(at.slot * C_::KV_BYTES);
           mbar_expect_tx_elect(bar, C_::KV_BYTES);
           const CUtensorMap* tm = (i & 1) ? &tmV : &tmK;
@@ -723,6 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = max(0, issued - SLOTS + 1); i <= issued; ++i)
             while (!mbar_try_wait(&r_full[i % SLOTS], (i / SLOTS) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
             }
+          __syncwarp();
         }
       }
     } else if (warp == 1 || warp == 2) {
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The whole warp runs the loop (it zeroes the last V tile's tail); lane 0 issues.
       const int t = warp - 1, nt = t ? nB : nA;
       if (nt > 0 || (t == 0 && two)) {
-        bool ok = mbar_wait(q_full, 0, abort_flag, err, kErrAttnWait);
+        bool ok = mbar_wait_warp(q_full, 0, abort_flag, err, kErrAttnWait);
         tc_fence_after();
         const uint64_t qd = sdesc_k_sw128(smem_u32(sQ + t * C_::Q_BYTES)), kd0 = sdesc_k_sw128(smem_u32(sR));
         const uint64_t vd0 = sdesc_mn_sw128(smem_u32(sR), C_::ATOM, 1024);
@@ -741,16 +742,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; ok && j <= nkv; ++j) {
           // K_j and V_(j-1) normally landed long ago; waiting for them before P_t(j-1) lets the
           // PV and the QK^T go out back to back once P is there.
-          if (j > 0 && !mbar_wait(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait)) break;
-          if (j < nkv && !mbar_wait(&r_full[k.slot], k.phase, abort_flag, err, kErrAttnWait)) break;
+          if (j > 0 && !mbar_wait_warp(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait)) break;
+          if (j < nkv && !mbar_wait_warp(&r_full[k.slot], k.phase, abort_flag, err, kErrAttnWait)) break;
           if (j > 0) {
             if (j <= nt) {
               if (j * kBK > q.kl) zero_v_tail<DP>(sR + v.slot * C_::KV_BYTES, q.kl - (j - 1) * kBK);
               const uint64_t vd = vd0 + (uint64_t)(v.slot * (C_::KV_BYTES >> 4));
-              if (!mbar_wait(&p_half[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
+              if (!mbar_wait_warp(&p_half[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
               tc_fence_after();
               umma4_f16_ts_elect(d_o, d_s, vd, IDESC_O, j > 1 ? 1u : 0u);
-              if (!mbar_wait(&p_full[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
+              if (!mbar_wait_warp(&p_full[t], (j - 1) & 1, abort_flag, err, kErrAttnWait)) break;
               tc_fence_after();
               umma4_f16_ts_elect(d_o, d_s + 32, vd + 512, IDESC_O, 1u);
               umma_commit_elect(&r_empty[v.slot]);
@@ -796,7 +797,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const int t = (warp - 4) >> 2, qq = warp & 3;
     const int r = qq * 32 + lane, nt = t ? nB : nA;
-    const Row w = make_row(p, q, s, kvh, tok0 + t * p.tpt, r);
+    Row w = make_row(p, q, s, kvh, tok0 + t * p.tpt, r);
+    if ((MOD & 1) && !w.valid) w.lim = 0;  // what nobody's row holds must not cost the warp the longer tanh
     const uint32_t lane_base = tmem + ((uint32_t)(qq * 32) << 16);
     const uint32_t s_addr = lane_base + (uint32_t)(t * kBK);
     const uint32_t o_addr = lane_base + kOCol + (uint32_t)(t * DP);
@@ -805,18 +807,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
-      if (!mbar_wait(&s_full[t], j & 1, abort_flag, err, kErrAttnWait)) {
+      if (!mbar_wait_warp(&s_full[t], j & 1, abort_flag, err, kErrAttnWait)) {
         ok = false;
         break;
       }
       tc_fence_after();
       const int kbase = j * kBK;
       ok = softmax_step<DP, T, MOD>(
-          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, (float)(w.pos - kbase), w.nslope, m, l,
+          p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, (float)(w.pos - kbase), w.nslope, m, l,
           [&]() {
             // The tiles take turns (A(0), B(0), A(1), ...) while both have keys.
             if (!two || (t == 0 ? j == 0 : j >= nA)) return true;
-            return mbar_wait(&turn[t ^ 1], (t == 0 ? j - 1 : j) & 1, abort_flag, err, kErrAttnWait);
+            return mbar_wait_warp(&turn[t ^ 1], (t == 0 ? j - 1 : j) & 1, abort_flag, err, kErrAttnWait);
           },
           [&]() {
             if (lane == 0) mbar_arrive(&p_half[t]);
@@ -827,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&turn[t]);
       }
     }
-    if (ok && (nt == 0 || mbar_wait(&o_final[t], 0, abort_flag, err, kErrAttnWait))) {
+    if (ok && (nt == 0 || mbar_wait_warp(&o_final[t], 0, abort_flag, err, kErrAttnWait))) {
       tc_fence_after();
       finish_rows<DP, T>(p, q, w, o_addr, nt > 0, m, l, 0, q.kl, nullptr, r);
     }
@@ -948,8 +950,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ StepList steps;
   __shared__ uint64_t bars[2][8 + 2 * kMaxSlots];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
-  volatile int* abort_flag = &abort_word;
+  __shared__ int abort_words[kAbortWords(kThreads / 32)];
+  volatile int* abort_flag = abort_words;
   // Q of worker 0 | Q of worker 1 | slots of worker 0 | of worker 1. A Q atom may be shorter
   // than 128 rows: the MMA then reads rows of what follows, into rows that nobody uses.
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -983,7 +985,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(z + 8 + i, 1);
       mbar_init(z + 8 + kMaxSlots + i, 1);
     }
-    abort_word = 0;
+    for (int& w : abort_words) w = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -1016,14 +1018,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int nt = it.tiles();
           if (nt == 0) continue;
           const Seq& q = steps.seq[it.s];
-          ok = mbar_wait(q_empty, (nq & 1) ^ 1u, abort_flag, err, kErrAttnWait);
+          ok = mbar_wait_warp(q_empty, (nq & 1) ^ 1u, abort_flag, err, kErrAttnWait);
           if (!ok) break;
           mbar_expect_tx_elect(qbar, ATOMS * p.G * p.tpt * 128);
           for (int a = 0; a < ATOMS; ++a)
             tma_load_3d_elect(smem_u32(sQ) + a * p.q_atom, &tmQ, qbar, a * 64, it.kvh * p.G, q.q0);
           ++nq;
           for (int i = 0; i < 2 * nt && ok; ++i, at.next(SL)) {
-            ok = mbar_wait(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait_warp(&r_empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             const uint32_t bar = full0 + (uint32_t)(at.slot * 8), dst = ring + (uint32_t)(at.slot * KV_BYTES);
             mbar_expect_tx_elect(bar, KV_BYTES);
@@ -1042,6 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = max(0, ld - SL); i < ld; ++i)
             while (!mbar_try_wait(&r_full[i % SL], (i / SL) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
             }
+          __syncwarp();
         }
       }
     } else {
@@ -1057,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int nt = it.tiles();
         if (nt == 0) continue;
         const int kl = steps.seq[it.s].kl;
-        ok = mbar_wait(q_full, nq & 1, abort_flag, err, kErrAttnWait);
+        ok = mbar_wait_warp(q_full, nq & 1, abort_flag, err, kErrAttnWait);
         ++nq;
         tc_fence_after();
         RingPos v = at;
@@ -1065,16 +1068,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; ok && j <= nt; ++j) {
           if (j > 0) {
             uint8_t* vp = sR + v.slot * KV_BYTES;
-            ok = mbar_wait(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait_warp(&r_full[v.slot], v.phase, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             const int left = kl - (it.kt0 + j - 1) * kBK;
             if (left < kBK) zero_v_tail<DP>(vp, left);
             const uint64_t vd = vd0 + (uint64_t)(v.slot * (KV_BYTES >> 4));
-            ok = mbar_wait(p_half, (step - 1) & 1, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait_warp(p_half, (step - 1) & 1, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
             umma4_f16_ts_elect(d_o, d_s, vd, IDESC_O, j > 1 ? 1u : 0u);
-            ok = mbar_wait(p_full, (step - 1) & 1, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait_warp(p_full, (step - 1) & 1, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
             umma4_f16_ts_elect(d_o, d_s + 32, vd + 512, IDESC_O, 1u);
@@ -1084,7 +1087,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             v.next(SL);
           }
           if (j < nt) {
-            ok = mbar_wait(&r_full[at.slot], at.phase, abort_flag, err, kErrAttnWait);
+            ok = mbar_wait_warp(&r_full[at.slot], at.phase, abort_flag, err, kErrAttnWait);
             if (!ok) break;
             tc_fence_after();
             const uint64_t kd = kd0 + (uint64_t)(at.slot * (KV_BYTES >> 4));
@@ -1124,7 +1127,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Seq q = steps.seq[it.s];
       const int nt = it.tiles(), rows = p.G * q.ql;
       const bool busy = qq * 32 >= lane0 && qq * 32 - lane0 < rows;  // the warp has rows (uniform)
-      const Row w = make_row(p, q, p.seq0 + it.s, it.kvh, 0, max(r, 0));
+      Row w = make_row(p, q, p.seq0 + it.s, it.kvh, 0, max(r, 0));
+      if ((MOD & 1) && !w.valid) w.lim = 0;
       const int lim0 = p.a.causal ? min(q.kl, max(q.kl - q.ql + 1, p.a.prefix ? p.a.prefix[p.seq0 + it.s] : 0)) : q.kl;
       float m = -INFINITY, l = 0.0f;
       FewRow few[2];
@@ -1138,7 +1142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       for (int j = 0; j < nt; ++j, ++step) {
-        if (!mbar_wait(s_full, step & 1, abort_flag, err, kErrAttnWait)) {
+        if (!mbar_wait_warp(s_full, step & 1, abort_flag, err, kErrAttnWait)) {
           ok = false;
           break;
         }
@@ -1158,7 +1162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           softmax_step<DP, T, MOD>(
-              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, w.valid, (float)(w.pos - kbase), w.nslope, m, l,
+              p, s_addr, o_addr, j > 0, kbase + kBK > lim0, w.lim - kbase, (float)(w.pos - kbase), w.nslope, m, l,
               []() { return true; },
               [&]() {
                 if (lane == 0) mbar_arrive(p_half);
@@ -1182,7 +1186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (nt > 0) {
-        if (!mbar_wait(o_full, pieces & 1, abort_flag, err, kErrAttnWait)) break;
+        if (!mbar_wait_warp(o_full, pieces & 1, abort_flag, err, kErrAttnWait)) break;
         ++pieces;
         tc_fence_after();
       }

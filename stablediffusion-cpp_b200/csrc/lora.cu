@@ -288,8 +288,8 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
   float* sums = reinterpret_cast<float*>(smem);  // [TN][128] after the MMAs: features side by side, for reads of whole lines
   __shared__ uint64_t full[C_::STAGES], empty[C_::STAGES], acc_full, list_full;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, ids[kMaxRowsSmall], list[kMaxRowsSmall], in_warp[4], mixed;
-  volatile int* abort_flag = &abort_word;
+  __shared__ int abort_words[kAbortWords(2 + kSumThreads / 32)], ids[kMaxRowsSmall], list[kMaxRowsSmall], in_warp[4], mixed;
+  volatile int* abort_flag = abort_words;
   const LoraLinear& p = g.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = g.splits;
   const int rank = blockIdx.x % splits, blocks = (int)((p.T + kMaxRowsSmall - 1) / kMaxRowsSmall);
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
     }
     mbar_init(&acc_full, 1);
     mbar_init(&list_full, 1);
-    abort_word = 0;
+    for (int& w : abort_words) w = 0;
     mixed = 0;
     fence_mbar_init();
   }
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
       bool ok = true;
       const uint32_t smem0 = smem_u32(smem), full0 = smem_u32(&full[0]);
       auto stage = [&](int bytes) {
-        ok = mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, p.err, kErrWaitEmpty);
+        ok = mbar_wait_warp(&empty[at.slot], at.phase ^ 1u, abort_flag, p.err, kErrWaitEmpty);
         if (ok) {
           mbar_expect_tx_elect(full0 + (uint32_t)(at.slot * 8), (uint32_t)bytes);
           ++done;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
         tma_load_2d_elect(st + C_::W_BYTES, &tmX, full0 + (uint32_t)(at.slot * 8), kb * 64, row0);
       }
       if (ok && g.rk.rc > 0) {
-        ok = mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull);
+        ok = mbar_wait_warp(&list_full, 0, abort_flag, p.err, kErrWaitFull);
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int nq = ok ? my_chunks() : 0;
         for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(C_::STAGES)) {
@@ -371,17 +371,17 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
       const uint64_t ad0 = sdesc_k_sw128(smem_u32(smem)), bd0 = sdesc_k_sw128(smem_u32(smem) + C_::W_BYTES);
       const uint32_t empty0 = smem_u32(&empty[0]);
       for (int kb = kb0; kb < kb1; ++kb, at.next(C_::STAGES)) {
-        ok = mbar_wait(&full[at.slot], at.phase, abort_flag, p.err, kErrWaitFull);
+        ok = mbar_wait_warp(&full[at.slot], at.phase, abort_flag, p.err, kErrWaitFull);
         if (!ok) break;
         tc_fence_after();
         const uint64_t off = (uint64_t)(at.slot * (C_::STAGE >> 4));
         umma4_elect(tmem, ad0 + off, bd0 + off, IDESC, kb > kb0, empty0 + 8 * at.slot);
       }
-      if (ok && g.rk.rc > 0 && mbar_wait(&list_full, 0, abort_flag, p.err, kErrWaitFull)) {
+      if (ok && g.rk.rc > 0 && mbar_wait_warp(&list_full, 0, abort_flag, p.err, kErrWaitFull)) {
         const int nq = my_chunks();
         for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(C_::STAGES)) {
           const int s = at.slot;
-          if (!mbar_wait(&full[s], at.phase, abort_flag, p.err, kErrWaitFull)) break;
+          if (!mbar_wait_warp(&full[s], at.phase, abort_flag, p.err, kErrWaitFull)) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::W_BYTES;
           for (int i = 0; i < min(per_stage, nq - q0); ++i)
@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(64 + kSumThreads, 2)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int q = warp & 3;  // TMEM lane quarter
-    if (warp < 6 && mbar_wait(&acc_full, 0, abort_flag, p.err, kErrWaitAccFull)) {
+    if (warp < 6 && mbar_wait_warp(&acc_full, 0, abort_flag, p.err, kErrWaitAccFull)) {
+      __syncwarp();
       tc_fence_after();
       const bool any = kb1 > kb0 || (g.rk.rc > 0 && my_chunks() > 0);
       float* mine = sums + q * 32 + lane;
@@ -772,24 +773,14 @@ __global__ void __launch_bounds__(kGroup) k_lora_lists(const LoraLinear p, const
   }
 }
 
-// Waits (bounded) until *flag, counted up by other CTAs of this launch, reaches want.
 __device__ __forceinline__ int ld_acquire(const int* p) {
   int v;
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+// Waits (bounded, a whole warp) until *flag, counted up by other CTAs of this launch, reaches want.
 __device__ __forceinline__ bool wait_count(const int* flag, int want, volatile int* abort_flag, int* err) {
-  if (ld_acquire(flag) >= want) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    if (ld_acquire(flag) >= want) return true;
-    if (*abort_flag) return false;
-    if (globaltimer_ns() - t0 > kWaitLimitNs) {
-      *abort_flag = 1;
-      atomicOr(err, kErrWaitFull);
-      return false;
-    }
-  }
+  return wait_warp([&]() { return ld_acquire(flag) >= want; }, abort_flag, err, kErrWaitFull);
 }
 
 // The elements of one 32-column chunk of a warp's rows whose sums are not finite, again
@@ -860,7 +851,7 @@ struct LoraGemmCfg {
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int STG_BYTES = 4 * 2 * 32 * 128;  // two 32 x 32 blocks of Y per epilogue warp
-  static constexpr int FIT = (kMaxSmem - 1024 - STG_BYTES - 2560) / STAGE;  // 2560: barriers, bias
+  static constexpr int FIT = (kMaxSmem - 1024 - STG_BYTES - 512 - 16 * BN) / STAGE;  // barriers, bias
   static constexpr int STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int SMEM = 1024 + STAGES * STAGE + STG_BYTES;
   static constexpr uint32_t COLS = 2 * BN <= 128 ? 128 : 2 * BN <= 256 ? 256 : 512;
@@ -902,9 +893,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drain;
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word, pass_ids[BN / 16];  // adapters of the chunks of a pass
-  __shared__ float4 sbias[2][BN / 4];            // bias of the tile's columns, by accumulator
-  volatile int* abort_flag = &abort_word;
+  __shared__ int abort_words[kAbortWords(kRowThreads / 32)], pass_ids[BN / 16];  // adapters of the chunks of a pass
+  __shared__ float4 sbias[4][BN / 4];            // bias of the tile's columns, one copy an epilogue warp
+  volatile int* abort_flag = abort_words;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
   const int unit = (int)blockIdx.x / CTAS, units = (int)gridDim.x / CTAS;
@@ -922,7 +913,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       mbar_init(&acc_empty[i], 4 * CTAS);
     }
     mbar_init(&drain, 1);
-    abort_word = 0;
+    for (int& w : abort_words) w = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -959,7 +950,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       int done = 0;  // stages filled
       bool ok = true, have_h = false;
       auto stage = [&](int bytes, uint32_t& st) {
-        ok = mbar_wait(&empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrWaitEmpty);
+        ok = mbar_wait_warp(&empty[at.slot], at.phase ^ 1u, abort_flag, err, kErrWaitEmpty);
         if (!ok) return false;
         st = smem0 + (uint32_t)(at.slot * C_::STAGE);
         if (rank == 0) mbar_expect_tx_elect(full_own + (uint32_t)(at.slot * 8), (uint32_t)(CTAS * bytes));
@@ -1065,7 +1056,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         const int count = count_of(mb);
         for (int ps = 0; ps < passes; ++ps, ++n) {
           const int acc = n & 1;
-          ok = mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1u, abort_flag, err, kErrWaitAccEmpty);
+          ok = mbar_wait_warp(&acc_empty[acc], ((n >> 1) & 1) ^ 1u, abort_flag, err, kErrWaitAccEmpty);
           if (!ok) break;
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(acc * BN);
@@ -1074,7 +1065,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           const uint32_t idesc = down ? make_idesc(1u, 0, 0, 128 * CTAS, (uint32_t)N) : IDESC;
           const uint32_t d_step = 4 * N <= BN ? (uint32_t)N : 0;  // four accumulators where they fit
           for (int kb = kb0; kb < kb1; ++kb, at.next(STAGES)) {
-            ok = mbar_wait(&full[at.slot], at.phase, abort_flag, err, kErrWaitFull);
+            ok = mbar_wait_warp(&full[at.slot], at.phase, abort_flag, err, kErrWaitFull);
             if (!ok) break;
             tc_fence_after();
             const uint64_t off = (uint64_t)(at.slot * (C_::STAGE >> 4));
@@ -1088,7 +1079,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
             const int nq = g.lk.chunks(count);
             for (int q0 = 0; q0 < nq; q0 += per_stage, at.next(STAGES)) {
               const int s = at.slot;
-              ok = mbar_wait(&full[s], at.phase, abort_flag, err, kErrWaitFull);
+              ok = mbar_wait_warp(&full[s], at.phase, abort_flag, err, kErrWaitFull);
               if (!ok) break;
               tc_fence_after();
               const uint32_t a0 = smem_u32(smem + s * C_::STAGE), b0 = a0 + C_::A_BYTES;
@@ -1159,7 +1150,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         };
         for (int c0 = 0; c0 < nch; c0 += per_pass, ++n) {
           const int acc = n & 1, used = min(per_pass, nch - c0), N = down_columns<CTAS>(used * cw);
-          ok = mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
+          ok = mbar_wait_warp(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
           if (!ok) break;
           tc_fence_after();
           const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
@@ -1247,14 +1238,17 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       // What the tile needs beside its sums is read before they are complete.
       const int local = (mb * CTAS + (int)rank) * 128 + q * 32 + lane;
       const bool row_ok = local < g.rows, mixed = g.lk.q_max && __ldcg(&list_of(mb)->mixed);
+      // Each warp has a copy of the bias: a warp whose wait expires leaves this loop alone, so none
+      // may wait for another in it.
       if (g.p.bias) {
-        for (int c = threadIdx.x - 64; c < BN; c += 128) {
+        __syncwarp();
+        for (int c = lane; c < BN; c += 32) {
           const int64_t col = (int64_t)nb * BN + c;
-          reinterpret_cast<float*>(sbias[acc])[c] = col < g.p.N ? __ldg(g.p.bias + col) : 0.0f;
+          reinterpret_cast<float*>(sbias[q])[c] = col < g.p.N ? __ldg(g.p.bias + col) : 0.0f;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        __syncwarp();
       }
-      ok = mbar_wait(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
+      ok = mbar_wait_warp(&acc_full[acc], (n >> 1) & 1, abort_flag, err, kErrWaitAccFull);
       if (!ok) break;
       ++n;
       tc_fence_after();
@@ -1285,7 +1279,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           if (g.p.bias) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
-              const float4 b = sbias[acc][(c * 32 + j) / 4];
+              const float4 b = sbias[q][(c * 32 + j) / 4];
               v[j] += b.x;
               v[j + 1] += b.y;
               v[j + 2] += b.z;
@@ -1351,8 +1345,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       release(acc);
     }
     if (lane == 0) tma_store_wait_all();
-    __syncwarp();
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR) cluster_sync();

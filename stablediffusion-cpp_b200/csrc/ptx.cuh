@@ -81,7 +81,7 @@ struct RingPos {
   }
 };
 
-// Waits until the phase with the given parity has completed. Returns false (after
+// Waits (each thread by itself) until the phase with the given parity has completed. Returns false (after
 // recording `code` in *err and raising the CTA abort flag) if the wait exceeds
 // kWaitLimitNs, or if another role of the CTA has already aborted.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
@@ -99,6 +99,51 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       }
     }
   }
+}
+
+// The same for the 32 lanes of a converged warp, which get one answer: what follows may need all of
+// them (elect.sync, votes, tcgen05 loads, barriers), and a lane that gave up by its own clock while
+// others saw the end would leave those waiting for it without a bound. A lane that sees the end
+// goes on at once (a vote on every wait cost up to 5% of a call). One that gives up says so in its
+// warp's count and returns false only when all 32 have: nobody then has gone on. If somebody has,
+// the wait is over and stays so, because no phase ends twice without this warp, and the next poll
+// sees that. `abort` points to the CTA's flag and, behind it, a zeroed count for each warp; no
+// wait of a warp may follow one that was false.
+constexpr int kAbortWords(int warps) { return 1 + warps; }
+template <class Done>
+__device__ __forceinline__ bool give_up_warp(Done done, volatile int* abort) {
+  int* count = const_cast<int*>(abort) + 1 + (threadIdx.x >> 5);
+  atomicAdd(count, 1);
+  for (;;) {
+    int n = *(volatile int*)count;
+    if (n >= 32) return false;
+    if (done())
+      for (;;) {  // back out, unless all had given up before
+        const int was = atomicCAS(count, n, n - 1);
+        if (was == n) return true;
+        if (was >= 32) return false;
+        n = was;
+      }
+  }
+}
+template <class Done>
+__device__ __forceinline__ bool wait_warp(Done done, volatile int* abort, int* err, int code) {
+  if (done()) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (done()) return true;
+    if ((i & 63u) == 0) {
+      const bool late = globaltimer_ns() - t0 > kWaitLimitNs;
+      if (late) {
+        *abort = 1;
+        if (err) atomicOr(err, code);
+      }
+      if (late || *abort) return give_up_warp(done, abort);
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  return wait_warp([&]() { return mbar_try_wait(bar, parity); }, abort, err, code);
 }
 
 // ---------------------------------------------------------------------------------
