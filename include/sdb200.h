@@ -16,13 +16,16 @@
  *   - M <= 0 or N <= 0 is a no-op (backend_cuda.cu:455, :464).
  *   - bf16 values are uint16_t bit patterns: the top 16 bits of an IEEE float
  *     (tensor.h:43-45, :137-142).
- *   - Every op is enqueued on the current device's stream (sdb200_set_stream; default
- *     the legacy default stream) and returns without synchronising, except
+ *   - Every op is enqueued on the calling thread's stream for the current device
+ *     (sdb200_set_stream; default the legacy default stream) and returns without synchronising, except
  *     sdb200_download and sdb200_synchronize.
  *   - Return value: 0 on success, otherwise an SDB200_ERR_* code; the message of the
  *     last failure on the calling thread is returned by sdb200_last_error().
  *   - Thread model: one host thread (or process) per GPU. Calls for one device must
- *     not run concurrently from several threads on the same stream's workspace.
+ *     not run concurrently from several threads on the same stream's workspace: of the
+ *     threads that call for a device at a time, one may use the ops that keep a workspace in
+ *     the library; those whose workspace is the caller's ("several requests at once")
+ *     may run beside them from others, each thread on its own stream.
  */
 #ifndef SDB200_H
 #define SDB200_H
@@ -60,7 +63,8 @@ size_t sdb200_device_memory(void);
  * calling thread's device. */
 int sdb200_set_device(int device);
 /* Extension (the reference uses the default stream only, backend_cuda.cu:10-11):
- * every later op of the current device is issued on `stream` (a cudaStream_t). */
+ * every later op of the calling thread for the current device is issued on `stream` (a
+ * cudaStream_t). A thread that set none uses the last one that any thread set. */
 int sdb200_set_stream(void* stream);
 void* sdb200_get_stream(void);
 /* Synchronises the stream, then reads the device error word that kernels set when a

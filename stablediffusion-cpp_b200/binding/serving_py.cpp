@@ -37,7 +37,7 @@ int (*attention_ragged)(const void*, int64_t, const void*, int64_t, const void*,
                         int64_t, int, const int32_t*, const int32_t*, const int32_t*, const int32_t*, int64_t, int64_t, int,
                         int, int64_t, float, float, const float*, int, const int32_t*, void*, int64_t);
 
-// The stream is the device's, so setting it and the call that uses it go together.
+// One call at a time: the library's first call of a kind sets attributes for all.
 std::mutex call_mutex;
 
 struct Refused {};  // an argument does not fit

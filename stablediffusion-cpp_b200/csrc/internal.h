@@ -36,6 +36,20 @@ enum : int {
   kErrUnsupported = 6,
 };
 
+// The stream a thread's ops of one device are issued on: the thread's own last choice, or for a thread
+// that made none, the last choice of any thread. With one choice for all, a thread could move the
+// launches of another in the middle of a call to its own stream.
+class ThreadStream {
+ public:
+  void bind(int device) { device_ = device; }
+  operator cudaStream_t() const;
+  void operator=(cudaStream_t s);
+
+ private:
+  int device_ = 0;
+  std::atomic<cudaStream_t> latest_{nullptr};
+};
+
 struct DeviceContext {
   // Set (release) once every other field is filled; readers that skip the creation lock
   // load it with acquire before touching the rest.
@@ -45,7 +59,7 @@ struct DeviceContext {
   int cc_major = 0, cc_minor = 0;
   size_t total_mem = 0;
   std::string name;
-  cudaStream_t stream = nullptr;   // stream every op of this device is issued on
+  ThreadStream stream;             // stream the calling thread's ops of this device are issued on
   int* err_word = nullptr;         // device int, OR-ed by kernels on bounded-wait expiry
   // Workspace for operand packing (grown on demand, never shrunk). Ops on one stream
   // run in order, so one workspace per context is safe.

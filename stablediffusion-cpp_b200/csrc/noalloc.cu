@@ -132,7 +132,7 @@ void gemm_noalloc(int64_t M, int64_t N, int64_t K, const float* A, int64_t lda, 
   require(dev >= 0 && dev < kNoAllocMaxDevices, "device ordinal out of range");
   NoAllocDevice& d = noalloc_setup(dev);
   DeviceContext* c = ctx_if_created(dev);  // never creates one (that would allocate)
-  cudaStream_t stream = c ? c->stream : nullptr;
+  cudaStream_t stream = c ? static_cast<cudaStream_t>(c->stream) : nullptr;
   const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>((M * std::max<int64_t>(K, N) + 255) / 256,
                                                                             (int64_t)d.num_sms * 16));
   if (K == 0) {

@@ -35,6 +35,23 @@ PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 constexpr int kErrBadIndexWord = 128;  // kErrBadIndex of ptx.cuh
 }  // namespace
 
+namespace {
+struct Choice {
+  cudaStream_t stream;
+  bool made;
+};
+thread_local Choice t_choice[kMaxDevices];
+}  // namespace
+
+ThreadStream::operator cudaStream_t() const {
+  const Choice& c = t_choice[device_];
+  return c.made ? c.stream : latest_.load(std::memory_order_relaxed);
+}
+void ThreadStream::operator=(cudaStream_t s) {
+  t_choice[device_] = Choice{s, true};
+  latest_.store(s, std::memory_order_relaxed);
+}
+
 void fail(int code, const std::string& msg) { throw Error{code, msg}; }
 
 void check_cuda(cudaError_t e, const char* what) {
@@ -64,7 +81,7 @@ static void init_context(DeviceContext& c, int dev) {
   c.name = prop.name;
   check_cuda(cudaMalloc(&c.err_word, sizeof(int)), "cudaMalloc(error word)");
   check_cuda(cudaMemset(c.err_word, 0, sizeof(int)), "cudaMemset(error word)");
-  c.stream = nullptr;
+  c.stream.bind(dev);
   c.device = dev;
 }
 
@@ -354,7 +371,7 @@ int sdb200_set_stream(void* stream) { SDB_GUARD({ ctx().stream = reinterpret_cas
 
 void* sdb200_get_stream(void) {
   try {
-    return reinterpret_cast<void*>(ctx().stream);
+    return static_cast<cudaStream_t>(ctx().stream);
   } catch (...) {
     return nullptr;
   }

@@ -4,8 +4,8 @@
 
 Tensors are CUDA torch tensors used as plain device buffers: fp32 activations
 (torch.float32) and bf16 weights (torch.bfloat16, whose bit pattern is the
-reference's uint16 bf16). Every call goes through libsdb200.so on the current
-device's stream; the wrappers bind that stream to torch's current stream first so
+reference's uint16 bf16). Every call goes through libsdb200.so on the thread's stream
+for the current device; the wrappers bind it to torch's current stream first so
 CUDA events recorded by torch order correctly with the library's kernels.
 """
 from __future__ import annotations
