@@ -177,31 +177,30 @@ __device__ __forceinline__ void heads_of(const QkNormRope& p, const TI* x, TO* y
       for (int o = 1 << lg >> 1; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       const float rstd = rsqrtf(fmaf(s, inv_d, p.eps));
       const float2 r2 = make_float2(rstd, rstd);
-      // Channels that are not rotated leave their partner out: 0 times an infinity there is NaN.
-      auto finish = [&](auto turn) {
+      // A channel that is not rotated has B = 0, but 0 times an infinity in its partner is NaN: it leaves
+      // the partner out, by a choice between values. (Branches took 12.75 instead of 12.4 us a call for
+      // 2397 tokens of 40 heads, 6.1 instead of 5.2 us for 976 of 60 heads of 40.)
+      float2 r[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float2 o = INTER ? make_float2(v[e].y, v[e].x) : v[(e + VE / 2) % VE];
+        r[e] = fmul2(v[e], A[e]);
+        if (cos) r[e] = ffma2(o, B[e], r[e]);
+        r[e] = fmul2(r2, r[e]);
+      }
+      if (on && h < n) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float f[VE];
 #pragma unroll
           for (int i = 0; i < VE / 2; ++i) {
-            const int e = k * VE / 2 + i;
-            const float2 o = INTER ? make_float2(v[e].y, v[e].x) : v[(e + VE / 2) % VE];
-            float2 r = fmul2(v[e], A[e]);
-            if constexpr (decltype(turn)::value) r = ffma2(o, B[e], r);
-            r = fmul2(r2, r);
-            f[2 * i] = r.x;
-            f[2 * i + 1] = r.y;
+            f[2 * i] = r[k * VE / 2 + i].x;
+            f[2 * i + 1] = r[k * VE / 2 + i].y;
           }
           Chunk<TO, VE> out;
           out.set(f);
           out.store(y + (int64_t)h * p.d + (k ? c1 : c0));
         }
-      };
-      if (on && h < n) {
-        if (cos)
-          finish(std::true_type{});
-        else
-          finish(std::false_type{});
       }
     }
   }
