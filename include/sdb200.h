@@ -24,8 +24,8 @@
  *   - Thread model: one host thread (or process) per GPU. Calls for one device must
  *     not run concurrently from several threads on the same stream's workspace: of the
  *     threads that call for a device at a time, one may use the ops that keep a workspace in
- *     the library; those whose workspace is the caller's ("several requests at once")
- *     may run beside them from others, each thread on its own stream.
+ *     the library, and one, on a stream of its own, those whose workspace is the caller's
+ *     ("several requests at once").
  */
 #ifndef SDB200_H
 #define SDB200_H
@@ -275,8 +275,15 @@ int sdb200_linear_lora(int64_t T, int64_t N, int64_t K, const void* X, int64_t l
  * (out_type), heads d <= 256 wide, out apart from the inputs. max_q / max_kv bound the lengths;
  * sequences may share key rows, not query rows. scale, cap, scale / cap and cap / scale are normal
  * fp32 numbers, with a factor of 1000 to spare.
- * What a mask hides does not reach the result, whatever it holds; rows of no sequence are
- * left as they were. ws: at least sdb200_attention_ragged_workspace() bytes. */
+ * What a mask hides does not reach the result, whatever it holds: finite keys and values change no
+ * bit of it. Where hidden values are infinities or NaN, rows are computed again without them, within the
+ * same roundings. Rows of no sequence are left as they were. P = softmax is rounded to in_type for the
+ * product with v (fp16: to 2^-36 of the row's largest where that is more).
+ * Heads of up to 128 channels, a multiple of 8, in rows on 16-byte boundaries run on the tensor
+ * core; all others take a plain kernel, a warp to a row, that is some hundred times slower for prompts.
+ * With max_q <= 128 / (heads / kv_heads) every sequence is one tile, and long caches are cut over all
+ * processors; a larger max_q, one that no sequence reaches included, gives that up.
+ * ws: at least sdb200_attention_ragged_workspace() bytes. */
 int64_t sdb200_attention_ragged_workspace(int n_seq, int64_t max_q, int64_t max_kv, int heads, int kv_heads,
                                           int64_t d);
 int sdb200_attention_ragged(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,

@@ -494,8 +494,7 @@ __device__ __noinline__ void redo_rows(const TcParams& p, const Seq& q, const Ro
   }
 }
 
-// O of one row from TMEM to out (normalised), or to a piece with m and l. all: no key of the
-// tile range but seen or zeroed ones entered the sum, so nothing needs redo_rows.
+// O of one row from TMEM to out (normalised), or to a piece with m and l.
 template <int DP, class T>
 __device__ __forceinline__ void finish_rows(const TcParams& p, const Seq& q, const Row& w, uint32_t o_addr, bool have_o,
                                             float m, float l, int j0, int j1, float* piece, int r) {
@@ -728,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1 || warp == 2) {
       // ------------------------------ MMA issuers -------------------------------
-      // The whole warp runs the loop (it zeroes the last V tile's tail); lane 0 issues.
+      // The whole warp runs the loop (it zeroes the last V tile's tail); an elected lane issues.
       const int t = warp - 1, nt = t ? nB : nA;
       if (nt > 0 || (t == 0 && two)) {
         bool ok = mbar_wait_warp(q_full, 0, abort_flag, err, kErrAttnWait);

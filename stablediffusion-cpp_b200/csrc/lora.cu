@@ -691,7 +691,7 @@ void launch_rows(LoraRows g) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = adapters ? 2 : 1;  // only k_lora_down_rows may be overtaken
+  cfg.numAttrs = adapters ? 2 : 1;  // only k_lora_down_rows or k_lora_down_runs may be overtaken
   check_cuda(cudaLaunchKernelEx(&cfg, k_lora_rows<TN>, tw, tx, tb, th, (const LoraRows)g), "linear_lora");
   check_launch("linear_lora");
 }
@@ -1361,7 +1361,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 }
 
 template <int BN, bool PAIR>
-void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) {
+void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool adapters) {
   const int64_t r = g.p.r;
   using C_ = LoraGemmCfg<BN, PAIR>;
   DeviceContext& c = ctx();
@@ -1374,7 +1374,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
   // Units that would wait for H take part in making it: up to 8 K splits of 2 blocks at least.
   const int units = c.num_sms / (PAIR ? 2 : 1);
   g.lk.ksplit = std::max(1, std::min({8, units / g.m_tiles, g.k_blocks / 2}));
-  if (overlap) {
+  if (adapters) {
     const int64_t groups = (g.rows + kGroup - 1) / kGroup;
     map_2d(&th, g.lk.H, g.lk.cw, groups * g.lk.q_max * kGroup, g.lk.cw, g.lk.cw, 128, swizzle_of(g.lk.cw));
     map_adapters(&tb, g.B, r, g.p.N, g.p.n_adapters, g.ldb, g.lk.cw, C_::B_ROWS, swizzle_of(g.lk.cw));
@@ -1415,7 +1415,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
     if (fit <= 0) fail(kErrUnsupported, "linear_lora: no cluster of 2 fits");
     clusters[c.device] = fit;
   }
-  if (overlap) {
+  if (adapters) {
     // Units wait for H that others make, so all must be resident: two such launches at once,
     // each with a part of the processors, would wait for each other's. (Starting beside
     // k_lora_lists as well would save under 1 us, but the profiler fails on such a launch.)
@@ -1424,7 +1424,7 @@ void launch_lora_gemm(LoraGemm g, const uint16_t* A, int64_t lda, bool overlap) 
     ++n;
   }
   cfg.numAttrs = n;
-  const int64_t items = (int64_t)g.m_tiles * (g.n_tiles + (overlap ? g.lk.ksplit : 0));
+  const int64_t items = (int64_t)g.m_tiles * (g.n_tiles + (adapters ? g.lk.ksplit : 0));
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(clusters[c.device], items) * (PAIR ? 2 : 1)));
   check_cuda(cudaLaunchKernelEx(&cfg, kern, tx, tw, th, tb, ta, ty, g), "linear_lora");
   check_launch("linear_lora");

@@ -364,7 +364,9 @@ def attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, s
     Query i stands at position i + kv_len - q_len; causal hides later keys except the first
     prefix[s]; cap > 0 turns a score z into cap tanh(z / cap); slopes [heads] subtract
     slope * distance. scale defaults to 1 / sqrt(d). Returns out [Tq, heads, d] in out_dtype
-    (bf16 or fp16, default as q); rows of no sequence keep what out held (zeros without out)."""
+    (bf16 or fp16, default as q); rows of no sequence keep what out held (zeros without out).
+    Fast for d <= 128, a multiple of 8, in aligned rows; single tokens over long caches want the
+    least max_q that holds."""
     r = (_calls or _serving()).attention_ragged(q, k, v, q_begin, q_len, kv_begin, kv_len, max_q, max_kv, scale, causal,
                                                 prefix, cap, slopes, out_dtype, out)
     if r is not None and r.__class__ is not int:
