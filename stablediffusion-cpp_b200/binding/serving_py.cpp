@@ -92,6 +92,7 @@ int64_t row_pitch(const Tensor& t) {
 }
 int64_t stack_pitch(const Tensor& t) {
   const int64_t n = t.size(0), rows = t.size(1), cols = t.size(2);
+  if (t.numel() == 0) return cols;
   const int64_t ld = rows > 1 ? t.stride(1) : n > 1 ? t.stride(0) : cols;
   want((t.stride(2) == 1 || cols <= 1) && (n <= 1 || t.stride(0) == rows * ld));
   return ld;

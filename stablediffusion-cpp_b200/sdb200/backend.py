@@ -290,7 +290,7 @@ def _refuse_stacks(op, **tensors):
         n, rows, cols = t.shape
         s0, s1, s2 = t.stride()
         ld = s1 if rows > 1 else s0 if n > 1 else cols
-        if (s2 != 1 and cols > 1) or (n > 1 and s0 != rows * ld):
+        if t.numel() and ((s2 != 1 and cols > 1) or (n > 1 and s0 != rows * ld)):
             raise ValueError(f"{op}: the adapters of {name} must follow one another in rows of one pitch")
 
 
